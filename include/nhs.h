@@ -446,6 +446,88 @@ int nhs_prefill_attention(const void* q, int64_t q_seq_stride, int64_t q_head_st
                           void* stream);
 
 /*
+ * Verifying drafted tokens. A request's draft is a tree of up to
+ * NHS_MAX_TREE_NODES nodes, each node's parent before it; node t's parent is
+ * parents[b, t], -1 for a node that follows the request's history directly,
+ * anything else outside [0, t) for an absent node. These have no counterpart
+ * in the reference, whose decode step takes one token per request.
+ *
+ * nhs_tree_plan: mask[b, t] has the bits of node t and of its ancestors (0
+ * for an absent node and whatever hangs below one), positions[b, t] =
+ * lengths[b] + the node's depth (0 for those). parents rows are
+ * parents_stride elements apart; mask and positions are [batch, nodes].
+ */
+#define NHS_MAX_TREE_NODES 64
+#define NHS_MAX_TREE_HEAD_DIM 256
+int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parents, int64_t parents_stride,
+                  const int64_t* lengths, int64_t* mask, int64_t* positions, void* stream);
+
+/*
+ * nhs_tree_attention: for request b, node t and query head h, with KV head
+ * h / (q_heads / kv_heads),
+ *   out[b, t, h] = softmax_x(q[b, t, h] . K[x] * head_dim^-0.5) . V[x]
+ * over the pool rows rows[b, c] in [0, pool_rows) (others are masked) and the
+ * drafted nodes j whose bit mask[b, t] holds (k[b, j], v[b, j], not in the
+ * pool). A node with mask word 0 yields zeros, and the keys and values of a
+ * node with mask word 0, like those that a mask hides, may hold anything.
+ * One dtype for all tensors; strides in elements, dims of a head contiguous;
+ * fp32 sums, one rounding of the output. head_dim up to
+ * NHS_MAX_TREE_HEAD_DIM, nodes up to NHS_MAX_TREE_NODES. pool_block_stride as in nhs_attend_rows. The workspace
+ * (nhs_tree_attention_workspace_bytes, 16-byte aligned, may be NULL where that is 0) holds
+ * anything before and after a call.
+ */
+int64_t nhs_tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t n_rows, int32_t q_heads,
+                                           int32_t kv_heads, int32_t head_dim);
+int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_node_stride, int64_t q_head_stride,
+                       const void* k, int64_t k_batch_stride, int64_t k_node_stride, int64_t k_head_stride,
+                       const void* v, int64_t v_batch_stride, int64_t v_node_stride, int64_t v_head_stride,
+                       const int64_t* mask, int64_t mask_batch_stride, int32_t dtype, const void* pool,
+                       int64_t pool_rows, int64_t pool_block_stride, const int64_t* rows, int64_t rows_batch_stride,
+                       int64_t rows_col_stride, int32_t batch, int32_t nodes, int32_t n_rows, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, void* out, int64_t out_batch_stride,
+                       int64_t out_node_stride, int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/*
+ * Per-head RMSNorm of queries and keys and their rotary embedding in one
+ * pass, fp32 with one rounding: for each row's head x of head_dim elements,
+ * y = x * rsqrt(mean(x^2) + eps) * weight (q_weight or k_weight, [head_dim]
+ * in dtype), then with c = cos[p, d], s = sin[p, d] for d < head_dim / 2 and
+ * the row's position p, out[d] = y[d] c - y[d + head_dim/2] s and
+ * out[d + head_dim/2] = y[d + head_dim/2] c + y[d] s. cos and sin are
+ * [table_rows, head_dim / 2] in dtype or fp32 (table_dtype); p is
+ * positions[row], clamped to the tables, or the row's index where positions is
+ * NULL. Strides in elements, dims of a head contiguous; an output may be its
+ * input (same address and strides), and overlaps nothing else.
+ */
+int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t dtype, const void* q,
+                     int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
+                     int64_t k_head_stride, const void* q_weight, const void* k_weight, float eps, const void* cos,
+                     const void* sin, int32_t table_dtype, int64_t table_rows, const int64_t* positions, void* q_out,
+                     int64_t qo_row_stride, int64_t qo_head_stride, void* k_out, int64_t ko_row_stride,
+                     int64_t ko_head_stride, void* stream);
+
+/*
+ * Log probabilities from logits [rows, vocab] (rows row_stride elements
+ * apart), in fp32: logprobs[r, g] = log softmax(logits[r])[tokens[r, g]] for
+ * g < tokens_per_row (-inf for a token outside [0, vocab)), entropy[r] =
+ * -sum p log p, and the `top` (<= NHS_MAX_TOP_LOGPROBS, <= vocab) largest
+ * logits of each row, equal ones by ascending index, a NaN above every
+ * number: top_ids and top_logprobs [rows, top]. A row that holds a NaN or
+ * +inf, or nothing above -inf, has no distribution: its log probabilities
+ * and entropy are NaN. The workspace
+ * (nhs_token_logprobs_workspace_bytes, 16-byte aligned, may be NULL where that is 0) holds
+ * anything before and after a call. No counterpart in the reference, which takes the argmax of its logits
+ * (engine.py:68-74).
+ */
+#define NHS_MAX_TOP_LOGPROBS 64
+int64_t nhs_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype, int32_t top);
+int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, int32_t rows, int32_t vocab,
+                       const int64_t* tokens, int64_t tokens_stride, int32_t tokens_per_row, int32_t top,
+                       float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/*
  * Legacy per-head selections: out[h, c] = columns[h, c] in [0, n) ?
  * shared_rows[columns[h, c]] : -1 for h < heads, c < width.
  * Replaces the head_columns branch of resolve_rows,

@@ -251,6 +251,65 @@ __global__ void silu_mul_kernel(const typename T::Bits* gu, typename T::Bits* ou
   out[idx] = T::from_float(s * u);
 }
 
+// Per-head RMSNorm of q and k and their rotation, in fp32 with one rounding
+// at the end: y = x * rsqrt(mean(x^2) + eps) * weight over a head's dims,
+// then (y[d], y[d + D/2]) rotated by the cos/sin row of the token's
+// position. A row's heads are q's, then k's.
+struct NormRopeArgs {
+  const char* q;
+  const char* k;
+  char* q_out;
+  char* k_out;
+  int64_t q_r, q_h, k_r, k_h, qo_r, qo_h, ko_r, ko_h;  // element strides
+  const char* q_weight;
+  const char* k_weight;
+  const char* cos;
+  const char* sin;
+  int64_t table_rows;
+  const int64_t* positions;  // null: row r's is r
+  int rows, q_heads, heads, half;
+  float eps;
+};
+
+__device__ __forceinline__ int64_t table_row(const NormRopeArgs& a, int64_t row) {
+  const int64_t at = a.positions ? a.positions[row] : row;
+  return min(max(at, (int64_t)0), a.table_rows - 1);
+}
+
+// Any even head_dim, stride and element type (of the tables: TT): one wave per (row, head).
+template <typename T, typename TT>
+__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(NormRopeArgs a) {
+  const int64_t item = (int64_t)blockIdx.x * (kRopeThreads / kWave) + (threadIdx.x >> 6);
+  if (item >= (int64_t)a.rows * a.heads) return;
+  const int lane = threadIdx.x & 63, half = a.half;
+  const int64_t row = item / a.heads;
+  int head = (int)(item - row * a.heads);
+  const bool is_k = head >= a.q_heads;
+  if (is_k) head -= a.q_heads;
+  const auto* x = reinterpret_cast<const typename T::Bits*>(is_k ? a.k : a.q) +
+                  (is_k ? row * a.k_r + head * a.k_h : row * a.q_r + head * a.q_h);
+  auto* y = reinterpret_cast<typename T::Bits*>(is_k ? a.k_out : a.q_out) +
+            (is_k ? row * a.ko_r + head * a.ko_h : row * a.qo_r + head * a.qo_h);
+  const auto* w = reinterpret_cast<const typename T::Bits*>(is_k ? a.k_weight : a.q_weight);
+  const int64_t at = table_row(a, row) * half;
+  const auto* cos = reinterpret_cast<const typename TT::Bits*>(a.cos) + at;
+  const auto* sin = reinterpret_cast<const typename TT::Bits*>(a.sin) + at;
+  float acc = 0.f;
+  for (int d = lane; d < 2 * half; d += kWave) {
+    const float v = T::to_float(x[d]);
+    acc = __builtin_fmaf(v, v, acc);
+  }
+  const float r = rsqrtf(group_sum(acc, kWave) / (float)(2 * half) + a.eps);
+  // a lane reads both halves of a pair before it writes them: the outputs may be the inputs
+  for (int d = lane; d < half; d += kWave) {
+    const float lo = T::to_float(x[d]) * r * T::to_float(w[d]);
+    const float hi = T::to_float(x[d + half]) * r * T::to_float(w[d + half]);
+    const float c = TT::to_float(cos[d]), s = TT::to_float(sin[d]);
+    y[d] = T::from_float(lo * c - hi * s);
+    y[d + half] = T::from_float(hi * c + lo * s);
+  }
+}
+
 // What a decode step reads by index, in one launch: x[b] = embed[ids[b]], cos_out[b] =
 // cos[positions[b]], sin_out[b] = sin[positions[b]], as 16-byte chunks
 // (blockIdx.y: the item). Indices are clamped to their table. Bound by its
@@ -373,6 +432,55 @@ extern "C" int nhs_rope(int32_t rows, int32_t heads, int32_t head_dim, int32_t d
     launch(rope_kernel<F32T>, grid, block, 0, s, ev.start, ev.stop, static_cast<float*>(t), row_stride, heads, half,
            static_cast<const float*>(cos), static_cast<const float*>(sin), total);
   return launch_status("nhs_rope");
+}
+
+extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t dtype,
+                                const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+                                int64_t k_row_stride, int64_t k_head_stride, const void* q_weight,
+                                const void* k_weight, float eps, const void* cos, const void* sin,
+                                int32_t table_dtype, int64_t table_rows, const int64_t* positions, void* q_out,
+                                int64_t qo_row_stride, int64_t qo_head_stride, void* k_out, int64_t ko_row_stride,
+                                int64_t ko_head_stride, void* stream) {
+  const LaunchEvents ev = take_launch_events();
+  const char* who = "nhs_qk_norm_rope";
+  if (rows < 0 || q_heads < 1 || k_heads < 1 || q_heads > 65536 || k_heads > 65536 || head_dim < 2 || head_dim % 2 ||
+      !valid_dtype(dtype) || (table_dtype != dtype && table_dtype != NHS_F32))
+    return fail(NHS_ERR_INVALID, "%s: bad shape/dtype", who);
+  if (rows == 0) return NHS_OK;
+  if (!q || !k || !q_weight || !k_weight || !cos || !sin || !q_out || !k_out)
+    return fail(NHS_ERR_INVALID, "%s: null pointer", who);
+  if (table_rows < 1 || (!positions && table_rows < rows))
+    return fail(NHS_ERR_INVALID, "%s: a cos/sin row for every token required", who);
+  const int esize = elem_size(dtype);
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight | (uintptr_t)k_weight) %
+          esize || ((uintptr_t)cos | (uintptr_t)sin) % elem_size(table_dtype) || (uintptr_t)positions % 8)
+    return fail(NHS_ERR_INVALID, "%s: misaligned pointer", who);
+  NormRopeArgs a;
+  a.q = static_cast<const char*>(q), a.k = static_cast<const char*>(k);
+  a.q_out = static_cast<char*>(q_out), a.k_out = static_cast<char*>(k_out);
+  a.q_r = q_row_stride, a.q_h = q_head_stride, a.k_r = k_row_stride, a.k_h = k_head_stride;
+  a.qo_r = qo_row_stride, a.qo_h = qo_head_stride, a.ko_r = ko_row_stride, a.ko_h = ko_head_stride;
+  a.q_weight = static_cast<const char*>(q_weight), a.k_weight = static_cast<const char*>(k_weight);
+  a.cos = static_cast<const char*>(cos), a.sin = static_cast<const char*>(sin);
+  a.table_rows = table_rows, a.positions = positions;
+  a.rows = rows, a.q_heads = q_heads, a.heads = q_heads + k_heads, a.half = head_dim / 2, a.eps = eps;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t items = (int64_t)rows * a.heads, blocks = (items + kRopeThreads / kWave - 1) / (kRopeThreads / kWave);
+  if (blocks > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  const auto run = [&](auto kernel) {
+    launch(kernel, dim3((unsigned)blocks), dim3(kRopeThreads), 0, s, ev.start, ev.stop, a);
+  };
+  if (dtype == NHS_F32)
+    run(qk_norm_rope_kernel<F32T, F32T>);
+  else if (dtype == NHS_BF16 && table_dtype == NHS_BF16)
+    run(qk_norm_rope_kernel<BF16T, BF16T>);
+  else if (dtype == NHS_BF16)
+    run(qk_norm_rope_kernel<BF16T, F32T>);
+  else if (table_dtype == NHS_F16)
+    run(qk_norm_rope_kernel<F16T, F16T>);
+  else
+    run(qk_norm_rope_kernel<F16T, F32T>);
+  return launch_status(who);
 }
 
 extern "C" int nhs_silu_mul(int32_t rows, int32_t inter, int32_t dtype, const void* gate_up, void* out,

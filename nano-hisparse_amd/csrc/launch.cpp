@@ -16,6 +16,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -149,6 +150,27 @@ PyObject* native(Py_ssize_t nargs, Py_ssize_t wanted, F body) {
   } catch (const std::exception&) {
   }
   Py_RETURN_NONE;
+}
+
+PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+  PyObject* result = PyTuple_New((Py_ssize_t)tensors.size());
+  if (!result) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& t : tensors) {
+    PyObject* item;
+    if (t.defined()) {
+      item = THPVariable_Wrap(t);
+    } else {
+      item = Py_None;
+      Py_INCREF(item);
+    }
+    if (!item) {
+      Py_DECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, i++, item);
+  }
+  return result;
 }
 
 // ---- decode linear layers -----------------------------------------------------------------
@@ -340,6 +362,182 @@ PyObject* prefill_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
+// ---- drafted tokens ---------------------------------------------------------------------------
+
+// Makes t's device current for the launches that follow, as row_kernels._on does.
+struct OnDevice {
+  c10::DeviceGuard guard;
+  explicit OnDevice(const Tensor& t) : guard(t.device()) {}
+};
+
+// A caller's output: a strided tensor whose heads are contiguous and whose elements are distinct (or Skip).
+void check_out(const Tensor& out, const Tensor& like) {
+  on_gpu(out, like.dim(), like);
+  need(same_sizes(out, like.sizes()) && out.scalar_type() == like.scalar_type() && out.stride(-1) == 1);
+  for (int64_t d = 0; d < out.dim(); ++d) need(out.stride(d) != 0 || out.size(d) == 1);
+}
+
+// Scratch memory of a call (nothing for 0 bytes): on the current stream's allocator, freed with the tensor.
+Tensor scratch(int64_t bytes, const Tensor& like) { return bytes ? make({bytes}, like, at::kByte) : Tensor(); }
+void* scratch_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+PyObject* tree_plan(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 2, [&]() -> PyObject* {
+    const Tensor &parents = tensor(a[0]), &lengths = tensor(a[1]);
+    on_gpu(parents, 2);
+    on_gpu(lengths, 1, parents);
+    const int64_t B = parents.size(0), T = parents.size(1);
+    need(parents.scalar_type() == at::kInt && parents.stride(1) == 1 && lengths.scalar_type() == at::kLong &&
+         lengths.size(0) == B && lengths.is_contiguous() && T <= NHS_MAX_TREE_NODES);
+    Tensor mask, positions;
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(parents);
+      mask = make({B, T}, parents, at::kLong);
+      positions = make({B, T}, parents, at::kLong);
+      st = nhs_tree_plan((int32_t)B, (int32_t)T, static_cast<const int32_t*>(parents.data_ptr()), parents.stride(0),
+                         static_cast<const int64_t*>(lengths.data_ptr()), static_cast<int64_t*>(mask.data_ptr()),
+                         static_cast<int64_t*>(positions.data_ptr()), stream_of(parents));
+    }
+    return st ? failed("nhs_tree_plan", st) : tuple_of({mask, positions});
+  });
+}
+
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 8, [&]() -> PyObject* {
+    const Tensor &q = tensor(a[0]), &pool = tensor(a[1]), &rows = tensor(a[2]), &k = tensor(a[3]), &v = tensor(a[4]),
+                 &mask = tensor(a[5]);
+    on_gpu(q, 4);
+    on_gpu(pool, 5, q);
+    on_gpu(rows, 2, q);
+    on_gpu(k, 4, q);
+    on_gpu(v, 4, q);
+    on_gpu(mask, 2, q);
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = pool.size(3), N = rows.size(1);
+    const int32_t P = integer32(a[6]);
+    const int code = dtype_code(q);
+    need(same_sizes(v, k.sizes()) && k.size(0) == B && k.size(1) == T && k.size(2) == Hkv && k.size(3) == D &&
+         pool.size(2) == P && pool.size(4) == D && Hq % Hkv == 0 && pool.scalar_type() == q.scalar_type() &&
+         k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && rows.size(0) == B &&
+         rows.scalar_type() == at::kLong && mask.size(0) == B && mask.size(1) == T && mask.stride(1) == 1 &&
+         mask.scalar_type() == at::kLong && q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1 &&
+         T <= NHS_MAX_TREE_NODES && D <= NHS_MAX_TREE_HEAD_DIM && pool.size(0) * P < (int64_t(1) << 31));
+    const int64_t stride = pool_block_stride(pool);
+    Tensor out;
+    if (a[7] != Py_None) {
+      out = tensor(a[7]);
+      check_out(out, q);
+    }
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(q);
+      if (!out.defined()) out = make(q.sizes(), q, q.scalar_type());
+      const int64_t bytes = nhs_tree_attention_workspace_bytes((int32_t)B, (int32_t)T, (int32_t)N, (int32_t)Hq,
+                                                               (int32_t)Hkv, (int32_t)D);
+      const Tensor ws = scratch(bytes, q);
+      st = nhs_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k.data_ptr(), k.stride(0),
+                              k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2),
+                              static_cast<const int64_t*>(mask.data_ptr()), mask.stride(0), code, pool.data_ptr(),
+                              pool.size(0) * P, stride, static_cast<const int64_t*>(rows.data_ptr()), rows.stride(0),
+                              rows.stride(1), (int32_t)B, (int32_t)T, (int32_t)N, (int32_t)Hq, (int32_t)Hkv,
+                              (int32_t)D, P, out.data_ptr(), out.stride(0), out.stride(1), out.stride(2),
+                              scratch_ptr(ws), bytes, stream_of(q));
+    }
+    return st ? failed("nhs_tree_attention", st) : THPVariable_Wrap(out);
+  });
+}
+
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 9, [&]() -> PyObject* {
+    const Tensor &q = tensor(a[0]), &k = tensor(a[1]), &qw = tensor(a[2]), &kw = tensor(a[3]), &cos = tensor(a[5]),
+                 &sin = tensor(a[6]);
+    on_gpu(q, 3);
+    on_gpu(k, 3, q);
+    const int64_t n = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+    need(k.size(0) == n && k.size(2) == D && k.scalar_type() == q.scalar_type() && D % 2 == 0 && q.stride(2) == 1 &&
+         k.stride(2) == 1);
+    for (const Tensor* w : {&qw, &kw}) {
+      on_gpu(*w, 1, q);
+      need(w->size(0) == D && w->scalar_type() == q.scalar_type() && w->is_contiguous());
+    }
+    for (const Tensor* t : {&cos, &sin}) {
+      on_gpu(*t, 2, q);
+      need(t->size(1) == D / 2 && t->is_contiguous());
+    }
+    need(same_sizes(sin, cos.sizes()) && sin.scalar_type() == cos.scalar_type() &&
+         (cos.scalar_type() == q.scalar_type() || cos.scalar_type() == at::kFloat));
+    need(PyFloat_CheckExact(a[4]));
+    const float eps = (float)PyFloat_AS_DOUBLE(a[4]);
+    const int64_t* positions = nullptr;
+    if (a[7] != Py_None) {
+      const Tensor& p = tensor(a[7]);
+      on_gpu(p, 1, q);
+      need(p.size(0) == n && p.scalar_type() == at::kLong && p.is_contiguous());
+      positions = static_cast<const int64_t*>(p.data_ptr());
+    } else {
+      need(cos.size(0) >= n);
+    }
+    const int code = dtype_code(q), table_code = dtype_code(cos);
+    Tensor q_out, k_out;
+    if (a[8] != Py_None) {
+      need(PyTuple_CheckExact(a[8]) && PyTuple_GET_SIZE(a[8]) == 2);
+      q_out = tensor(PyTuple_GET_ITEM(a[8], 0));
+      k_out = tensor(PyTuple_GET_ITEM(a[8], 1));
+      check_out(q_out, q);
+      check_out(k_out, k);
+    }
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(q);
+      if (!q_out.defined()) {
+        q_out = make(q.sizes(), q, q.scalar_type());
+        k_out = make(k.sizes(), k, k.scalar_type());
+      }
+      st = nhs_qk_norm_rope((int32_t)n, (int32_t)Hq, (int32_t)Hkv, (int32_t)D, code, q.data_ptr(), q.stride(0),
+                            q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), qw.data_ptr(), kw.data_ptr(), eps,
+                            cos.data_ptr(), sin.data_ptr(), table_code, cos.size(0), positions, q_out.data_ptr(),
+                            q_out.stride(0), q_out.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1),
+                            stream_of(q));
+    }
+    return st ? failed("nhs_qk_norm_rope", st) : tuple_of({q_out, k_out});
+  });
+}
+
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 3, [&]() -> PyObject* {
+    const Tensor &logits = tensor(a[0]), &tokens = tensor(a[1]);
+    on_gpu(logits, 2);
+    need(tokens.dim() == 1 || tokens.dim() == 2);
+    on_gpu(tokens, tokens.dim(), logits);
+    const int64_t R = logits.size(0), V = logits.size(1), per_row = tokens.dim() == 2 ? tokens.size(1) : 1;
+    const int32_t top = integer32(a[2]);
+    const int code = dtype_code(logits);
+    need(logits.stride(1) == 1 && tokens.size(0) == R && tokens.scalar_type() == at::kLong && tokens.is_contiguous() &&
+         top >= 0 && top <= NHS_MAX_TOP_LOGPROBS && top <= V);
+    Tensor logprobs, entropy, ids, values;
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(logits);
+      logprobs = make(tokens.sizes(), logits, at::kFloat);
+      entropy = make({R}, logits, at::kFloat);
+      ids = make({R, top}, logits, at::kLong);
+      values = make({R, top}, logits, at::kFloat);
+      const int64_t bytes = nhs_token_logprobs_workspace_bytes((int32_t)R, (int32_t)V, code, top);
+      const Tensor ws = scratch(bytes, logits);
+      st = nhs_token_logprobs(logits.data_ptr(), logits.stride(0), code, (int32_t)R, (int32_t)V,
+                              static_cast<const int64_t*>(tokens.data_ptr()), per_row, (int32_t)per_row, top,
+                              static_cast<float*>(logprobs.data_ptr()), static_cast<float*>(entropy.data_ptr()),
+                              static_cast<int64_t*>(ids.data_ptr()), static_cast<float*>(values.data_ptr()),
+                              scratch_ptr(ws), bytes, stream_of(logits));
+    }
+    return st ? failed("nhs_token_logprobs", st) : tuple_of({logprobs, entropy, ids, values});
+  });
+}
+
 // ---- selection --------------------------------------------------------------------------------
 
 struct Selection {
@@ -349,27 +547,6 @@ struct Selection {
     positions = make({B, top * P}, like, at::kInt);
   }
 };
-
-PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
-  PyObject* result = PyTuple_New((Py_ssize_t)tensors.size());
-  if (!result) return nullptr;
-  Py_ssize_t i = 0;
-  for (const Tensor& t : tensors) {
-    PyObject* item;
-    if (t.defined()) {
-      item = THPVariable_Wrap(t);
-    } else {
-      item = Py_None;
-      Py_INCREF(item);
-    }
-    if (!item) {
-      Py_DECREF(result);
-      return nullptr;
-    }
-    PyTuple_SET_ITEM(result, i++, item);
-  }
-  return result;
-}
 
 PyObject* quest_batched(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return native(nargs, 8, [&]() -> PyObject* {
@@ -543,7 +720,8 @@ PyObject* held_state(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 PyMethodDef methods[] = {NHS_METHOD(linear_small_m), NHS_METHOD(linear_silu_mul),   NHS_METHOD(linear_rope),
                          NHS_METHOD(add_rmsnorm),    NHS_METHOD(attend_batched),    NHS_METHOD(prefill_attention),
                          NHS_METHOD(quest_batched),  NHS_METHOD(select_resolve_batched),
-                         NHS_METHOD(append_page),    NHS_METHOD(held_state),
+                         NHS_METHOD(append_page),    NHS_METHOD(held_state),        NHS_METHOD(tree_plan),
+                         NHS_METHOD(tree_attention), NHS_METHOD(qk_norm_rope),      NHS_METHOD(token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

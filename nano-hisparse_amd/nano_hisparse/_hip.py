@@ -88,6 +88,21 @@ SIGNATURES = {
         [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _p],
         ctypes.c_int,
     ),
+    "nhs_tree_plan": ([_i32, _i32, _p, _i64, _p, _p, _p, _p], ctypes.c_int),
+    "nhs_tree_attention_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32], ctypes.c_int64),
+    "nhs_tree_attention": (
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i32, _p, _i64, _i64, _p, _i64,
+         _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _i64, _p, _i64, _p],
+        ctypes.c_int,
+    ),
+    "nhs_qk_norm_rope": (
+        [_i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _p, ctypes.c_float, _p, _p, _i32, _i64, _p,
+         _p, _i64, _i64, _p, _i64, _i64, _p],
+        ctypes.c_int,
+    ),
+    "nhs_token_logprobs_workspace_bytes": ([_i32, _i32, _i32, _i32], ctypes.c_int64),
+    "nhs_token_logprobs": (
+        [_p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _i32, _p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
     "nhs_expand_columns": ([_p, _i64, _p, _i64, _i64, _p, _p], ctypes.c_int),
 }
 

@@ -11,7 +11,9 @@ provider explicitly (set_cpu_provider); the library never installs one.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
@@ -89,6 +91,23 @@ def _require_gpu(what, *tensors):
         if t is not None and t.device != device:
             raise ValueError(f"{what}: all tensors must be on {device}")
     return device
+
+
+def _on(device):
+    """Makes `device` current for a launch, where it is not (a launch on a
+    stream of another device is an error)."""
+    if _device_index(device) == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_out(who, out, shape, dtype, device):
+    """An output of the caller's: its shape, dtype and device, dims of a head
+    contiguous, no element twice."""
+    if out.shape != shape or out.dtype != dtype or out.device != device:
+        raise ValueError(f"{who}: out must be {list(shape)} {dtype} on {device}")
+    if out.numel() and (out.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape))):
+        raise ValueError(f"{who}: out's head dims must be contiguous and its elements distinct")
 
 
 def timing_events():
@@ -853,3 +872,198 @@ def linear_rope(x, weight, bias, rope_heads, head_dim, cos, sin):
                                  out.stride(0), _stream(device))
     _hip.check(status, "nhs_linear_rope")
     return out
+
+
+# ---- drafted tokens --------------------------------------------------------------------------
+
+MAX_TREE_NODES = 64  # of a request's tree of drafted tokens: one bit of a mask word each
+MAX_TREE_HEAD_DIM = 256
+MAX_TOP_LOGPROBS = 64
+
+
+def tree_plan(parents, lengths):
+    """Ancestor masks and positions of a batch of token trees: parents
+    [B, T <= 64] int32, each node's parent before it (-1: the node follows
+    the request's history; anything else outside [0, t) marks node t absent,
+    and nodes below an absent one are absent too); lengths [B] int64, the
+    histories' lengths. Returns (mask, positions), int64 [B, T]: mask[b, t]
+    has the bits of node t and its ancestors, positions[b, t] is
+    lengths[b] + the node's depth; both are 0 for an absent node."""
+    if parents.is_cuda:
+        done = (_launch or _load_launch()).tree_plan(parents, lengths)
+        if done is not None:
+            return done
+    device = _require_gpu("tree_plan", parents, lengths)
+    if parents.ndim != 2 or parents.dtype != torch.int32 or lengths.dtype != torch.int64 \
+            or lengths.shape != parents.shape[:1]:
+        raise ValueError("tree_plan: parents [B, T] int32, lengths [B] int64")
+    B, T = parents.shape
+    if T > MAX_TREE_NODES:
+        raise ValueError(f"tree_plan: at most {MAX_TREE_NODES} nodes")
+    if parents.stride(1) != 1:
+        parents = parents.contiguous()
+    lengths = lengths.contiguous()
+    mask = torch.empty(B, T, dtype=torch.int64, device=device)
+    positions = torch.empty_like(mask)
+    if mask.numel():
+        with _on(device):
+            status = _hip.load().nhs_tree_plan(B, T, _ptr(parents), parents.stride(0), _ptr(lengths), _ptr(mask),
+                                               _ptr(positions), _stream(device))
+        _hip.check(status, "nhs_tree_plan")
+    return mask, positions
+
+
+def tree_attention(query, pool, rows, k, v, mask, page_size, out=None):
+    """Attention of drafted nodes: query [B, T <= 64, Hq, D] over the pool
+    rows rows [B, N] (int64, shared by a request's nodes and heads; rows
+    outside the pool, such as -1, are masked) and over the drafted keys and
+    values k, v [B, T, Hkv, D] whose bits mask [B, T] (int64, as tree_plan
+    makes it) holds. Returns [B, T, Hq, D]; a node with mask 0 yields zeros.
+    One dtype (bf16, fp16 or fp32) for all, D up to 256."""
+    if query.is_cuda:
+        done = (_launch or _load_launch()).tree_attention(query, pool, rows, k, v, mask, page_size, out)
+        if done is not None:
+            return done
+    device = _require_gpu("tree_attention", query, pool, rows, k, v, mask)
+    if query.ndim != 4 or pool.ndim != 5 or k.ndim != 4 or k.shape != v.shape or k.shape[:2] != query.shape[:2]:
+        raise ValueError("tree_attention: query [B, T, Hq, D], pool [blocks, 2, P, Hkv, D], k and v [B, T, Hkv, D]")
+    B, T, Hq, D = query.shape
+    Hkv = pool.shape[3]
+    if pool.shape[1] != 2 or pool.shape[2] != page_size or pool.shape[4] != D or k.shape[2:] != (Hkv, D) \
+            or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("tree_attention: query/pool/draft head shape mismatch")
+    if not query.dtype == pool.dtype == k.dtype == v.dtype:
+        raise ValueError("tree_attention: query, pool, k and v must have one dtype")
+    code = dtype_code(query.dtype)
+    if rows.ndim != 2 or rows.shape[0] != B or rows.dtype != torch.int64:
+        raise ValueError("tree_attention: rows [B, N] int64")
+    if mask.shape != (B, T) or mask.dtype != torch.int64:
+        raise ValueError("tree_attention: mask [B, T] int64")
+    if T > MAX_TREE_NODES or D > MAX_TREE_HEAD_DIM:
+        raise ValueError(f"tree_attention: at most {MAX_TREE_NODES} nodes and heads of {MAX_TREE_HEAD_DIM}")
+    if any(t.stride(3) != 1 for t in (query, k, v)):
+        raise ValueError("tree_attention: head dims must be contiguous")
+    stride = pool_block_stride(pool)
+    if pool.shape[0] * page_size >= 2**31:
+        raise ValueError("tree_attention: pool rows must be < 2^31")
+    if mask.stride(1) != 1:
+        mask = mask.contiguous()
+    if out is None:
+        out = torch.empty(B, T, Hq, D, dtype=query.dtype, device=device)
+    else:
+        _check_out("tree_attention", out, query.shape, query.dtype, device)
+    if out.numel() == 0:
+        return out
+    N = rows.shape[1] if pool.shape[0] else 0
+    lib = _hip.load()
+    need = lib.nhs_tree_attention_workspace_bytes(B, T, N, Hq, Hkv, D)
+    with _on(device):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        status = lib.nhs_tree_attention(
+            _ptr(query), *query.stride()[:3], _ptr(k), *k.stride()[:3], _ptr(v), *v.stride()[:3], _ptr(mask),
+            mask.stride(0), code, _ptr(pool), pool.shape[0] * page_size, stride, _ptr(rows), rows.stride(0),
+            rows.stride(1), B, T, N, Hq, Hkv, D, page_size, _ptr(out), *out.stride()[:3], _ptr(workspace), need,
+            _stream(device),
+        )
+    _hip.check(status, "nhs_tree_attention")
+    return out
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, eps, cos, sin, positions=None, out=None):
+    """Per-head RMSNorm of q [n, Hq, D] and k [n, Hkv, D] (times q_weight /
+    k_weight [D]) and their rotary embedding, one pass, fp32 with one
+    rounding. cos/sin [rows, D/2] in q's dtype or float32; row r's position
+    is positions[r] (int64 [n], clamped to the tables) or r. Returns new
+    (q, k), or writes to `out`, a pair that may be (q, k) itself."""
+    if q.is_cuda:
+        done = (_launch or _load_launch()).qk_norm_rope(q, k, q_weight, k_weight, float(eps), cos, sin, positions, out)
+        if done is not None:
+            return done
+    device = _require_gpu("qk_norm_rope", q, k, q_weight, k_weight, cos, sin, positions)
+    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+        raise ValueError("qk_norm_rope: q [n, Hq, D] and k [n, Hkv, D] of one dtype")
+    n, Hq, D = q.shape
+    code = dtype_code(q.dtype)
+    if D < 2 or D % 2 or Hq < 1 or k.shape[1] < 1:
+        raise ValueError("qk_norm_rope: heads of an even number of dims")
+    if any(w.shape != (D,) or w.dtype != q.dtype or not w.is_contiguous() for w in (q_weight, k_weight)):
+        raise ValueError("qk_norm_rope: weights must be contiguous [D] of q's dtype")
+    if cos.ndim != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.dtype != sin.dtype \
+            or cos.dtype not in (q.dtype, torch.float32) or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("qk_norm_rope: cos/sin must be contiguous [rows, D/2] in q's dtype or float32")
+    if positions is not None and (positions.shape != (n,) or positions.dtype != torch.int64):
+        raise ValueError("qk_norm_rope: positions must be int64 [n]")
+    if n and (cos.shape[0] < 1 or (positions is None and cos.shape[0] < n)):
+        raise ValueError("qk_norm_rope: cos/sin need a row for every token")
+    if q.stride(2) != 1 or k.stride(2) != 1:
+        raise ValueError("qk_norm_rope: head dims must be contiguous")
+    if out is None:
+        outs = (torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device))
+    else:
+        outs = tuple(out)
+        if len(outs) != 2:
+            raise ValueError("qk_norm_rope: out is a pair (q, k)")
+        for t, o in zip((q, k), outs):
+            _check_out("qk_norm_rope", o, t.shape, t.dtype, device)
+    if n == 0:
+        return outs
+    if positions is not None:
+        positions = positions.contiguous()
+    with _on(device):
+        status = _hip.load().nhs_qk_norm_rope(
+            n, Hq, k.shape[1], D, code, _ptr(q), *q.stride()[:2], _ptr(k), *k.stride()[:2], _ptr(q_weight),
+            _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), dtype_code(cos.dtype), cos.shape[0], _ptr(positions),
+            _ptr(outs[0]), *outs[0].stride()[:2], _ptr(outs[1]), *outs[1].stride()[:2], _stream(device),
+        )
+    _hip.check(status, "nhs_qk_norm_rope")
+    return outs
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns, on the logits' device."""
+
+    logprobs: torch.Tensor  # float32, the tokens' shape
+    entropy: torch.Tensor  # float32 [rows], natural logarithm
+    top_ids: torch.Tensor  # int64 [rows, top], most likely first
+    top_logprobs: torch.Tensor  # float32 [rows, top]
+
+
+def token_logprobs(logits, tokens, top=0):
+    """Log probabilities of tokens (int64 [rows], or [rows, n] for several per
+    row) under logits [rows, vocab] (bf16, fp16 or fp32), the entropy of every
+    row and its `top` <= 64 most likely tokens (equal logits by ascending
+    id), in fp32. A token outside the vocabulary has log probability -inf; a
+    row with a NaN or +inf, or with nothing above -inf, yields NaN."""
+    if logits.is_cuda:
+        done = (_launch or _load_launch()).token_logprobs(logits, tokens, top)
+        if done is not None:
+            return TokenLogprobs(*done)
+    device = _require_gpu("token_logprobs", logits, tokens)
+    if logits.ndim != 2 or tokens.ndim not in (1, 2) or tokens.shape[0] != logits.shape[0] \
+            or tokens.dtype != torch.int64:
+        raise ValueError("token_logprobs: logits [rows, vocab], tokens int64 [rows] or [rows, n]")
+    code, top = dtype_code(logits.dtype), int(top)
+    R, V = logits.shape
+    if V < 1 or not 0 <= top <= min(MAX_TOP_LOGPROBS, V):
+        raise ValueError(f"token_logprobs: top must be 0 to {MAX_TOP_LOGPROBS}, and no more than the vocabulary")
+    if logits.stride(1) != 1 and V > 1:
+        raise ValueError("token_logprobs: rows of logits must be contiguous")
+    tokens = tokens.contiguous()
+    result = TokenLogprobs(torch.empty(tokens.shape, dtype=torch.float32, device=device),
+                           torch.empty(R, dtype=torch.float32, device=device),
+                           torch.empty(R, top, dtype=torch.int64, device=device),
+                           torch.empty(R, top, dtype=torch.float32, device=device))
+    if R == 0:
+        return result
+    per_row = tokens.shape[1] if tokens.ndim == 2 else 1
+    lib = _hip.load()
+    need = lib.nhs_token_logprobs_workspace_bytes(R, V, code, top)
+    with _on(device):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        status = lib.nhs_token_logprobs(
+            _ptr(logits), logits.stride(0), code, R, V, _ptr(tokens), per_row, per_row, top, _ptr(result.logprobs),
+            _ptr(result.entropy), _ptr(result.top_ids), _ptr(result.top_logprobs), _ptr(workspace), need,
+            _stream(device),
+        )
+    _hip.check(status, "nhs_token_logprobs")
+    return result
