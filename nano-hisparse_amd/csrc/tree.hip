@@ -4,8 +4,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
-#include "nhs_common.h"
+#include "flash_common.h"
 
 namespace nhs {
 
@@ -62,7 +63,7 @@ struct TreeArgs {
   const int64_t* rows;
   int64_t r_b, r_c;
   int n_rows, rows_per_split, n_splits;
-  int nodes, q_heads, kv_heads, group, head_dim, page_size;
+  int batch, nodes, q_heads, kv_heads, group, head_dim, page_size;
   int query_rows, row_blocks;  // nodes * group, and blocks of them
   FastDiv group_div, page_div;
   float scale_log2;  // D^-1/2 * log2(e)
@@ -203,6 +204,322 @@ __global__ __launch_bounds__(kTgThreads) void tree_general_kernel(TreeArgs a) {
     if (sub + 16 * i < D) store_elem(a.out, T::dtype, at + sub + 16 * i, some ? acc[i] / l : 0.f);
 }
 
+// ---- 16-bit heads of 64 and 128 on the matrix cores ----
+
+// rows whose addresses are in LDS at a time: with four waves of queries half as many, so that two workgroups share a CU
+constexpr int tf_stage(int qw) { return qw == 4 ? 1024 : 2048; }
+__device__ __attribute__((aligned(256))) char tree_zeros[256];  // read in place of a masked row
+
+// QW waves hold 32 query rows each; KW such sets share the keys (KW tiles of
+// BN keys a round). The layouts are those of prefill_attention_kernel:
+// S^T = K Q^T and O^T = V^T P^T, tiles straight from global memory to LDS.
+//
+// Every row of a tile has an address of its own, so a stage of up to 2048 rows
+// (tf_stage) is turned into addresses in LDS first (a masked row's is that of zeros, and
+// its bit of the tile's word is clear); the loads of a round then need one LDS
+// read each. The drafted keys are a last round of the last split. A masked
+// weight is 0, which a matrix core would multiply with whatever V holds, so
+// what a mask hides must be finite: masked rows and absent nodes read zeros,
+// and NaN and infinities of drafted values are taken out of the tile, then
+// added to the outputs of the nodes that see them.
+//
+// With QW = 1 a wave loads and reads its own tiles only and no barrier stands
+// in the loop.
+template <typename T, int D, int QW, int KW, int BN>
+__global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a) {
+  constexpr int W = QW * KW, THREADS = W * kWave;
+  constexpr int KS = D / 16, DB = D / 32, C = D / 8, NB = BN / 32;
+  constexpr int kRows = 1024 / (D * 2);        // of a load instruction
+  constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
+  constexpr int kTile = BN * D * 2;            // bytes
+  constexpr int kRound = BN * KW;              // keys
+  constexpr int kTfStage = tf_stage(QW);
+  constexpr unsigned kDraft = T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;  // exponent bits of NaN and infinities
+  static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1, "tile shape");
+  __shared__ __attribute__((aligned(16))) char k0[KW * kTile], k1[KW * kTile];
+  __shared__ __attribute__((aligned(16))) char v0[KW * kTile], v1[KW * kTile];
+  __shared__ __attribute__((aligned(16))) int64_t stage[kTfStage];
+  __shared__ uint32_t words[kTfStage / 32];
+  __shared__ int odd;  // the draft's values hold a NaN or an infinity
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = wave_id % QW, share = wave_id / QW;
+  const int half = lane >> 5, n = lane & 31;
+  // The items of one (request, KV head) and split are a multiple of the items apart: on one XCD where they are a
+  // multiple of 8, so that the blocks of query rows read the keys from one L2.
+  const int items = a.batch * a.kv_heads;
+  const int bk = blockIdx.x % items, rest = blockIdx.x / items;
+  const int block = rest % a.row_blocks, split = rest / a.row_blocks;
+  const int b = bk / a.kv_heads, kv = bk - b * a.kv_heads;
+
+  const int r = (block * QW + wave) * 32 + n;  // this lane's query row (column of S^T)
+  const bool live = r < a.query_rows;
+  const int rr = min(r, a.query_rows - 1);
+  const int node = (int)a.group_div.div((uint32_t)rr), head = kv * a.group + rr - node * a.group;
+  const int64_t* mask = a.mask + (int64_t)b * a.mask_b;
+  const uint64_t word = live ? (uint64_t)mask[node] : 0;
+  uint4 qf[KS];
+  {
+    const char* qp = a.q + ((int64_t)b * a.q_b + (int64_t)node * a.q_n + (int64_t)head * a.q_h) * 2 + half * 16;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 32);
+  }
+  float m = -INFINITY, l = 0.f;  // running max (of the unscaled scores) and this lane's share of the denominator
+  pf_f32x16 o[DB];
+#pragma unroll
+  for (int x = 0; x < DB; ++x)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[x][i] = 0.f;
+
+  const int lrow = lane / C, lchunk = lane % C;
+  const int k_row = n * (D * 2);
+  const int j4 = (lane & 15) >> 2;
+  int v_at[DB];
+#pragma unroll
+  for (int x = 0; x < DB; ++x)
+    v_at[x] = (4 * half + j4) * (D * 2) +
+              pf_v_slot<D>(j4, x * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+
+  const int64_t head_bytes = (int64_t)kv * D * 2, plane = a.plane_bytes;
+  const int64_t zeros = (int64_t)tree_zeros;
+  auto load_tile = [&](int t, char* kb, char* vb) {  // this share's tile of the stage's round t
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int row = (i * QW + wave) * kRows + lrow;
+      const int64_t at = stage[t * kRound + share * BN + row];
+      const int dst = share * kTile + (i * QW + wave) * 1024;
+      const char* ks = (const char*)at + pf_k_slot<D>(row, lchunk) * 16;
+      const char* vs = (const char*)(at == zeros ? at : at + plane) + pf_v_slot<D>(row, lchunk) * 16;
+      pf_load_lds(ks, kb + dst);
+      pf_load_lds(vs, vb + dst);
+    }
+  };
+  // the tile in (kb, vb), of which the lane's query sees the keys of `seen` (bit = key of the tile)
+  auto tile = [&](const char* kb, const char* vb, const uint32_t (&seen)[NB]) {
+    const char* kl = kb + share * kTile + k_row;
+    const char* vl = vb + share * kTile;
+    pf_f32x16 s[NB];
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+#pragma unroll
+    for (int st = 0; st < KS; ++st)
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        const uint4 kf = *reinterpret_cast<const uint4*>(kl + x * 32 * D * 2 + pf_k_slot<D>(n, 2 * st + half) * 16);
+        s[x] = mfma32x32x16<T>(kf, qf[st], s[x]);
+      }
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+      if (__any(seen[x] != 0xffffffffu)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(seen[x] >> ((i >> 2) * 8 + half * 4 + (i & 3)) & 1)) s[x][i] = -INFINITY;
+      }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m)) {
+      const float moved = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - (moved == -INFINITY ? 0.f : moved)) * a.scale_log2);
+      m = moved;
+      l *= alpha;
+#pragma unroll
+      for (int x = 0; x < DB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[x][i] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
+    uint4 pb[2 * NB];
+    float tile_sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float e0 = s[j >> 1][(j & 1) * 8 + 2 * x], e1 = s[j >> 1][(j & 1) * 8 + 2 * x + 1];
+        w[x] = pf_pack<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(e0, a.scale_log2, -ref)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(e1, a.scale_log2, -ref)));
+        tile_sum = pf_add_pair<T>(w[x], tile_sum);
+      }
+      pb[j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    l += tile_sum;
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j)
+#pragma unroll
+      for (int x = 0; x < DB; ++x) {
+        const uint2 lo = pf_read_tr(vl + v_at[x] + (16 * j) * (D * 2));
+        const uint2 hi = pf_read_tr(vl + v_at[x] + (16 * j + 8) * (D * 2));
+        o[x] = mfma32x32x16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[j], o[x]);
+      }
+  };
+
+  const int begin = split * a.rows_per_split, end = min(a.n_rows, begin + a.rows_per_split);
+  const int64_t* rows = a.rows + (int64_t)b * a.r_b;
+  for (int s0 = begin; s0 < end; s0 += kTfStage) {
+    const int count = min(kTfStage, end - s0), rounds = (count + kRound - 1) / kRound;
+    if (s0 != begin) __syncthreads();  // the last stage's addresses and tiles are read
+    for (int i = tid; i < rounds * kRound; i += THREADS) {
+      const int64_t at = i < count ? rows[(int64_t)(s0 + i) * a.r_c] : -1;
+      const bool ok = at >= 0 && at < a.pool_rows;
+      const uint32_t page = a.page_div.div((uint32_t)at);
+      const int64_t in_page = (uint32_t)at - page * (uint32_t)a.page_size;
+      stage[i] = ok ? (int64_t)a.pool + page * a.block_stride + in_page * a.row_bytes + head_bytes : zeros;
+      const uint64_t live_rows = __ballot(ok);  // of this wave's 64 consecutive rows
+      if (lane == 0) {
+        words[i / 32] = (uint32_t)live_rows;
+        words[i / 32 + 1] = (uint32_t)(live_rows >> 32);
+      }
+    }
+    __syncthreads();
+    auto round = [&](int t, char* kb, char* vb, char* kb_next, char* vb_next) {
+      // this wave's loads of round t are in; after the barrier every wave's are, and every wave is done with the other
+      // buffers, which take round t + 1
+      if constexpr (QW > 1) {
+        __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
+        __syncthreads();
+      } else {  // the wave's reads of the other buffers are back too
+        __builtin_amdgcn_s_waitcnt(kPfVmcnt0 & kPfLgkmcnt0);
+        asm volatile("" ::: "memory");
+      }
+      if (t + 1 < rounds) load_tile(t + 1, kb_next, vb_next);
+      uint32_t seen[NB];
+      bool some = false;
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        seen[x] = __builtin_amdgcn_readfirstlane(words[(t * kRound + share * BN) / 32 + x]);
+        some |= seen[x] != 0;
+      }
+      if (some) tile(kb, vb, seen);
+    };
+    load_tile(0, k0, v0);
+    for (int t = 0; t < rounds; t += 2) {
+      round(t, k0, v0, k1, v1);
+      if (t + 1 < rounds) round(t + 1, k1, v1, k0, v0);
+    }
+  }
+
+  uint64_t present = 0;  // drafted nodes
+  if (split == a.n_splits - 1) {  // the drafted keys, as they lie: node j of the round is key j
+    __syncthreads();
+    present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
+    if (tid == 0) odd = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int row = (i * QW + wave) * kRows + lrow, j = share * BN + row;
+      const bool ok = j < a.nodes && (present >> j & 1);
+      const int dst = share * kTile + (i * QW + wave) * 1024;
+      const char* ks = ok ? a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2 : tree_zeros;
+      const char* vs = ok ? a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 : tree_zeros;
+      pf_load_lds(ks + pf_k_slot<D>(row, lchunk) * 16, k0 + dst);
+      pf_load_lds(vs + pf_v_slot<D>(row, lchunk) * 16, v0 + dst);
+    }
+    __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
+    __syncthreads();
+    for (int c = tid; c < min(a.nodes, kRound) * C; c += THREADS) {
+      uint4* p = reinterpret_cast<uint4*>(v0) + c;  // rows lie one after another, shares too
+      uint32_t w[4] = {p->x, p->y, p->z, p->w};
+      bool found = false;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const bool lo = (w[x] & kDraft) == kDraft, hi = (w[x] >> 16 & kDraft) == kDraft;
+        found |= lo || hi;
+        w[x] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+      }
+      if (found) {
+        *p = make_uint4(w[0], w[1], w[2], w[3]);
+        odd = 1;
+      }
+    }
+    __syncthreads();
+    if (share * BN < a.nodes) {
+      uint32_t seen[NB];
+#pragma unroll
+      for (int x = 0; x < NB; ++x) seen[x] = (uint32_t)((word & present) >> (share * BN + 32 * x));
+      tile(k0, v0, seen);
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  if constexpr (KW > 1) {
+    // the waves of the other shares hand their sums over through the tile buffers, one share at a time (registers by
+    // lane: the partners hold the same query rows and dims)
+    float* part = reinterpret_cast<float*>(wave < (QW + 1) / 2 ? k0 : v0) +
+                  (wave < (QW + 1) / 2 ? wave : wave - (QW + 1) / 2) * (DB * 16 * kWave) + lane;
+    float* stat = reinterpret_cast<float*>(stage) + wave * 2 * kWave + lane;
+    static_assert((QW + 1) / 2 * DB * 16 * kWave * 4 <= KW * kTile && QW * 2 * kWave * 4 <= kTfStage * 8, "merge space");
+    for (int from = 1; from < KW; ++from) {
+      __syncthreads();
+      if (share == from) {
+#pragma unroll
+        for (int x = 0; x < DB; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[(x * 16 + i) * kWave] = o[x][i];
+        stat[0] = m;
+        stat[kWave] = l;
+      }
+      __syncthreads();
+      if (share == 0) {
+        const float m2 = stat[0], l2 = stat[kWave];
+        const float both = fmaxf(m, m2), ref = both == -INFINITY ? 0.f : both;
+        const float f1 = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2);
+        const float f2 = __builtin_amdgcn_exp2f((m2 - ref) * a.scale_log2);
+        m = both;
+        l = l * f1 + l2 * f2;
+#pragma unroll
+        for (int x = 0; x < DB; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[x][i] = o[x][i] * f1 + part[(x * 16 + i) * kWave] * f2;
+      }
+    }
+    if (share) return;
+  }
+  if (!live) return;
+  if (split == a.n_splits - 1 && odd) {
+    for (int j = 0; j < a.nodes; ++j) {
+      if (!((word & present) >> j & 1)) continue;
+      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 + half * 8;
+#pragma unroll
+      for (int x = 0; x < DB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t bits = *reinterpret_cast<const uint16_t*>(vs + x * 64 + (i >> 2) * 16 + (i & 3) * 2);
+          if ((bits & kDraft) == kDraft)
+            o[x][i] += T::dtype == NHS_BF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits);
+        }
+    }
+  }
+  if (a.n_splits > 1) {
+    const int64_t at = (int64_t)split * a.out_rows + ((int64_t)b * a.nodes + node) * a.q_heads + head;
+    if (half == 0) *reinterpret_cast<float2*>(a.stats + 2 * at) = make_float2(m * a.scale_log2, l);
+    float* p = a.partial + at * D + half * 4;
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y)  // dims x*32 + y*8 + half*4 .. +3 of the lane's query row
+        *reinterpret_cast<float4*>(p + x * 32 + y * 8) =
+            make_float4(o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]);
+    return;
+  }
+  const bool some = word != 0 && m != -INFINITY;
+  const float inv = some ? 1.f / l : 0.f;
+  char* op = a.out + ((int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h) * 2 + half * 8;
+#pragma unroll
+  for (int x = 0; x < DB; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const uint32_t w0 = pf_pack<T>(o[x][4 * y] * inv, o[x][4 * y + 1] * inv);
+      const uint32_t w1 = pf_pack<T>(o[x][4 * y + 2] * inv, o[x][4 * y + 3] * inv);
+      *reinterpret_cast<uint2*>(op + x * 64 + y * 16) = some ? make_uint2(w0, w1) : make_uint2(0u, 0u);
+    }
+}
+
 // Joins the splits of every output row, one wave per row: the sums are scaled
 // to the largest of the splits' maxima, added and divided.
 template <typename T>
@@ -231,21 +548,34 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 }
 
 struct TreeShape {
+  int waves, shares;  // of the matrix-core kernel (QW, KW); 0: the general one
   int row_blocks, n_splits, rows_per_split;
 };
 
-// How the rows of a (request, KV head) are split: about 512 workgroups in
-// all, none of less than 64 rows.
-static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int kv_heads) {
+// How a (request, KV head)'s query rows and keys are divided. `flash`: the
+// matrix-core kernel takes the call (16-bit heads of 64 or 128).
+static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim, bool flash) {
   TreeShape s;
-  s.row_blocks = (nodes * (q_heads / kv_heads) + kTgRows - 1) / kTgRows;
+  const int query_rows = nodes * (q_heads / kv_heads);
+  int block_rows = kTgRows, per_cu = 2, least = 64;
+  s.waves = s.shares = 0;
+  if (flash) {
+    s.waves = query_rows <= 32 ? 1 : query_rows <= 64 ? 2 : 4;
+    s.shares = 4 / s.waves;
+    block_rows = 32 * s.waves;
+    per_cu = s.waves == 4 ? 2 : 1;
+    least = 128;
+  }
+  s.row_blocks = (query_rows + block_rows - 1) / block_rows;
   const int64_t items = (int64_t)batch * kv_heads * s.row_blocks;
-  const int64_t wanted = std::max<int64_t>(1, 512 / items), most = std::max(1, n_rows / 64);
+  const int64_t wanted = std::max<int64_t>(1, 256 * per_cu / items), most = std::max(1, n_rows / least);
   s.n_splits = (int)std::min(wanted, most);
-  s.rows_per_split = ((n_rows + s.n_splits - 1) / s.n_splits + 31) / 32 * 32;
-  s.n_splits = std::max(1, (n_rows + std::max(s.rows_per_split, 1) - 1) / std::max(s.rows_per_split, 1));
+  s.rows_per_split = std::max(((n_rows + s.n_splits - 1) / s.n_splits + least - 1) / least * least, 1);
+  s.n_splits = std::max(1, (n_rows + s.rows_per_split - 1) / s.rows_per_split);
   return s;
 }
+
+static bool tree_flash_head(int dtype, int head_dim) { return dtype != NHS_F32 && (head_dim == 64 || head_dim == 128); }
 
 static bool tree_valid(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim) {
   return batch >= 0 && nodes >= 1 && nodes <= kTreeNodes && n_rows >= 0 && q_heads >= 1 && kv_heads >= 1 &&
@@ -271,9 +601,13 @@ extern "C" int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parent
 extern "C" int64_t nhs_tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t n_rows, int32_t q_heads,
                                                       int32_t kv_heads, int32_t head_dim) {
   if (!tree_valid(batch, nodes, n_rows, q_heads, kv_heads, head_dim)) return 0;
-  const TreeShape s = tree_shape(std::max(batch, 1), nodes, n_rows, q_heads, kv_heads);
-  if (s.n_splits == 1) return 0;
-  return (int64_t)s.n_splits * batch * nodes * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+  int splits = 0;  // the most that any kernel makes of the shape: which one runs depends on dtype and alignment too
+  for (const bool flash : {false, true}) {
+    if (flash && !tree_flash_head(NHS_BF16, head_dim)) continue;
+    splits = std::max(splits, tree_shape(std::max(batch, 1), nodes, n_rows, q_heads, kv_heads, head_dim, flash).n_splits);
+  }
+  if (splits == 1) return 0;
+  return (int64_t)splits * batch * nodes * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_node_stride, int64_t q_head_stride,
@@ -303,7 +637,13 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)pool) % esize ||
       ((uintptr_t)mask | (uintptr_t)rows) % 8)
     return fail(NHS_ERR_INVALID, "%s: misaligned pointer", who);
-  const TreeShape shape = tree_shape(batch, nodes, n_rows, q_heads, kv_heads);
+  bool flash = tree_flash_head(dtype, head_dim) && pool_block_stride % 16 == 0 &&
+               ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)pool) % 16 == 0;
+  for (const int64_t stride : {q_batch_stride, q_node_stride, q_head_stride, k_batch_stride, k_node_stride,
+                               k_head_stride, v_batch_stride, v_node_stride, v_head_stride, out_batch_stride,
+                               out_node_stride, out_head_stride})
+    flash = flash && stride % 8 == 0;
+  const TreeShape shape = tree_shape(batch, nodes, n_rows, q_heads, kv_heads, head_dim, flash);
   const int64_t need = nhs_tree_attention_workspace_bytes(batch, nodes, n_rows, q_heads, kv_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(NHS_ERR_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", who, (long long)need);
@@ -322,7 +662,7 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   a.block_stride = pool_block_stride;
   a.rows = rows, a.r_b = rows_batch_stride, a.r_c = rows_col_stride;
   a.n_rows = n_rows, a.rows_per_split = shape.rows_per_split, a.n_splits = shape.n_splits;
-  a.nodes = nodes, a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads;
+  a.batch = batch, a.nodes = nodes, a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads;
   a.head_dim = head_dim, a.page_size = page_size;
   a.query_rows = nodes * a.group, a.row_blocks = shape.row_blocks;
   a.group_div = FastDiv((uint32_t)a.group), a.page_div = FastDiv((uint32_t)page_size);
@@ -334,19 +674,36 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   a.partial = a.stats + 2 * a.out_rows * shape.n_splits;
   hipStream_t s = (hipStream_t)stream;
   const hipEvent_t none = nullptr;
-  auto run = [&](auto kernel, auto join) {
+  const auto run = [&](auto kernel, auto join, int threads) {
     const bool joined = shape.n_splits > 1;
-    launch(kernel, dim3((unsigned)blocks), dim3(kTgThreads), 0, s, ev.start, joined ? none : ev.stop, a);
+    launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, s, ev.start, joined ? none : ev.stop, a);
     if (joined) launch(join, dim3((unsigned)((a.out_rows + 3) / 4)), dim3(256), 0, s, none, ev.stop, a);
   };
   const auto general = [&](auto tag) {
     using T = decltype(tag);
     if (head_dim <= 128)
-      run(tree_general_kernel<T, 32, 128>, tree_join_kernel<T>);
+      run(tree_general_kernel<T, 32, 128>, tree_join_kernel<T>, kTgThreads);
     else
-      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_kernel<T>);
+      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_kernel<T>, kTgThreads);
   };
-  if (dtype == NHS_BF16)
+  const auto on_mfma = [&](auto tag, auto dim) {
+    using T = decltype(tag);
+    constexpr int D = decltype(dim)::value;
+    const int threads = shape.waves * shape.shares * kWave;
+    if (shape.waves == 1)
+      run(tree_flash_kernel<T, D, 1, 4, 32>, tree_join_kernel<T>, threads);
+    else if (shape.waves == 2)
+      run(tree_flash_kernel<T, D, 2, 2, 64>, tree_join_kernel<T>, threads);
+    else
+      run(tree_flash_kernel<T, D, 4, 1, 64>, tree_join_kernel<T>, threads);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (flash && dtype == NHS_BF16)
+    head_dim == 128 ? on_mfma(BF16{}, D128{}) : on_mfma(BF16{}, D64{});
+  else if (flash)
+    head_dim == 128 ? on_mfma(F16{}, D128{}) : on_mfma(F16{}, D64{});
+  else if (dtype == NHS_BF16)
     general(BF16{});
   else if (dtype == NHS_F16)
     general(F16{});
