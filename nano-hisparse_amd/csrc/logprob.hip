@@ -16,8 +16,11 @@
 
 namespace nhs {
 
-constexpr int kLpThreads = 256, kLpMaxTop = NHS_MAX_TOP_LOGPROBS;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave, kLpMaxTop = NHS_MAX_TOP_LOGPROBS;
+constexpr int kLpCandidates = 1024;  // keys held in LDS
+constexpr int kLpMaxSplits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.693147180559945309417;
 
 struct LogprobArgs {
   const char* logits;
@@ -25,10 +28,13 @@ struct LogprobArgs {
   int vocab, top, per_row;
   const int64_t* tokens;
   int64_t tokens_stride;
-  float* logprobs;  // [rows, per_row]
-  float* entropy;   // [rows]
+  float* logprobs;   // [rows, per_row]
+  float* entropy;    // [rows]
   int64_t* top_ids;  // [rows, top]
   float* top_logprobs;
+  int splits, split_chunks;
+  float4* sums;    // splits > 1: [rows, splits] (reference, S, W, unused)
+  uint64_t* keys;  // and [rows, splits, top], 0 where a split has fewer elements
 };
 
 // The order of the alternatives as unsigned keys: larger logit, larger key (-0 equals +0, a NaN is above +inf); the
@@ -42,6 +48,7 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
 __device__ __forceinline__ uint64_t lp_key(float x, int index) {
   return (uint64_t)lp_order(x) << 32 | (uint32_t)~index;
 }
+__device__ __forceinline__ int lp_index(uint64_t key) { return (int)~(uint32_t)key; }
 
 __device__ __forceinline__ uint64_t lp_wave_max(uint64_t key) {
 #pragma unroll
@@ -52,19 +59,253 @@ __device__ __forceinline__ uint64_t lp_wave_max(uint64_t key) {
   return key;
 }
 
-// One workgroup per row: a pass for the maximum and the sums, then a pass per alternative for the largest key below the
-// last one.
+struct LogprobShared {
+  float m[kLpWaves], s[kLpWaves], w[kLpWaves];
+  uint64_t best[2][kLpWaves];
+  uint32_t lane_max[kLpThreads];     // order of the largest logit of each thread, 0 without one
+  int hot[kLpThreads];               // threads whose elements may be among the alternatives
+  int n_hot, n_found, scan[kLpWaves + 1];
+  uint32_t threshold;
+  uint64_t found[kLpCandidates];
+  uint64_t sorted[kLpMaxTop];
+};
+
+// Sums of a row or of a part: S = sum 2^(x log2 e - ref), W = sum 2^(...) (x log2 e - ref).
+struct LpSums {
+  float ref, s, w;
+};
+__device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b) {
+  const float ref = fmaxf(a.ref, b.ref), da = a.ref - ref, db = b.ref - ref;
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  // (below -1e9 the factor is 0: the product must only be finite)
+  return {ref, a.s * fa + b.s * fb,
+          fa * __builtin_fmaf(fmaxf(da, -1e9f), a.s, a.w) + fb * __builtin_fmaf(fmaxf(db, -1e9f), b.s, b.w)};
+}
+
+// The chunks of 16 bytes of a row that lie wholly inside it, and the elements before and after them.
 template <typename T>
-__global__ __launch_bounds__(kLpThreads) void logprob_rows_kernel(LogprobArgs a) {
-  __shared__ float sm[kLpThreads / kWave], ss[kLpThreads / kWave], sw[kLpThreads / kWave];
-  __shared__ uint64_t best[2][kLpThreads / kWave];
-  const int64_t row = blockIdx.x;
+struct LpRow {
+  static constexpr int E = 16 / T::bytes;
+  const char* base;  // the first whole chunk
+  int lead, chunks, vocab;
+  __device__ LpRow(const LogprobArgs& a, int64_t row) : vocab(a.vocab) {
+    const char* p = a.logits + row * a.row_stride * T::bytes;
+    lead = min(vocab, (int)(-(intptr_t)p & 15) / T::bytes);
+    chunks = (vocab - lead) / E;
+    base = p + lead * T::bytes;
+  }
+  __device__ int index(int chunk, int e) const { return lead + chunk * E + e; }
+  __device__ uint4 load(int chunk) const { return *reinterpret_cast<const uint4*>(base + (int64_t)chunk * 16); }
+  __device__ float at(int64_t i) const { return load_elem(base, T::dtype, i - lead); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[E]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (T::dtype == NHS_F32)
+        x[e] = __uint_as_float(w[e]);
+      else if constexpr (T::dtype == NHS_BF16)
+        x[e] = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+      else
+        x[e] = f16_bits_to_f32((e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu);
+    }
+  }
+};
+
+// Chunks [first, last) of a row and, with `lead` / `tail`, the elements around all chunks.
+struct LpPart {
+  int first, last;
+  bool lead, tail;
+};
+
+// The keys of the part's `top` largest elements to sh.sorted, one pass over the part per key.
+template <typename T>
+__device__ void lp_top_by_rounds(const LpRow<T>& row, const LpPart& part, int top, LogprobShared& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t base = row * a.row_stride;
+  const int begin = part.lead ? 0 : row.index(part.first, 0), end = part.tail ? row.vocab : row.index(part.last, 0);
+  uint64_t last = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    uint64_t key = 0;
+    for (int i = begin + tid; i < end; i += kLpThreads) {
+      const uint64_t x = lp_key(row.at(i), i);
+      if (x < last && x > key) key = x;
+    }
+    key = lp_wave_max(key);
+    if (lane == 0) sh.best[k & 1][wave] = key;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kLpWaves; ++i) key = key > sh.best[k & 1][i] ? key : sh.best[k & 1][i];
+    last = key;
+    if (tid == 0) sh.sorted[k] = key;
+  }
+  __syncthreads();
+}
+
+// The `top` largest of sh.found[0 .. n) in descending order to sh.sorted (0 beyond n): every key's place is the number
+// of larger ones.
+__device__ __forceinline__ void lp_sort_found(int n, int top, LogprobShared& sh) {
+  const int tid = threadIdx.x;
+  if (tid < top) sh.sorted[tid] = 0;
+  __syncthreads();
+  constexpr int kMine = kLpCandidates / kLpThreads;
+  uint64_t key[kMine];
+  int place[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = tid + j * kLpThreads;
+    key[j] = i < n ? sh.found[i] : 0;
+    place[j] = 0;
+  }
+  const int mine = (n + kLpThreads - 1) / kLpThreads;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t other = sh.found[i];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      if (j < mine) place[j] += other > key[j];
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; ++j)
+    if (key[j] && place[j] < top) sh.sorted[place[j]] = key[j];
+  __syncthreads();
+}
+
+// The `top` largest elements of the part, given each thread's largest (of chunks first + thread, + kLpThreads, ...):
+// the top-th largest of these is a lower bound, and only the few threads that reach it hold elements that count; their
+// chunks are read again and compared by the whole workgroup. Where more elements equal the bound than LDS holds (masked
+// vocabularies), those above it are kept and the equal ones counted off in index order.
+template <typename T>
+__device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool any, float thread_max,
+                       LogprobShared& sh) {
+  constexpr int E = LpRow<T>::E;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint32_t mine = any ? lp_order(thread_max) : 0u;
+  sh.lane_max[tid] = mine;
+  if (tid == 0) sh.n_hot = sh.n_found = 0;
+  __syncthreads();
+  int place = 0;
+  const uint4* all = reinterpret_cast<const uint4*>(sh.lane_max);
+#pragma unroll 4
+  for (int i = 0; i < kLpThreads / 4; ++i) {
+    const uint4 v = all[i];
+    const int above = tid - 4 * i;  // of equal ones, lower threads come first
+    place += (v.x > mine || (v.x == mine && 0 < above)) + (v.y > mine || (v.y == mine && 1 < above)) +
+             (v.z > mine || (v.z == mine && 2 < above)) + (v.w > mine || (v.w == mine && 3 < above));
+  }
+  if (place == top - 1) sh.threshold = mine;
+  __syncthreads();
+  const uint32_t threshold = sh.threshold;
+  if (mine >= max(threshold, 1u)) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
+  __syncthreads();
+  const int per_thread = (part.last - part.first + kLpThreads - 1) / kLpThreads;
+  const int pairs = sh.n_hot * per_thread;  // at most 256 threads x their chunks: the part
+  // pushes the elements whose order is at least `least`
+  const auto collect = [&](uint32_t least) {
+    const auto push = [&](float x, int i) {
+      if (lp_order(x) >= least) {
+        const int at = atomicAdd(&sh.n_found, 1);
+        if (at < kLpCandidates) sh.found[at] = lp_key(x, i);
+      }
+    };
+    for (int p = tid; p < pairs; p += kLpThreads) {
+      const int chunk = part.first + sh.hot[p / per_thread] + (p % per_thread) * kLpThreads;
+      if (chunk >= part.last) continue;
+      float x[E];
+      LpRow<T>::unpack(row.load(chunk), x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) push(x[e], row.index(chunk, e));
+    }
+    if (part.lead && tid < row.lead) push(row.at(tid), tid);
+    if (part.tail)
+      for (int i = row.index(row.chunks, 0) + tid; i < row.vocab; i += kLpThreads) push(row.at(i), i);
+  };
+  collect(threshold);
+  __syncthreads();
+  if (sh.n_found > kLpCandidates) {
+    __syncthreads();
+    if (tid == 0) sh.n_found = 0;
+    __syncthreads();
+    collect(threshold + 1);
+    __syncthreads();
+    const int above = sh.n_found;
+    if (above > kLpCandidates - kLpMaxTop) {
+      lp_top_by_rounds(row, part, top, sh);
+      return;
+    }
+    // the first elements equal to the threshold, in index order: those before the chunks, chunk by chunk, those behind
+    int left = max(top - above, 0), taken = above;
+    const auto equal = [&](uint32_t bits, int first) {  // bit e: element first + e
+      const int count = __popc(bits);
+      int incl = count;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+      }
+      if (lane == kWave - 1) sh.scan[tid >> 6] = incl;
+      __syncthreads();
+      int before = incl - count, total = 0;
+#pragma unroll
+      for (int w = 0; w < kLpWaves; ++w) {
+        if (w < (tid >> 6)) before += sh.scan[w];
+        total += sh.scan[w];
+      }
+      for (uint32_t b = bits; b && before < left; b &= b - 1, ++before)
+        sh.found[taken + before] = (uint64_t)threshold << 32 | (uint32_t)~(first + __ffs(b) - 1);
+      const int used = min(total, left);
+      taken += used, left -= used;
+      __syncthreads();
+    };
+    if (part.lead) equal(tid < row.lead && lp_order(row.at(tid)) == threshold, tid);
+    for (int c = part.first; c < part.last && left > 0; c += kLpThreads) {
+      uint32_t bits = 0;
+      if (c + tid < part.last) {
+        float x[E];
+        LpRow<T>::unpack(row.load(c + tid), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) bits |= (uint32_t)(lp_order(x[e]) == threshold) << e;
+      }
+      equal(bits, row.index(c + tid, 0));
+    }
+    if (part.tail && left > 0) {  // fewer elements than threads
+      const int i = row.index(row.chunks, 0) + tid;
+      equal(i < row.vocab && lp_order(row.at(i)) == threshold, i);
+    }
+    lp_sort_found(taken, top, sh);
+    return;
+  }
+  lp_sort_found(sh.n_found, top, sh);
+}
+
+// The outputs of a row from its sums and sh.sorted. The sums are those of x * (1 + beta), where kLog2e rounds to
+// log2 e * (1 + beta): to first order lse(x) = lse(x (1 + beta)) - beta * sum p x.
+template <typename T>
+__device__ void lp_finish(const LogprobArgs& a, int64_t r, const LpRow<T>& row, const LpSums& t,
+                          LogprobShared& sh) {
+  constexpr double beta = (double)kLog2e * kLn2 - 1.0;
+  const double bits = (double)log2f(t.s), mean = (double)t.w / (double)t.s;
+  const double lse = ((double)t.ref + bits - beta * (mean + (double)t.ref)) * kLn2;
+  const int tid = threadIdx.x;
+  if (tid == 0) a.entropy[r] = (float)((bits - mean) * kLn2);
+  for (int g = tid; g < a.per_row; g += kLpThreads) {
+    const int64_t token = a.tokens[r * a.tokens_stride + g];
+    const bool known = token >= 0 && token < a.vocab;
+    a.logprobs[r * a.per_row + g] = known ? (float)((double)row.at(known ? token : 0) - lse) : -INFINITY;
+  }
+  if (tid < a.top) {
+    const int i = lp_index(sh.sorted[tid]);
+    a.top_ids[r * a.top + tid] = i;
+    a.top_logprobs[r * a.top + tid] = (float)((double)row.at(i) - lse);
+  }
+}
+
+// A row whose sums overflow or vanish in the form above (a NaN, +inf, nothing above -inf, logits beyond 1e38): the
+// formulas as they stand, one pass per step.
+template <typename T>
+__device__ void lp_unusual_row(const LogprobArgs& a, int64_t r, const LpRow<T>& row, LogprobShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float m = -INFINITY;
   bool nan = false;
   for (int i = tid; i < a.vocab; i += kLpThreads) {
-    const float x = load_elem(a.logits, T::dtype, base + i);
+    const float x = row.at(i);
     nan |= x != x;
     m = fmaxf(m, x);
   }
@@ -74,49 +315,175 @@ __global__ __launch_bounds__(kLpThreads) void logprob_rows_kernel(LogprobArgs a)
     const float other = __shfl_xor(m, d);
     m = m != m || other != other ? NAN : fmaxf(m, other);
   }
-  if (lane == 0) sm[wave] = m;
+  __syncthreads();
+  if (lane == 0) sh.m[wave] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kLpThreads / kWave; ++w) m = m != m || sm[w] != sm[w] ? NAN : fmaxf(m, sm[w]);
+  for (int w = 0; w < kLpWaves; ++w) m = m != m || sh.m[w] != sh.m[w] ? NAN : fmaxf(m, sh.m[w]);
   float s = 0.f, w = 0.f;
   for (int i = tid; i < a.vocab; i += kLpThreads) {
-    const float y = (load_elem(a.logits, T::dtype, base + i) - m) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+    const float y = (row.at(i) - m) * kLog2e, e = __builtin_amdgcn_exp2f(y);
     s += e;
     if (e != 0.f) w = __builtin_fmaf(e, y, w);
   }
   s = group_sum(s, kWave), w = group_sum(w, kWave);
-  if (lane == 0) ss[wave] = s, sw[wave] = w;
+  if (lane == 0) sh.s[wave] = s, sh.w[wave] = w;
   __syncthreads();
   s = w = 0.f;
 #pragma unroll
-  for (int i = 0; i < kLpThreads / kWave; ++i) s += ss[i], w += sw[i];
+  for (int i = 0; i < kLpWaves; ++i) s += sh.s[i], w += sh.w[i];
   const float log_s = logf(s);
-  if (tid == 0) a.entropy[row] = log_s - w / s * kLn2;
+  if (tid == 0) a.entropy[r] = log_s - w / s * (float)kLn2;
   for (int g = tid; g < a.per_row; g += kLpThreads) {
-    const int64_t token = a.tokens[row * a.tokens_stride + g];
+    const int64_t token = a.tokens[r * a.tokens_stride + g];
     const bool known = token >= 0 && token < a.vocab;
-    a.logprobs[row * a.per_row + g] =
-        known ? load_elem(a.logits, T::dtype, base + token) - m - log_s : s == s ? -INFINITY : NAN;
+    a.logprobs[r * a.per_row + g] = known ? row.at(known ? token : 0) - m - log_s : s == s ? -INFINITY : NAN;
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t key = 0;
-    for (int i = tid; i < a.vocab; i += kLpThreads) {
-      const uint64_t x = lp_key(load_elem(a.logits, T::dtype, base + i), i);
-      if (x < last && x > key) key = x;
-    }
-    key = lp_wave_max(key);
-    if (lane == 0) best[k & 1][wave] = key;
-    __syncthreads();
+  lp_top_by_rounds(row, LpPart{0, row.chunks, true, true}, a.top, sh);
+  if (tid < a.top) {
+    const int i = lp_index(sh.sorted[tid]);
+    a.top_ids[r * a.top + tid] = i;
+    a.top_logprobs[r * a.top + tid] = row.at(i) - m - log_s;
+  }
+}
+
+__device__ __forceinline__ bool lp_usual(const LpSums& t) { return t.s > 0.f && t.s < INFINITY; }
+
+// One pass over a row or a part of it. Every thread keeps a reference of its
+// own (its running maximum times log2 e, rounded: the exponents are exact
+// relative to it, and references only ever meet as these numbers), S and W
+// over blocks of four chunks, and its largest logit, which the search for the
+// alternatives starts from.
+template <typename T>
+__global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
+  constexpr int E = LpRow<T>::E, U = 4;
+  __shared__ LogprobShared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x / (unsigned)a.splits;
+  const int split = blockIdx.x - (int)r * a.splits;
+  const LpRow<T> row(a, r);
+  LpPart part;
+  part.first = min(split * a.split_chunks, row.chunks);
+  part.last = split == a.splits - 1 ? row.chunks : min(part.first + a.split_chunks, row.chunks);
+  part.lead = split == 0, part.tail = split == a.splits - 1;
+
+  float m = -1e38f, top = -INFINITY;  // (a finite start: nothing above it leaves S at 0)
+  LpSums t{m * kLog2e, 0.f, 0.f};
+  const auto raise = [&](float block_max) {
+#pragma clang fp contract(off)  // d is the difference of the rounded references
+    top = fmaxf(top, block_max);
+    const float ref = fmaxf(m, block_max) * kLog2e, d = t.s > 0.f ? t.ref - ref : 0.f;
+    const float f = __builtin_amdgcn_exp2f(d);
+    m = fmaxf(m, block_max);
+    t.w = f * __builtin_fmaf(fmaxf(d, -1e9f), t.s, t.w);
+    t.s *= f;
+    t.ref = ref;
+  };
+  const auto add = [&](float x, float& s, float& w) {
+    const float y = __builtin_fmaf(x, kLog2e, -t.ref), e = __builtin_amdgcn_exp2f(y);
+    s += e;
+    w = __builtin_fmaf(e, fmaxf(y, -1e9f), w);  // 0 and not NaN where x is -inf
+  };
+  int c = part.first + tid;
+  for (; c + (U - 1) * kLpThreads < part.last; c += U * kLpThreads) {
+    uint4 v[U];
 #pragma unroll
-    for (int i = 0; i < kLpThreads / kWave; ++i) key = key > best[k & 1][i] ? key : best[k & 1][i];
-    last = key;
-    if (tid == 0) {
-      const int index = (int)~(uint32_t)key;
-      a.top_ids[row * a.top + k] = index;
-      a.top_logprobs[row * a.top + k] = load_elem(a.logits, T::dtype, base + index) - m - log_s;
+    for (int u = 0; u < U; ++u) v[u] = row.load(c + u * kLpThreads);
+    float x[U][E], block_max = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      LpRow<T>::unpack(v[u], x[u]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) block_max = fmaxf(block_max, x[u][e]);
     }
+    raise(block_max);
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) add(x[u][e], s, w);
+    t.s += s, t.w += w;
   }
+  for (; c < part.last; c += kLpThreads) {
+    float x[E], block_max = -INFINITY, s = 0.f, w = 0.f;
+    LpRow<T>::unpack(row.load(c), x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) block_max = fmaxf(block_max, x[e]);
+    raise(block_max);
+#pragma unroll
+    for (int e = 0; e < E; ++e) add(x[e], s, w);
+    t.s += s, t.w += w;
+  }
+  const bool any = part.first + tid < part.last;
+  const float thread_max = top;
+  // the elements around the chunks, which the search looks at in any case
+  if (part.lead && tid < row.lead) {
+    const float x = row.at(tid);
+    raise(x);
+    add(x, t.s, t.w);
+  }
+  if (part.tail && row.index(row.chunks, 0) + tid < row.vocab) {
+    const float x = row.at(row.index(row.chunks, 0) + tid);
+    raise(x);
+    add(x, t.s, t.w);
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1)
+    t = lp_join(t, LpSums{__shfl_xor(t.ref, d), __shfl_xor(t.s, d), __shfl_xor(t.w, d)});
+  if (lane == 0) sh.m[wave] = t.ref, sh.s[wave] = t.s, sh.w[wave] = t.w;
+  __syncthreads();
+  t = {sh.m[0], sh.s[0], sh.w[0]};
+#pragma unroll
+  for (int w = 1; w < kLpWaves; ++w) t = lp_join(t, LpSums{sh.m[w], sh.s[w], sh.w[w]});
+  if (a.splits == 1 && !lp_usual(t)) {
+    lp_unusual_row(a, r, row, sh);
+    return;
+  }
+  if (a.top) lp_top(row, part, a.top, any, thread_max, sh);
+  if (a.splits == 1) {
+    lp_finish(a, r, row, t, sh);
+    return;
+  }
+  if (tid == 0) a.sums[blockIdx.x] = make_float4(t.ref, t.s, t.w, 0.f);
+  if (tid < a.top) a.keys[(int64_t)blockIdx.x * a.top + tid] = sh.sorted[tid];
+}
+
+// Joins the parts of a row, one workgroup per row.
+template <typename T>
+__global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(LogprobArgs a) {
+  __shared__ LogprobShared sh;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t r = blockIdx.x;
+  const LpRow<T> row(a, r);
+  const int n = a.splits * a.top;  // at most kLpCandidates
+  for (int i = tid; i < n; i += kLpThreads) sh.found[i] = a.keys[r * n + i];
+  const float4 part = a.sums[r * a.splits + min(lane, a.splits - 1)];
+  LpSums t{part.x, lane < a.splits ? part.y : 0.f, lane < a.splits ? part.z : 0.f};
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1)
+    t = lp_join(t, LpSums{__shfl_xor(t.ref, d), __shfl_xor(t.s, d), __shfl_xor(t.w, d)});
+  __syncthreads();
+  if (!lp_usual(t)) {
+    lp_unusual_row(a, r, row, sh);
+    return;
+  }
+  if (a.top) lp_sort_found(n, a.top, sh);
+  lp_finish(a, r, row, t, sh);
+}
+
+struct LogprobShape {
+  int splits, split_chunks;
+};
+
+// About 1024 workgroups in all (four on a CU), none of less than 1024 chunks (four loads of every thread).
+static LogprobShape logprob_shape(int rows, int vocab, int dtype, int top) {
+  const int chunks = vocab / (16 / elem_size(dtype));
+  int64_t splits = std::min<int64_t>(1024 / std::max(rows, 1), chunks / 1024);
+  splits = std::min<int64_t>(splits, std::min(kLpMaxSplits, kLpCandidates / std::max(top, 1)));
+  LogprobShape s;
+  s.splits = (int)std::max<int64_t>(splits, 1);
+  s.split_chunks = (chunks + s.splits - 1) / s.splits;
+  return s;
 }
 
 }  // namespace nhs
@@ -124,7 +491,9 @@ __global__ __launch_bounds__(kLpThreads) void logprob_rows_kernel(LogprobArgs a)
 using namespace nhs;
 
 extern "C" int64_t nhs_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype, int32_t top) {
-  return 0;
+  if (rows < 1 || vocab < 1 || top < 0 || top > kLpMaxTop || !valid_dtype(dtype)) return 0;
+  const LogprobShape s = logprob_shape(rows, vocab, dtype, top);
+  return s.splits == 1 ? 0 : (int64_t)rows * s.splits * (int64_t)(sizeof(float4) + top * sizeof(uint64_t));
 }
 
 extern "C" int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, int32_t rows, int32_t vocab,
@@ -142,15 +511,26 @@ extern "C" int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_
   if ((uintptr_t)logits % elem_size(dtype) || ((uintptr_t)tokens | (uintptr_t)top_ids) % 8 ||
       ((uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_logprobs) % 4)
     return fail(NHS_ERR_INVALID, "%s: misaligned pointer", who);
+  const LogprobShape shape = logprob_shape(rows, vocab, dtype, top);
+  const int64_t need = nhs_token_logprobs_workspace_bytes(rows, vocab, dtype, top), parts = (int64_t)rows * shape.splits;
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return fail(NHS_ERR_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", who, (long long)need);
   LogprobArgs a{static_cast<const char*>(logits), row_stride, vocab, top, tokens_per_row, tokens, tokens_stride,
-                logprobs, entropy, top_ids, top_logprobs};
-  const dim3 grid((unsigned)rows), block(kLpThreads);
+                logprobs, entropy, top_ids, top_logprobs, shape.splits, shape.split_chunks,
+                static_cast<float4*>(workspace), nullptr};
+  a.keys = reinterpret_cast<uint64_t*>(a.sums + parts);
   hipStream_t s = (hipStream_t)stream;
+  const hipEvent_t none = nullptr;
+  const auto run = [&](auto kernel, auto join) {
+    const bool joined = shape.splits > 1;
+    launch(kernel, dim3((unsigned)parts), dim3(kLpThreads), 0, s, ev.start, joined ? none : ev.stop, a);
+    if (joined) launch(join, dim3((unsigned)rows), dim3(kLpThreads), 0, s, none, ev.stop, a);
+  };
   if (dtype == NHS_BF16)
-    launch(logprob_rows_kernel<BF16>, grid, block, 0, s, ev.start, ev.stop, a);
+    run(logprob_kernel<BF16>, logprob_join_kernel<BF16>);
   else if (dtype == NHS_F16)
-    launch(logprob_rows_kernel<F16>, grid, block, 0, s, ev.start, ev.stop, a);
+    run(logprob_kernel<F16>, logprob_join_kernel<F16>);
   else
-    launch(logprob_rows_kernel<F32>, grid, block, 0, s, ev.start, ev.stop, a);
+    run(logprob_kernel<F32>, logprob_join_kernel<F32>);
   return launch_status(who);
 }
