@@ -49,6 +49,10 @@ __device__ __forceinline__ uint64_t lp_key(float x, int index) {
   return (uint64_t)lp_order(x) << 32 | (uint32_t)~index;
 }
 __device__ __forceinline__ int lp_index(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float lp_value(uint64_t key) {  // the logit (+0 for -0, a NaN for a NaN)
+  const uint32_t o = key >> 32;
+  return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
 
 __device__ __forceinline__ uint64_t lp_wave_max(uint64_t key) {
 #pragma unroll
@@ -62,11 +66,11 @@ __device__ __forceinline__ uint64_t lp_wave_max(uint64_t key) {
 struct LogprobShared {
   float m[kLpWaves], s[kLpWaves], w[kLpWaves];
   uint64_t best[2][kLpWaves];
-  uint32_t lane_max[kLpThreads];     // order of the largest logit of each thread, 0 without one
+  __attribute__((aligned(16))) uint32_t lane_max[kLpThreads];  // order of the largest logit of each thread, 0 without one
   int hot[kLpThreads];               // threads whose elements may be among the alternatives
   int n_hot, n_found, scan[kLpWaves + 1];
   uint32_t threshold;
-  uint64_t found[kLpCandidates];
+  __attribute__((aligned(16))) uint64_t found[kLpCandidates];
   uint64_t sorted[kLpMaxTop];
 };
 
@@ -80,6 +84,15 @@ __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b) {
   // (below -1e9 the factor is 0: the product must only be finite)
   return {ref, a.s * fa + b.s * fb,
           fa * __builtin_fmaf(fmaxf(da, -1e9f), a.s, a.w) + fb * __builtin_fmaf(fmaxf(db, -1e9f), b.s, b.w)};
+}
+
+// over the wave: every lane moves to the largest reference, then plain sums
+__device__ __forceinline__ LpSums lp_wave_join(LpSums t) {
+  float ref = t.ref;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) ref = fmaxf(ref, __shfl_xor(ref, d));
+  const float d = t.ref - ref, f = __builtin_amdgcn_exp2f(d);
+  return {ref, group_sum(t.s * f, kWave), group_sum(f * __builtin_fmaf(fmaxf(d, -1e9f), t.s, t.w), kWave)};
 }
 
 // The chunks of 16 bytes of a row that lie wholly inside it, and the elements before and after them.
@@ -141,30 +154,25 @@ __device__ void lp_top_by_rounds(const LpRow<T>& row, const LpPart& part, int to
 }
 
 // The `top` largest of sh.found[0 .. n) in descending order to sh.sorted (0 beyond n): every key's place is the number
-// of larger ones.
+// of larger ones. Sixteen keys are read at a time, so that the wait for LDS is paid once for them.
 __device__ __forceinline__ void lp_sort_found(int n, int top, LogprobShared& sh) {
-  const int tid = threadIdx.x;
+  constexpr int kStep = 16;
+  const int tid = threadIdx.x, padded = (n + kStep - 1) / kStep * kStep;
   if (tid < top) sh.sorted[tid] = 0;
+  if (tid < padded - n) sh.found[n + tid] = 0;
   __syncthreads();
-  constexpr int kMine = kLpCandidates / kLpThreads;
-  uint64_t key[kMine];
-  int place[kMine];
+  for (int i = tid; i < n; i += kLpThreads) {
+    const uint64_t key = sh.found[i];
+    int place[2] = {0, 0};
+    for (int x = 0; x < padded; x += kStep) {
+      uint64_t other[kStep];
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) {
-    const int i = tid + j * kLpThreads;
-    key[j] = i < n ? sh.found[i] : 0;
-    place[j] = 0;
+      for (int e = 0; e < kStep; ++e) other[e] = sh.found[x + e];
+#pragma unroll
+      for (int e = 0; e < kStep; ++e) place[e & 1] += other[e] > key;
+    }
+    if (key && place[0] + place[1] < top) sh.sorted[place[0] + place[1]] = key;
   }
-  const int mine = (n + kLpThreads - 1) / kLpThreads;
-  for (int i = 0; i < n; ++i) {
-    const uint64_t other = sh.found[i];
-#pragma unroll
-    for (int j = 0; j < kMine; ++j)
-      if (j < mine) place[j] += other > key[j];
-  }
-#pragma unroll
-  for (int j = 0; j < kMine; ++j)
-    if (key[j] && place[j] < top) sh.sorted[place[j]] = key[j];
   __syncthreads();
 }
 
@@ -179,22 +187,23 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
   const int tid = threadIdx.x, lane = tid & 63;
   const uint32_t mine = any ? lp_order(thread_max) : 0u;
   sh.lane_max[tid] = mine;
-  if (tid == 0) sh.n_hot = sh.n_found = 0;
+  if (tid == 0) sh.n_hot = sh.n_found = 0, sh.threshold = 0xffffffffu;
   __syncthreads();
-  int place = 0;
+  // the threads with fewer than `top` larger ones; the least of them is the top-th largest
+  int larger[2] = {0, 0};
   const uint4* all = reinterpret_cast<const uint4*>(sh.lane_max);
-#pragma unroll 4
+#pragma unroll 16
   for (int i = 0; i < kLpThreads / 4; ++i) {
     const uint4 v = all[i];
-    const int above = tid - 4 * i;  // of equal ones, lower threads come first
-    place += (v.x > mine || (v.x == mine && 0 < above)) + (v.y > mine || (v.y == mine && 1 < above)) +
-             (v.z > mine || (v.z == mine && 2 < above)) + (v.w > mine || (v.w == mine && 3 < above));
+    larger[0] += (v.x > mine) + (v.z > mine);
+    larger[1] += (v.y > mine) + (v.w > mine);
   }
-  if (place == top - 1) sh.threshold = mine;
+  if (larger[0] + larger[1] < top) {
+    atomicMin(&sh.threshold, mine);
+    if (mine) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
+  }
   __syncthreads();
   const uint32_t threshold = sh.threshold;
-  if (mine >= max(threshold, 1u)) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
-  __syncthreads();
   const int per_thread = (part.last - part.first + kLpThreads - 1) / kLpThreads;
   const int pairs = sh.n_hot * per_thread;  // at most 256 threads x their chunks: the part
   // pushes the elements whose order is at least `least`
@@ -275,25 +284,35 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
   lp_sort_found(sh.n_found, top, sh);
 }
 
+// The logit of a given token.
+struct LpToken {
+  float x;
+  bool known;
+};
+template <typename T>
+__device__ __forceinline__ LpToken lp_token(const LogprobArgs& a, int64_t r, const LpRow<T>& row, int g) {
+  const int64_t token = a.tokens[r * a.tokens_stride + g];
+  const bool known = token >= 0 && token < a.vocab;
+  return {row.at(known ? token : 0), known};
+}
+
 // The outputs of a row from its sums and sh.sorted. The sums are those of x * (1 + beta), where kLog2e rounds to
 // log2 e * (1 + beta): to first order lse(x) = lse(x (1 + beta)) - beta * sum p x.
-template <typename T>
-__device__ void lp_finish(const LogprobArgs& a, int64_t r, const LpRow<T>& row, const LpSums& t,
-                          LogprobShared& sh) {
+template <typename F>
+__device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t r, const LpSums& t, const LpToken& first,
+                                          F logit, LogprobShared& sh) {
   constexpr double beta = (double)kLog2e * kLn2 - 1.0;
   const double bits = (double)log2f(t.s), mean = (double)t.w / (double)t.s;
   const double lse = ((double)t.ref + bits - beta * (mean + (double)t.ref)) * kLn2;
   const int tid = threadIdx.x;
   if (tid == 0) a.entropy[r] = (float)((bits - mean) * kLn2);
   for (int g = tid; g < a.per_row; g += kLpThreads) {
-    const int64_t token = a.tokens[r * a.tokens_stride + g];
-    const bool known = token >= 0 && token < a.vocab;
-    a.logprobs[r * a.per_row + g] = known ? (float)((double)row.at(known ? token : 0) - lse) : -INFINITY;
+    const LpToken token = g == tid ? first : logit(g);
+    a.logprobs[r * a.per_row + g] = token.known ? (float)((double)token.x - lse) : -INFINITY;
   }
   if (tid < a.top) {
-    const int i = lp_index(sh.sorted[tid]);
-    a.top_ids[r * a.top + tid] = i;
-    a.top_logprobs[r * a.top + tid] = (float)((double)row.at(i) - lse);
+    a.top_ids[r * a.top + tid] = lp_index(sh.sorted[tid]);
+    a.top_logprobs[r * a.top + tid] = (float)((double)lp_value(sh.sorted[tid]) - lse);
   }
 }
 
@@ -335,15 +354,13 @@ __device__ void lp_unusual_row(const LogprobArgs& a, int64_t r, const LpRow<T>& 
   const float log_s = logf(s);
   if (tid == 0) a.entropy[r] = log_s - w / s * (float)kLn2;
   for (int g = tid; g < a.per_row; g += kLpThreads) {
-    const int64_t token = a.tokens[r * a.tokens_stride + g];
-    const bool known = token >= 0 && token < a.vocab;
-    a.logprobs[r * a.per_row + g] = known ? row.at(known ? token : 0) - m - log_s : s == s ? -INFINITY : NAN;
+    const LpToken token = lp_token(a, r, row, g);
+    a.logprobs[r * a.per_row + g] = token.known ? token.x - m - log_s : s == s ? -INFINITY : NAN;
   }
   lp_top_by_rounds(row, LpPart{0, row.chunks, true, true}, a.top, sh);
   if (tid < a.top) {
-    const int i = lp_index(sh.sorted[tid]);
-    a.top_ids[r * a.top + tid] = i;
-    a.top_logprobs[r * a.top + tid] = row.at(i) - m - log_s;
+    a.top_ids[r * a.top + tid] = lp_index(sh.sorted[tid]);
+    a.top_logprobs[r * a.top + tid] = lp_value(sh.sorted[tid]) - m - log_s;
   }
 }
 
@@ -367,6 +384,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
   part.last = split == a.splits - 1 ? row.chunks : min(part.first + a.split_chunks, row.chunks);
   part.lead = split == 0, part.tail = split == a.splits - 1;
 
+  // the given tokens' logits are asked for first
+  const LpToken token = a.splits == 1 && tid < a.per_row ? lp_token(a, r, row, tid) : LpToken{0.f, false};
   float m = -1e38f, top = -INFINITY;  // (a finite start: nothing above it leaves S at 0)
   LpSums t{m * kLog2e, 0.f, 0.f};
   const auto raise = [&](float block_max) {
@@ -384,11 +403,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     s += e;
     w = __builtin_fmaf(e, fmaxf(y, -1e9f), w);  // 0 and not NaN where x is -inf
   };
-  int c = part.first + tid;
-  for (; c + (U - 1) * kLpThreads < part.last; c += U * kLpThreads) {
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = row.load(c + u * kLpThreads);
+  const auto block = [&](const uint4 (&v)[U]) {
     float x[U][E], block_max = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -403,16 +418,23 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) add(x[u][e], s, w);
     t.s += s, t.w += w;
+  };
+  int c = part.first + tid;
+  for (; c + (U - 1) * kLpThreads < part.last; c += U * kLpThreads) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = row.load(c + u * kLpThreads);
+    block(v);
   }
-  for (; c < part.last; c += kLpThreads) {
-    float x[E], block_max = -INFINITY, s = 0.f, w = 0.f;
-    LpRow<T>::unpack(row.load(c), x);
+  if (c < part.last) {  // the last block: chunks past the end count as -inf
+    constexpr uint32_t none = T::dtype == NHS_F32 ? 0xff800000u : T::dtype == NHS_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    uint4 v[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) block_max = fmaxf(block_max, x[e]);
-    raise(block_max);
-#pragma unroll
-    for (int e = 0; e < E; ++e) add(x[e], s, w);
-    t.s += s, t.w += w;
+    for (int u = 0; u < U; ++u) {
+      v[u] = make_uint4(none, none, none, none);
+      if (c + u * kLpThreads < part.last) v[u] = row.load(c + u * kLpThreads);
+    }
+    block(v);
   }
   const bool any = part.first + tid < part.last;
   const float thread_max = top;
@@ -427,9 +449,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     raise(x);
     add(x, t.s, t.w);
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1)
-    t = lp_join(t, LpSums{__shfl_xor(t.ref, d), __shfl_xor(t.s, d), __shfl_xor(t.w, d)});
+  t = lp_wave_join(t);
   if (lane == 0) sh.m[wave] = t.ref, sh.s[wave] = t.s, sh.w[wave] = t.w;
   __syncthreads();
   t = {sh.m[0], sh.s[0], sh.w[0]};
@@ -441,7 +461,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
   }
   if (a.top) lp_top(row, part, a.top, any, thread_max, sh);
   if (a.splits == 1) {
-    lp_finish(a, r, row, t, sh);
+    lp_finish(a, r, t, token, [&](int g) { return lp_token(a, r, row, g); }, sh);
     return;
   }
   if (tid == 0) a.sums[blockIdx.x] = make_float4(t.ref, t.s, t.w, 0.f);
@@ -455,20 +475,19 @@ __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(LogprobArgs a)
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t r = blockIdx.x;
   const LpRow<T> row(a, r);
-  const int n = a.splits * a.top;  // at most kLpCandidates
+  const int n = a.splits * a.top;  // at most kLpThreads
+  const LpToken token = tid < a.per_row ? lp_token(a, r, row, tid) : LpToken{0.f, false};
   for (int i = tid; i < n; i += kLpThreads) sh.found[i] = a.keys[r * n + i];
   const float4 part = a.sums[r * a.splits + min(lane, a.splits - 1)];
   LpSums t{part.x, lane < a.splits ? part.y : 0.f, lane < a.splits ? part.z : 0.f};
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1)
-    t = lp_join(t, LpSums{__shfl_xor(t.ref, d), __shfl_xor(t.s, d), __shfl_xor(t.w, d)});
+  t = lp_wave_join(t);
   __syncthreads();
   if (!lp_usual(t)) {
     lp_unusual_row(a, r, row, sh);
     return;
   }
   if (a.top) lp_sort_found(n, a.top, sh);
-  lp_finish(a, r, row, t, sh);
+  lp_finish(a, r, t, token, [&](int g) { return lp_token(a, r, row, g); }, sh);
 }
 
 struct LogprobShape {
@@ -479,7 +498,8 @@ struct LogprobShape {
 static LogprobShape logprob_shape(int rows, int vocab, int dtype, int top) {
   const int chunks = vocab / (16 / elem_size(dtype));
   int64_t splits = std::min<int64_t>(1024 / std::max(rows, 1), chunks / 1024);
-  splits = std::min<int64_t>(splits, std::min(kLpMaxSplits, kLpCandidates / std::max(top, 1)));
+  // (the join sorts a key per thread)
+  splits = std::min<int64_t>(splits, std::min(kLpMaxSplits, kLpThreads / std::max(top, 1)));
   LogprobShape s;
   s.splits = (int)std::max<int64_t>(splits, 1);
   s.split_chunks = (chunks + s.splits - 1) / s.splits;
