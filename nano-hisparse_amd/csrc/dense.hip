@@ -4,6 +4,8 @@
 // torch bf16/fp16 operation computes in fp32 and rounds its result to the
 // tensor dtype; separate torch operations never fuse a multiply into an
 // add, hence fp contract(off)), so only reduction order can differ.
+#include <type_traits>
+
 #include "nhs_common.h"
 
 namespace nhs {
@@ -205,6 +207,7 @@ __global__ void rope_kernel(typename T::Bits* t, int64_t row_stride, int heads, 
 // 32 heads of 128: 66 MB moved, 16.8 us; 2 bytes a lane and a division
 // per element took 30.0).
 constexpr int kRopeThreads = 256;
+constexpr int64_t kNormRopeWide = 4096;  // waves of one round of heads from which a wave takes four
 
 template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(uint16_t* t, int64_t row_stride, int chunks, int half,
@@ -271,6 +274,26 @@ struct NormRopeArgs {
   float eps;
 };
 
+// eight 16-bit elements as fp32
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = T::to_float((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+}
+
+// eight elements of a table, from element `at` on
+template <typename TT>
+__device__ __forceinline__ void load_table(const char* table, int64_t at, float (&x)[8]) {
+  if constexpr (sizeof(typename TT::Bits) == 2) {
+    unpack8<TT>(*reinterpret_cast<const uint4*>(table + at * 2), x);
+  } else {
+    const float4 lo = *reinterpret_cast<const float4*>(table + at * 4);
+    const float4 hi = *reinterpret_cast<const float4*>(table + at * 4 + 16);
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+  }
+}
+
 __device__ __forceinline__ int64_t table_row(const NormRopeArgs& a, int64_t row) {
   const int64_t at = a.positions ? a.positions[row] : row;
   return min(max(at, (int64_t)0), a.table_rows - 1);
@@ -307,6 +330,69 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(NormRopeArgs
     const float c = TT::to_float(cos[d]), s = TT::to_float(sin[d]);
     y[d] = T::from_float(lo * c - hi * s);
     y[d + half] = T::from_float(hi * c + lo * s);
+  }
+}
+
+// The same for 16-bit heads whose halves are whole 16-byte chunks (at most 64
+// of them): the LANES lanes of a head hold one chunk of each half, so a pair
+// and its sum of squares never leave them; a wave takes U x 64 / LANES heads
+// of one row, whose cos/sin chunks it loads once, and asks for every head
+// before it computes the first. Bound by memory (each element moves once):
+// 16001 rows of 32 + 8 heads of 128, 332 MB.
+template <typename T, typename TT, int LANES, int U>
+__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_vec_kernel(NormRopeArgs a, FastDiv parts) {
+  constexpr int GROUPS = kWave / LANES;
+  const uint32_t item = blockIdx.x * (kRopeThreads / kWave) + (threadIdx.x >> 6);
+  const uint32_t row = parts.div(item);
+  if (row >= (uint32_t)a.rows) return;
+  const int lane = threadIdx.x & 63, group = lane / LANES, d = (lane % LANES) * 8;
+  const bool live = d < a.half;
+  const int first = (int)(item - row * parts.d) * (GROUPS * U) + group;
+  const auto chunk = [](const char* base, int64_t element, bool ok) {
+    return ok ? *reinterpret_cast<const uint4*>(base + element * 2) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  uint4 lo[U], hi[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = first + u * GROUPS, kh = h - a.q_heads;
+    const bool ok = live && h < a.heads;
+    const int64_t at = (kh < 0 ? row * a.q_r + h * a.q_h : row * a.k_r + kh * a.k_h) + d;
+    lo[u] = chunk(kh < 0 ? a.q : a.k, at, ok);
+    hi[u] = chunk(kh < 0 ? a.q : a.k, at + a.half, ok);
+  }
+  float c[8], s[8];
+  {
+    const int64_t at = live ? table_row(a, row) * a.half + d : 0;
+    load_table<TT>(a.cos, at, c);
+    load_table<TT>(a.sin, at, s);
+  }
+  const int dw = live ? d : 0;
+  const uint4 qw_lo = chunk(a.q_weight, dw, true), qw_hi = chunk(a.q_weight, dw + a.half, true);
+  const uint4 kw_lo = chunk(a.k_weight, dw, true), kw_hi = chunk(a.k_weight, dw + a.half, true);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = first + u * GROUPS, kh = h - a.q_heads;
+    float x[8], y[8], acc = 0.f;
+    unpack8<T>(lo[u], x);
+    unpack8<T>(hi[u], y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], acc));
+    const float r = rsqrtf(group_sum(acc, LANES) / (float)(2 * a.half) + a.eps);
+    float wx[8], wy[8];
+    unpack8<T>(kh < 0 ? qw_lo : kw_lo, wx);
+    unpack8<T>(kh < 0 ? qw_hi : kw_hi, wy);
+    uint32_t ox[4] = {0, 0, 0, 0}, oy[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = x[e] * r * wx[e], q = y[e] * r * wy[e];
+      ox[e >> 1] |= (uint32_t)T::from_float(p * c[e] - q * s[e]) << (16 * (e & 1));
+      oy[e >> 1] |= (uint32_t)T::from_float(q * c[e] + p * s[e]) << (16 * (e & 1));
+    }
+    if (!live || h >= a.heads) continue;
+    const int64_t at = (kh < 0 ? row * a.qo_r + h * a.qo_h : row * a.ko_r + kh * a.ko_h) + d;
+    char* out = kh < 0 ? a.q_out : a.k_out;
+    *reinterpret_cast<uint4*>(out + at * 2) = make_uint4(ox[0], ox[1], ox[2], ox[3]);
+    *reinterpret_cast<uint4*>(out + (at + a.half) * 2) = make_uint4(oy[0], oy[1], oy[2], oy[3]);
   }
 }
 
@@ -465,6 +551,56 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
   a.table_rows = table_rows, a.positions = positions;
   a.rows = rows, a.q_heads = q_heads, a.heads = q_heads + k_heads, a.half = head_dim / 2, a.eps = eps;
   hipStream_t s = (hipStream_t)stream;
+  bool vec = dtype != NHS_F32 && a.half % 8 == 0 && a.half <= 512 &&
+             ((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight |
+              (uintptr_t)k_weight | (uintptr_t)cos | (uintptr_t)sin) % 16 == 0;
+  for (const int64_t stride : {q_row_stride, q_head_stride, k_row_stride, k_head_stride, qo_row_stride,
+                               qo_head_stride, ko_row_stride, ko_head_stride})
+    vec = vec && stride % 8 == 0;
+  if (vec) {
+    int lanes = 1;
+    while (lanes * 8 < a.half) lanes *= 2;
+    const int groups = kWave / lanes, per_wave = (a.heads + groups - 1) / groups;  // rounds of a wave that takes a row
+    const bool wide = (int64_t)rows * per_wave >= kNormRopeWide;
+    const int u = wide ? 4 : 1;
+    const int64_t parts = (per_wave + u - 1) / u, waves = rows * parts;
+    if (waves <= 0x7fffffff) {
+      const dim3 grid((unsigned)((waves + 3) / 4)), block(kRopeThreads);
+      const auto run_vec = [&](auto t, auto table, auto l) {
+        using T = decltype(t);
+        using TT = decltype(table);
+        constexpr int L = decltype(l)::value;
+        if (wide)
+          launch(qk_norm_rope_vec_kernel<T, TT, L, 4>, grid, block, 0, s, ev.start, ev.stop, a,
+                 FastDiv((uint32_t)parts));
+        else
+          launch(qk_norm_rope_vec_kernel<T, TT, L, 1>, grid, block, 0, s, ev.start, ev.stop, a,
+                 FastDiv((uint32_t)parts));
+      };
+      const auto by_lanes = [&](auto t, auto table) {
+        switch (lanes) {
+          case 1: return run_vec(t, table, std::integral_constant<int, 1>());
+          case 2: return run_vec(t, table, std::integral_constant<int, 2>());
+          case 4: return run_vec(t, table, std::integral_constant<int, 4>());
+          case 8: return run_vec(t, table, std::integral_constant<int, 8>());
+          case 16: return run_vec(t, table, std::integral_constant<int, 16>());
+          case 32: return run_vec(t, table, std::integral_constant<int, 32>());
+          default: return run_vec(t, table, std::integral_constant<int, 64>());
+        }
+      };
+      const auto by_table = [&](auto t) {
+        if (table_dtype == NHS_F32)
+          by_lanes(t, F32T{});
+        else
+          by_lanes(t, t);
+      };
+      if (dtype == NHS_BF16)
+        by_table(BF16T{});
+      else
+        by_table(F16T{});
+      return launch_status(who);
+    }
+  }
   const int64_t items = (int64_t)rows * a.heads, blocks = (items + kRopeThreads / kWave - 1) / (kRopeThreads / kWave);
   if (blocks > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "%s: too many workgroups", who);
   const auto run = [&](auto kernel) {
