@@ -207,7 +207,9 @@ __global__ void rope_kernel(typename T::Bits* t, int64_t row_stride, int heads, 
 // 32 heads of 128: 66 MB moved, 16.8 us; 2 bytes a lane and a division
 // per element took 30.0).
 constexpr int kRopeThreads = 256;
-constexpr int64_t kNormRopeWide = 4096;  // waves of one round of heads from which a wave takes four
+// Waves of one round of heads from which a wave takes two rounds. us with one / two (bf16, rows x heads x 128): 4000 x 40
+// (20000 waves) 17.8 / 18.5, 16001 x 32 (64004) 52.1 / 46.8, 16001 x 40 (80005) 65.4 / 61.6; three to five lose.
+constexpr int64_t kNormRopeWide = 40960;
 
 template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void rope_vec_kernel(uint16_t* t, int64_t row_stride, int chunks, int half,
@@ -274,25 +276,50 @@ struct NormRopeArgs {
   float eps;
 };
 
-// eight 16-bit elements as fp32
+// eight consecutive elements: 16 bytes of a 16-bit type, 32 of fp32
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Chunk8 {
+  static constexpr int W = sizeof(typename T::Bits) / 2;
+  uint4 v[W];
+  __device__ __forceinline__ void load(const char* base, int64_t element, bool ok = true) {
+    const uint4* p = reinterpret_cast<const uint4*>(base + element * (int)sizeof(typename T::Bits));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = T::to_float((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
-}
-
-// eight elements of a table, from element `at` on
-template <typename TT>
-__device__ __forceinline__ void load_table(const char* table, int64_t at, float (&x)[8]) {
-  if constexpr (sizeof(typename TT::Bits) == 2) {
-    unpack8<TT>(*reinterpret_cast<const uint4*>(table + at * 2), x);
-  } else {
-    const float4 lo = *reinterpret_cast<const float4*>(table + at * 4);
-    const float4 hi = *reinterpret_cast<const float4*>(table + at * 4 + 16);
-    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+    for (int i = 0; i < W; ++i) v[i] = ok ? p[i] : make_uint4(0u, 0u, 0u, 0u);
   }
-}
+  __device__ __forceinline__ void store(char* base, int64_t element) const {
+    uint4* p = reinterpret_cast<uint4*>(base + element * (int)sizeof(typename T::Bits));
+#pragma unroll
+    for (int i = 0; i < W; ++i) p[i] = v[i];
+  }
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+    if constexpr (W == 1) {
+      const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = T::to_float((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = __uint_as_float(w[e]);
+      }
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&x)[8]) {
+    if constexpr (W == 1) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = (uint32_t)T::from_float(x[2 * e]) | (uint32_t)T::from_float(x[2 * e + 1]) << 16;
+      v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        v[i] = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i + 2]),
+                          __float_as_uint(x[4 * i + 3]));
+    }
+  }
+};
 
 __device__ __forceinline__ int64_t table_row(const NormRopeArgs& a, int64_t row) {
   const int64_t at = a.positions ? a.positions[row] : row;
@@ -333,12 +360,13 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(NormRopeArgs
   }
 }
 
-// The same for 16-bit heads whose halves are whole 16-byte chunks (at most 64
+// The same for heads whose halves are whole chunks of 8 elements (at most 64
 // of them): the LANES lanes of a head hold one chunk of each half, so a pair
 // and its sum of squares never leave them; a wave takes U x 64 / LANES heads
 // of one row, whose cos/sin chunks it loads once, and asks for every head
 // before it computes the first. Bound by memory (each element moves once):
-// 16001 rows of 32 + 8 heads of 128, 332 MB.
+// 16001 rows of 32 + 8 heads of 128 in bf16, 332 MB, 62 us (5.3 TB/s, the
+// rate of a large copy); an element per lane took 216.
 template <typename T, typename TT, int LANES, int U>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_vec_kernel(NormRopeArgs a, FastDiv parts) {
   constexpr int GROUPS = kWave / LANES;
@@ -348,51 +376,50 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_vec_kernel(NormRope
   const int lane = threadIdx.x & 63, group = lane / LANES, d = (lane % LANES) * 8;
   const bool live = d < a.half;
   const int first = (int)(item - row * parts.d) * (GROUPS * U) + group;
-  const auto chunk = [](const char* base, int64_t element, bool ok) {
-    return ok ? *reinterpret_cast<const uint4*>(base + element * 2) : make_uint4(0u, 0u, 0u, 0u);
-  };
-  uint4 lo[U], hi[U];
+  Chunk8<T> lo[U], hi[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = first + u * GROUPS, kh = h - a.q_heads;
     const bool ok = live && h < a.heads;
     const int64_t at = (kh < 0 ? row * a.q_r + h * a.q_h : row * a.k_r + kh * a.k_h) + d;
-    lo[u] = chunk(kh < 0 ? a.q : a.k, at, ok);
-    hi[u] = chunk(kh < 0 ? a.q : a.k, at + a.half, ok);
-  }
-  float c[8], s[8];
-  {
-    const int64_t at = live ? table_row(a, row) * a.half + d : 0;
-    load_table<TT>(a.cos, at, c);
-    load_table<TT>(a.sin, at, s);
+    lo[u].load(kh < 0 ? a.q : a.k, at, ok);
+    hi[u].load(kh < 0 ? a.q : a.k, at + a.half, ok);
   }
   const int dw = live ? d : 0;
-  const uint4 qw_lo = chunk(a.q_weight, dw, true), qw_hi = chunk(a.q_weight, dw + a.half, true);
-  const uint4 kw_lo = chunk(a.k_weight, dw, true), kw_hi = chunk(a.k_weight, dw + a.half, true);
+  const int64_t at_table = table_row(a, row) * a.half + dw;
+  Chunk8<TT> cos, sin;
+  cos.load(a.cos, at_table);
+  sin.load(a.sin, at_table);
+  Chunk8<T> qw_lo, qw_hi, kw_lo, kw_hi;
+  qw_lo.load(a.q_weight, dw), qw_hi.load(a.q_weight, dw + a.half);
+  kw_lo.load(a.k_weight, dw), kw_hi.load(a.k_weight, dw + a.half);
+  float c[8], s[8];
+  cos.unpack(c);
+  sin.unpack(s);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = first + u * GROUPS, kh = h - a.q_heads;
-    float x[8], y[8], acc = 0.f;
-    unpack8<T>(lo[u], x);
-    unpack8<T>(hi[u], y);
+    float x[8], y[8], wx[8], wy[8], acc = 0.f;
+    lo[u].unpack(x);
+    hi[u].unpack(y);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc = __builtin_fmaf(x[e], x[e], __builtin_fmaf(y[e], y[e], acc));
     const float r = rsqrtf(group_sum(acc, LANES) / (float)(2 * a.half) + a.eps);
-    float wx[8], wy[8];
-    unpack8<T>(kh < 0 ? qw_lo : kw_lo, wx);
-    unpack8<T>(kh < 0 ? qw_hi : kw_hi, wy);
-    uint32_t ox[4] = {0, 0, 0, 0}, oy[4] = {0, 0, 0, 0};
+    (kh < 0 ? qw_lo : kw_lo).unpack(wx);
+    (kh < 0 ? qw_hi : kw_hi).unpack(wy);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float p = x[e] * r * wx[e], q = y[e] * r * wy[e];
-      ox[e >> 1] |= (uint32_t)T::from_float(p * c[e] - q * s[e]) << (16 * (e & 1));
-      oy[e >> 1] |= (uint32_t)T::from_float(q * c[e] + p * s[e]) << (16 * (e & 1));
+      x[e] = p * c[e] - q * s[e];
+      y[e] = q * c[e] + p * s[e];
     }
     if (!live || h >= a.heads) continue;
     const int64_t at = (kh < 0 ? row * a.qo_r + h * a.qo_h : row * a.ko_r + kh * a.ko_h) + d;
     char* out = kh < 0 ? a.q_out : a.k_out;
-    *reinterpret_cast<uint4*>(out + at * 2) = make_uint4(ox[0], ox[1], ox[2], ox[3]);
-    *reinterpret_cast<uint4*>(out + (at + a.half) * 2) = make_uint4(oy[0], oy[1], oy[2], oy[3]);
+    lo[u].pack(x);
+    lo[u].store(out, at);
+    hi[u].pack(y);
+    hi[u].store(out, at + a.half);
   }
 }
 
@@ -551,18 +578,18 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
   a.table_rows = table_rows, a.positions = positions;
   a.rows = rows, a.q_heads = q_heads, a.heads = q_heads + k_heads, a.half = head_dim / 2, a.eps = eps;
   hipStream_t s = (hipStream_t)stream;
-  bool vec = dtype != NHS_F32 && a.half % 8 == 0 && a.half <= 512 &&
+  bool vec = a.half % 8 == 0 && a.half <= 512 &&
              ((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight |
               (uintptr_t)k_weight | (uintptr_t)cos | (uintptr_t)sin) % 16 == 0;
   for (const int64_t stride : {q_row_stride, q_head_stride, k_row_stride, k_head_stride, qo_row_stride,
                                qo_head_stride, ko_row_stride, ko_head_stride})
-    vec = vec && stride % 8 == 0;
+    vec = vec && stride * esize % 16 == 0;
   if (vec) {
     int lanes = 1;
     while (lanes * 8 < a.half) lanes *= 2;
     const int groups = kWave / lanes, per_wave = (a.heads + groups - 1) / groups;  // rounds of a wave that takes a row
     const bool wide = (int64_t)rows * per_wave >= kNormRopeWide;
-    const int u = wide ? 4 : 1;
+    const int u = wide ? 2 : 1;
     const int64_t parts = (per_wave + u - 1) / u, waves = rows * parts;
     if (waves <= 0x7fffffff) {
       const dim3 grid((unsigned)((waves + 3) / 4)), block(kRopeThreads);
@@ -571,7 +598,7 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
         using TT = decltype(table);
         constexpr int L = decltype(l)::value;
         if (wide)
-          launch(qk_norm_rope_vec_kernel<T, TT, L, 4>, grid, block, 0, s, ev.start, ev.stop, a,
+          launch(qk_norm_rope_vec_kernel<T, TT, L, 2>, grid, block, 0, s, ev.start, ev.stop, a,
                  FastDiv((uint32_t)parts));
         else
           launch(qk_norm_rope_vec_kernel<T, TT, L, 1>, grid, block, 0, s, ev.start, ev.stop, a,
@@ -596,8 +623,10 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
       };
       if (dtype == NHS_BF16)
         by_table(BF16T{});
-      else
+      else if (dtype == NHS_F16)
         by_table(F16T{});
+      else
+        by_lanes(F32T{}, F32T{});
       return launch_status(who);
     }
   }
