@@ -56,8 +56,10 @@ __device__ __forceinline__ int pf_v_slot(int r, int c) {
   return D == 128 ? c ^ (4 * (r & 3)) : c ^ (4 * ((r >> 1) & 1));
 }
 
-constexpr int kPfVmcnt0 = 0x0f70;    // s_waitcnt vmcnt(0), the other counters left alone
-constexpr int kPfLgkmcnt0 = 0xc07f;  // s_waitcnt lgkmcnt(0); both: kPfVmcnt0 & kPfLgkmcnt0
+// s_waitcnt vmcnt(n), the other counters left alone; with kPfLgkmcnt0: & lgkmcnt(0)
+constexpr int pf_vmcnt(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
+constexpr int kPfVmcnt0 = pf_vmcnt(0);
+constexpr int kPfLgkmcnt0 = 0xc07f | 0xf;
 
 // 16 bytes per lane from global memory to LDS at `dst` (uniform over the wave) + 16 * lane
 __device__ __forceinline__ void pf_load_lds(const char* src, char* dst) {

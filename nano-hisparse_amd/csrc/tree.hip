@@ -206,8 +206,7 @@ __global__ __launch_bounds__(kTgThreads) void tree_general_kernel(TreeArgs a) {
 
 // ---- 16-bit heads of 64 and 128 on the matrix cores ----
 
-// rows whose addresses are in LDS at a time: with four waves of queries half as many, so that two workgroups share a CU
-constexpr int tf_stage(int qw) { return qw == 4 ? 1024 : 2048; }
+constexpr int kTfStage = 2048;  // rows whose addresses are in LDS at a time
 __device__ __attribute__((aligned(256))) char tree_zeros[256];  // read in place of a masked row
 
 // QW waves hold 32 query rows each; KW such sets share the keys (KW tiles of
@@ -215,7 +214,7 @@ __device__ __attribute__((aligned(256))) char tree_zeros[256];  // read in place
 // S^T = K Q^T and O^T = V^T P^T, tiles straight from global memory to LDS.
 //
 // Every row of a tile has an address of its own, so a stage of up to 2048 rows
-// (tf_stage) is turned into addresses in LDS first (a masked row's is that of zeros, and
+// is turned into addresses in LDS first (a masked row's is that of zeros, and
 // its bit of the tile's word is clear); the loads of a round then need one LDS
 // read each. The drafted keys are a last round of the last split. A masked
 // weight is 0, which a matrix core would multiply with whatever V holds, so
@@ -233,9 +232,10 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
   constexpr int kTile = BN * D * 2;            // bytes
   constexpr int kRound = BN * KW;              // keys
-  constexpr int kTfStage = tf_stage(QW);
   constexpr unsigned kDraft = T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;  // exponent bits of NaN and infinities
   static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1, "tile shape");
+  // Tiles under names of their own, used by rounds in turn: the compiler then knows that reads of one need not wait for
+  // loads into the others.
   __shared__ __attribute__((aligned(16))) char k0[KW * kTile], k1[KW * kTile];
   __shared__ __attribute__((aligned(16))) char v0[KW * kTile], v1[KW * kTile];
   __shared__ __attribute__((aligned(16))) int64_t stage[kTfStage];
@@ -311,6 +311,15 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         const uint4 kf = *reinterpret_cast<const uint4*>(kl + x * 32 * D * 2 + pf_k_slot<D>(n, 2 * st + half) * 16);
         s[x] = mfma32x32x16<T>(kf, qf[st], s[x]);
       }
+    if constexpr (D == 128 && NB == 2) {  // as in the prompt attention: eight K reads ahead of the MFMAs
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
+    }
 #pragma unroll
     for (int x = 0; x < NB; ++x)
       if (__any(seen[x] != 0xffffffffu)) {
@@ -362,8 +371,24 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
 
   const int begin = split * a.rows_per_split, end = min(a.n_rows, begin + a.rows_per_split);
   const int64_t* rows = a.rows + (int64_t)b * a.r_b;
-  for (int s0 = begin; s0 < end; s0 += kTfStage) {
-    const int count = min(kTfStage, end - s0), rounds = (count + kRound - 1) / kRound;
+  const bool draft = split == a.n_splits - 1;
+  uint64_t present = 0;  // drafted nodes
+  if (draft) {  // the drafted keys as they lie (node j is key j of a round), asked for before the rows' indices are read
+    present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
+    if (tid == 0) odd = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int row = (i * QW + wave) * kRows + lrow, j = share * BN + row;
+      const bool ok = j < a.nodes && (present >> j & 1);
+      const int dst = share * kTile + (i * QW + wave) * 1024;
+      const char* ks = ok ? a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2 : tree_zeros;
+      const char* vs = ok ? a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 : tree_zeros;
+      pf_load_lds(ks + pf_k_slot<D>(row, lchunk) * 16, k0 + dst);
+      pf_load_lds(vs + pf_v_slot<D>(row, lchunk) * 16, v0 + dst);
+    }
+  }
+  for (int s0 = begin; s0 < end || s0 == begin; s0 += kTfStage) {
+    const int count = min(kTfStage, max(end - s0, 0)), rounds = (count + kRound - 1) / kRound;
     if (s0 != begin) __syncthreads();  // the last stage's addresses and tiles are read
     for (int i = tid; i < rounds * kRound; i += THREADS) {
       const int64_t at = i < count ? rows[(int64_t)(s0 + i) * a.r_c] : -1;
@@ -377,7 +402,33 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         words[i / 32 + 1] = (uint32_t)(live_rows >> 32);
       }
     }
+    if (draft && s0 == begin) __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
     __syncthreads();
+    if (rounds > 0) load_tile(0, k1, v1);
+    if (draft && s0 == begin) {
+      for (int c = tid; c < min(a.nodes, kRound) * C; c += THREADS) {
+        uint4* p = reinterpret_cast<uint4*>(v0) + c;  // rows lie one after another, shares too
+        uint32_t w[4] = {p->x, p->y, p->z, p->w};
+        bool found = false;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const bool lo = (w[x] & kDraft) == kDraft, hi = (w[x] >> 16 & kDraft) == kDraft;
+          found |= lo || hi;
+          w[x] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+        if (found) {
+          *p = make_uint4(w[0], w[1], w[2], w[3]);
+          odd = 1;
+        }
+      }
+      __syncthreads();
+      if (share * BN < a.nodes) {
+        uint32_t seen[NB];
+#pragma unroll
+        for (int x = 0; x < NB; ++x) seen[x] = (uint32_t)((word & present) >> (share * BN + 32 * x));
+        tile(k0, v0, seen);
+      }
+    }
     auto round = [&](int t, char* kb, char* vb, char* kb_next, char* vb_next) {
       // this wave's loads of round t are in; after the barrier every wave's are, and every wave is done with the other
       // buffers, which take round t + 1
@@ -388,61 +439,21 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         __builtin_amdgcn_s_waitcnt(kPfVmcnt0 & kPfLgkmcnt0);
         asm volatile("" ::: "memory");
       }
-      if (t + 1 < rounds) load_tile(t + 1, kb_next, vb_next);
       uint32_t seen[NB];
+#pragma unroll
+      for (int x = 0; x < NB; ++x) seen[x] = words[(t * kRound + share * BN) / 32 + x];
+      if (t + 1 < rounds) load_tile(t + 1, kb_next, vb_next);
       bool some = false;
 #pragma unroll
       for (int x = 0; x < NB; ++x) {
-        seen[x] = __builtin_amdgcn_readfirstlane(words[(t * kRound + share * BN) / 32 + x]);
+        seen[x] = __builtin_amdgcn_readfirstlane(seen[x]);
         some |= seen[x] != 0;
       }
       if (some) tile(kb, vb, seen);
     };
-    load_tile(0, k0, v0);
     for (int t = 0; t < rounds; t += 2) {
-      round(t, k0, v0, k1, v1);
-      if (t + 1 < rounds) round(t + 1, k1, v1, k0, v0);
-    }
-  }
-
-  uint64_t present = 0;  // drafted nodes
-  if (split == a.n_splits - 1) {  // the drafted keys, as they lie: node j of the round is key j
-    __syncthreads();
-    present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
-    if (tid == 0) odd = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int row = (i * QW + wave) * kRows + lrow, j = share * BN + row;
-      const bool ok = j < a.nodes && (present >> j & 1);
-      const int dst = share * kTile + (i * QW + wave) * 1024;
-      const char* ks = ok ? a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2 : tree_zeros;
-      const char* vs = ok ? a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 : tree_zeros;
-      pf_load_lds(ks + pf_k_slot<D>(row, lchunk) * 16, k0 + dst);
-      pf_load_lds(vs + pf_v_slot<D>(row, lchunk) * 16, v0 + dst);
-    }
-    __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
-    __syncthreads();
-    for (int c = tid; c < min(a.nodes, kRound) * C; c += THREADS) {
-      uint4* p = reinterpret_cast<uint4*>(v0) + c;  // rows lie one after another, shares too
-      uint32_t w[4] = {p->x, p->y, p->z, p->w};
-      bool found = false;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const bool lo = (w[x] & kDraft) == kDraft, hi = (w[x] >> 16 & kDraft) == kDraft;
-        found |= lo || hi;
-        w[x] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-      }
-      if (found) {
-        *p = make_uint4(w[0], w[1], w[2], w[3]);
-        odd = 1;
-      }
-    }
-    __syncthreads();
-    if (share * BN < a.nodes) {
-      uint32_t seen[NB];
-#pragma unroll
-      for (int x = 0; x < NB; ++x) seen[x] = (uint32_t)((word & present) >> (share * BN + 32 * x));
-      tile(k0, v0, seen);
+      round(t, k1, v1, k0, v0);
+      if (t + 1 < rounds) round(t + 1, k0, v0, k1, v1);
     }
   }
 
@@ -450,10 +461,9 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   if constexpr (KW > 1) {
     // the waves of the other shares hand their sums over through the tile buffers, one share at a time (registers by
     // lane: the partners hold the same query rows and dims)
-    float* part = reinterpret_cast<float*>(wave < (QW + 1) / 2 ? k0 : v0) +
-                  (wave < (QW + 1) / 2 ? wave : wave - (QW + 1) / 2) * (DB * 16 * kWave) + lane;
+    float* part = reinterpret_cast<float*>(wave == 0 ? k0 : wave == 1 ? v0 : wave == 2 ? k1 : v1) + lane;
     float* stat = reinterpret_cast<float*>(stage) + wave * 2 * kWave + lane;
-    static_assert((QW + 1) / 2 * DB * 16 * kWave * 4 <= KW * kTile && QW * 2 * kWave * 4 <= kTfStage * 8, "merge space");
+    static_assert(QW <= 4 && DB * 16 * kWave * 4 <= KW * kTile && QW * 2 * kWave * 4 <= kTfStage * 8, "merge space");
     for (int from = 1; from < KW; ++from) {
       __syncthreads();
       if (share == from) {
@@ -481,7 +491,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     if (share) return;
   }
   if (!live) return;
-  if (split == a.n_splits - 1 && odd) {
+  if (draft && odd) {
     for (int j = 0; j < a.nodes; ++j) {
       if (!((word & present) >> j & 1)) continue;
       const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 + half * 8;
@@ -520,28 +530,111 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     }
 }
 
-// Joins the splits of every output row, one wave per row: the sums are scaled
-// to the largest of the splits' maxima, added and divided.
-template <typename T>
+// Joins the splits of every output row: the sums are scaled to the largest of
+// the splits' maxima, added and divided. WAVES waves of a workgroup share a row
+// (four where there are more than 16 splits: few rows, long chains of loads);
+// LANES lanes of four dims read one split while the others read the next ones,
+// all the splits of a wave in flight at once.
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
+  constexpr int LANES = D / 4, SIDE = kWave / LANES, U = 16 / SIDE;
+  __shared__ __attribute__((aligned(16))) float part[WAVES > 1 ? 4 : 1][WAVES > 1 ? D : 4];
+  __shared__ float stat[WAVES > 1 ? 4 : 1][2];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t out_row = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (out_row >= a.out_rows) return;  // (a whole workgroup or a wave without barriers)
+  const int64_t bn = out_row / a.q_heads;
+  const int head = (int)(out_row - bn * a.q_heads);
+  const int b = (int)(bn / a.nodes), node = (int)(bn - (int64_t)b * a.nodes);
+  const bool present = a.mask[(int64_t)b * a.mask_b + node] != 0;
+  const int side = lane / LANES, d = lane % LANES * 4;
+  const int each = (a.n_splits + WAVES - 1) / WAVES, begin = WAVES > 1 ? wave * each : 0;
+  const int end = min(begin + each, a.n_splits);
+  float top = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = begin; s0 < end; s0 += SIDE * U) {
+    float4 p[U];
+    float2 st[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (int64_t)min(s0 + u * SIDE + side, end - 1) * a.out_rows + out_row;
+      p[u] = *reinterpret_cast<const float4*>(a.partial + at * D + d);
+      st[u] = *reinterpret_cast<const float2*>(a.stats + 2 * at);
+    }
+    float moved = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) moved = fmaxf(moved, st[u].x);
+    const float ref = moved == -INFINITY ? 0.f : moved, alpha = __builtin_amdgcn_exp2f(top - ref);
+    top = moved;
+    total *= alpha;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= alpha;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * SIDE + side >= end) continue;
+      const float f = __builtin_amdgcn_exp2f(st[u].x - ref);
+      total = __builtin_fmaf(f, st[u].y, total);
+      o[0] = __builtin_fmaf(f, p[u].x, o[0]), o[1] = __builtin_fmaf(f, p[u].y, o[1]);
+      o[2] = __builtin_fmaf(f, p[u].z, o[2]), o[3] = __builtin_fmaf(f, p[u].w, o[3]);
+    }
+  }
+  // the sides, then the waves
+#pragma unroll
+  for (int x = LANES; x < kWave; x <<= 1) {
+    const float m2 = __shfl_xor(top, x), both = fmaxf(top, m2), ref = both == -INFINITY ? 0.f : both;
+    const float f1 = __builtin_amdgcn_exp2f(top - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+    total = total * f1 + __shfl_xor(total, x) * f2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f1 + __shfl_xor(o[e], x) * f2;
+    top = both;
+  }
+  if constexpr (WAVES > 1) {
+    if (side == 0) *reinterpret_cast<float4*>(&part[wave][d]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) stat[wave][0] = top, stat[wave][1] = total;
+    __syncthreads();
+    if (wave) return;
+    for (int w = 1; w < WAVES; ++w) {
+      const float m2 = stat[w][0], both = fmaxf(top, m2), ref = both == -INFINITY ? 0.f : both;
+      const float f1 = __builtin_amdgcn_exp2f(top - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+      const float4 q = *reinterpret_cast<const float4*>(&part[w][d]);
+      total = total * f1 + stat[w][1] * f2;
+      o[0] = o[0] * f1 + q.x * f2, o[1] = o[1] * f1 + q.y * f2;
+      o[2] = o[2] * f1 + q.z * f2, o[3] = o[3] * f1 + q.w * f2;
+      top = both;
+    }
+  }
+  if (side) return;
+  const bool some = present && top != -INFINITY;
+  const int64_t at = (int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_elem(a.out, T::dtype, at + e, some ? o[e] / total : 0.f);
+}
+
+// The same for every head_dim, one wave per row and a dim per lane.
+template <typename T>
+__global__ __launch_bounds__(256) void tree_join_general_kernel(TreeArgs a) {
   const int64_t out_row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (out_row >= a.out_rows) return;
   const int lane = threadIdx.x & 63, D = a.head_dim;
   const int64_t bn = out_row / a.q_heads;
   const int head = (int)(out_row - bn * a.q_heads);
   const int b = (int)(bn / a.nodes), node = (int)(bn - (int64_t)b * a.nodes);
-  float top = -INFINITY;
-  for (int s = 0; s < a.n_splits; ++s) top = fmaxf(top, a.stats[2 * ((int64_t)s * a.out_rows + out_row)]);
+  float top = -INFINITY, total = 0.f;
+  for (int s = lane; s < a.n_splits; s += kWave) top = fmaxf(top, a.stats[2 * ((int64_t)s * a.out_rows + out_row)]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float ref = top == -INFINITY ? 0.f : top;
   const bool some = a.mask[(int64_t)b * a.mask_b + node] != 0 && top != -INFINITY;
+  for (int s = lane; s < a.n_splits; s += kWave) {
+    const float* st = a.stats + 2 * ((int64_t)s * a.out_rows + out_row);
+    total = __builtin_fmaf(__builtin_amdgcn_exp2f(st[0] - ref), st[1], total);
+  }
+  total = group_sum(total, kWave);
   const int64_t at = (int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h;
   for (int d = lane; d < D; d += kWave) {
-    float total = 0.f, o = 0.f;
+    float o = 0.f;
     for (int s = 0; s < a.n_splits; ++s) {
       const int64_t p = (int64_t)s * a.out_rows + out_row;
-      const float f = __builtin_amdgcn_exp2f(a.stats[2 * p] - ref);
-      total = __builtin_fmaf(f, a.stats[2 * p + 1], total);
-      o = __builtin_fmaf(f, a.partial[p * D + d], o);
+      o = __builtin_fmaf(__builtin_amdgcn_exp2f(a.stats[2 * p] - ref), a.partial[p * D + d], o);
     }
     store_elem(a.out, T::dtype, at + d, some ? o / total : 0.f);
   }
@@ -561,9 +654,9 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
   s.waves = s.shares = 0;
   if (flash) {
     s.waves = query_rows <= 32 ? 1 : query_rows <= 64 ? 2 : 4;
-    s.shares = 4 / s.waves;
+    s.shares = s.waves == 1 ? 4 : 2;
     block_rows = 32 * s.waves;
-    per_cu = s.waves == 4 ? 2 : 1;
+    per_cu = 1;
     least = 128;
   }
   s.row_blocks = (query_rows + block_rows - 1) / block_rows;
@@ -674,28 +767,35 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   a.partial = a.stats + 2 * a.out_rows * shape.n_splits;
   hipStream_t s = (hipStream_t)stream;
   const hipEvent_t none = nullptr;
-  const auto run = [&](auto kernel, auto join, int threads) {
+  const auto run = [&](auto kernel, auto join, int threads, int rows_each) {
     const bool joined = shape.n_splits > 1;
     launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, s, ev.start, joined ? none : ev.stop, a);
-    if (joined) launch(join, dim3((unsigned)((a.out_rows + 3) / 4)), dim3(256), 0, s, none, ev.stop, a);
+    if (joined)
+      launch(join, dim3((unsigned)((a.out_rows + rows_each - 1) / rows_each)), dim3(256), 0, s, none, ev.stop, a);
   };
   const auto general = [&](auto tag) {
     using T = decltype(tag);
     if (head_dim <= 128)
-      run(tree_general_kernel<T, 32, 128>, tree_join_kernel<T>, kTgThreads);
+      run(tree_general_kernel<T, 32, 128>, tree_join_general_kernel<T>, kTgThreads, 4);
     else
-      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_kernel<T>, kTgThreads);
+      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_general_kernel<T>, kTgThreads, 4);
   };
   const auto on_mfma = [&](auto tag, auto dim) {
     using T = decltype(tag);
     constexpr int D = decltype(dim)::value;
     const int threads = shape.waves * shape.shares * kWave;
+    const auto go = [&](auto kernel) {
+      if (shape.n_splits > 16)
+        run(kernel, tree_join_kernel<T, D, 4>, threads, 1);
+      else
+        run(kernel, tree_join_kernel<T, D, 1>, threads, 4);
+    };
     if (shape.waves == 1)
-      run(tree_flash_kernel<T, D, 1, 4, 32>, tree_join_kernel<T>, threads);
+      go(tree_flash_kernel<T, D, 1, 4, 32>);
     else if (shape.waves == 2)
-      run(tree_flash_kernel<T, D, 2, 2, 64>, tree_join_kernel<T>, threads);
+      go(tree_flash_kernel<T, D, 2, 2, 64>);
     else
-      run(tree_flash_kernel<T, D, 4, 1, 64>, tree_join_kernel<T>, threads);
+      go(tree_flash_kernel<T, D, 4, 2, 64>);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

@@ -554,8 +554,9 @@ def test_qk_norm_rope_in_place_and_layouts(gpu, dtype):
     check_norm(c, expected, c["at"], 1e-5)
     same = rk.qk_norm_rope(c["q"].clone().transpose(0, 1).contiguous().transpose(0, 1), c["k"].contiguous(), *args)
     assert all(torch.equal(a, b) for a, b in zip(same, expected))
+    # heads at any element: another order of the squares' sum, within the bound that holds for every order
     off = torch.zeros(13 * 7 * 67 + 1, dtype=dtype, device=gpu)[1:].view(13, 7, 67)[:, :6, :64].copy_(c["q"])
-    assert all(torch.equal(a, b) for a, b in zip(rk.qk_norm_rope(off, c["k"], *args), expected))
+    check_norm(c, rk.qk_norm_rope(off, c["k"], *args), c["at"], 1e-5)
     wide = torch.full((15, 10, 80), 3.0, dtype=dtype, device=gpu)
     outs = wide[1:14, 1:7, 8:72], wide[1:14, 7:9, 8:72]
     rk.qk_norm_rope(c["q"], c["k"], *args, out=outs)
