@@ -374,18 +374,17 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   const bool draft = split == a.n_splits - 1;
   uint64_t present = 0;  // drafted nodes
   if (draft) {  // the drafted keys as they lie (node j is key j of a round), asked for before the rows' indices are read
-    present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
-    if (tid == 0) odd = 0;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int row = (i * QW + wave) * kRows + lrow, j = share * BN + row;
-      const bool ok = j < a.nodes && (present >> j & 1);
+      const int row = (i * QW + wave) * kRows + lrow, j = min(share * BN + row, a.nodes - 1);
       const int dst = share * kTile + (i * QW + wave) * 1024;
-      const char* ks = ok ? a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2 : tree_zeros;
-      const char* vs = ok ? a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 : tree_zeros;
+      const char* ks = a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2;
+      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2;
       pf_load_lds(ks + pf_k_slot<D>(row, lchunk) * 16, k0 + dst);
       pf_load_lds(vs + pf_v_slot<D>(row, lchunk) * 16, v0 + dst);
     }
+    present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
+    if (tid == 0) odd = 0;
   }
   for (int s0 = begin; s0 < end || s0 == begin; s0 += kTfStage) {
     const int count = min(kTfStage, max(end - s0, 0)), rounds = (count + kRound - 1) / kRound;
@@ -405,55 +404,58 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     if (draft && s0 == begin) __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
     __syncthreads();
     if (rounds > 0) load_tile(0, k1, v1);
-    if (draft && s0 == begin) {
-      for (int c = tid; c < min(a.nodes, kRound) * C; c += THREADS) {
-        uint4* p = reinterpret_cast<uint4*>(v0) + c;  // rows lie one after another, shares too
+    const bool with_draft = draft && s0 == begin;
+    if (with_draft) {  // zeros for the values of absent nodes (those past the last are copies of it), NaN and infinities
+      for (int c = tid; c < kTreeNodes * C; c += THREADS) {  // rows lie one after another, shares too
+        uint4* p = reinterpret_cast<uint4*>(v0) + c;
+        const bool here = present >> (c / C) & 1;
         uint32_t w[4] = {p->x, p->y, p->z, p->w};
         bool found = false;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const bool lo = (w[x] & kDraft) == kDraft, hi = (w[x] >> 16 & kDraft) == kDraft;
           found |= lo || hi;
-          w[x] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          w[x] = here ? w[x] & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u)) : 0u;
         }
-        if (found) {
-          *p = make_uint4(w[0], w[1], w[2], w[3]);
-          odd = 1;
-        }
+        if (found || !here) *p = make_uint4(w[0], w[1], w[2], w[3]);
+        if (found && here) odd = 1;
       }
       __syncthreads();
-      if (share * BN < a.nodes) {
-        uint32_t seen[NB];
-#pragma unroll
-        for (int x = 0; x < NB; ++x) seen[x] = (uint32_t)((word & present) >> (share * BN + 32 * x));
-        tile(k0, v0, seen);
-      }
     }
+    // round t of the stage's rows; t = -1: the draft, whose tile is in place
     auto round = [&](int t, char* kb, char* vb, char* kb_next, char* vb_next) {
-      // this wave's loads of round t are in; after the barrier every wave's are, and every wave is done with the other
-      // buffers, which take round t + 1
-      if constexpr (QW > 1) {
-        __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
-        __syncthreads();
-      } else {  // the wave's reads of the other buffers are back too
-        __builtin_amdgcn_s_waitcnt(kPfVmcnt0 & kPfLgkmcnt0);
-        asm volatile("" ::: "memory");
-      }
       uint32_t seen[NB];
+      bool some;
+      if (t >= 0) {
+        // this wave's loads of round t are in; after the barrier every wave's are, and every wave is done with the
+        // other buffers, which take round t + 1
+        if constexpr (QW > 1) {
+          __builtin_amdgcn_s_waitcnt(kPfVmcnt0);
+          __syncthreads();
+        } else {  // the wave's reads of the other buffers are back too
+          __builtin_amdgcn_s_waitcnt(kPfVmcnt0 & kPfLgkmcnt0);
+          asm volatile("" ::: "memory");
+        }
 #pragma unroll
-      for (int x = 0; x < NB; ++x) seen[x] = words[(t * kRound + share * BN) / 32 + x];
-      if (t + 1 < rounds) load_tile(t + 1, kb_next, vb_next);
-      bool some = false;
+        for (int x = 0; x < NB; ++x) seen[x] = words[(t * kRound + share * BN) / 32 + x];
+        if (t + 1 < rounds) load_tile(t + 1, kb_next, vb_next);
+        some = false;
 #pragma unroll
-      for (int x = 0; x < NB; ++x) {
-        seen[x] = __builtin_amdgcn_readfirstlane(seen[x]);
-        some |= seen[x] != 0;
+        for (int x = 0; x < NB; ++x) {
+          seen[x] = __builtin_amdgcn_readfirstlane(seen[x]);
+          some |= seen[x] != 0;
+        }
+      } else {
+        some = share * BN < a.nodes;
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+          seen[x] = some ? (uint32_t)((word & present) >> (share * BN + 32 * x)) : 0u;
       }
       if (some) tile(kb, vb, seen);
     };
-    for (int t = 0; t < rounds; t += 2) {
-      round(t, k1, v1, k0, v0);
-      if (t + 1 < rounds) round(t + 1, k0, v0, k1, v1);
+    for (int t = -1; t < rounds; t += 2) {
+      if (t >= 0 || with_draft) round(t, k0, v0, k1, v1);
+      if (t + 1 < rounds) round(t + 1, k1, v1, k0, v0);
     }
   }
 

@@ -399,6 +399,21 @@ def test_a_draft_s_infinities_reach_its_descendants_only(gpu, dtype, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D,T", [(bf16, 128, 9), (f16, 64, 3), (bf16, 128, 20), (f16, 128, 33), (f32, 32, 9)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_the_last_node_s_value_reaches_no_other(gpu, dtype, D, T, value):
+    """Nor its key: tiles hold more keys than the tree has nodes."""
+    print("case:", dict(dtype=dtype, D=D, T=T, value=value), flush=True)
+    c = tree_case(gpu, dtype, 2, T, 8, 2, D, 16, 70, seed=T, fused=False)
+    c["mask"] = plan_oracle(torch.tensor([[-1] + [0] * (T - 1)] * 2, dtype=torch.int32), torch.zeros(2).long())[0].to(gpu)
+    expected, tol = tree_oracle(*(c[n] for n in ("q", "pool", "rows", "k", "v", "mask", "page")), dtype != f32)
+    c["v"][:, T - 1], c["k"][:, T - 1] = value, value
+    got = run_tree(c)
+    check(got[:, : T - 1], expected[:, : T - 1], tol[:, : T - 1])
+    assert not got[:, T - 1].isfinite().any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [bf16, f32])
 def test_infinite_keys_of_the_past(gpu, dtype):
     """A key of -inf against a positive query scores -inf (weight 0); NaN keys make their readers NaN, no one else."""
