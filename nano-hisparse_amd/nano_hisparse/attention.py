@@ -39,3 +39,33 @@ def row_attention(query, cache, request_id, layer, topk, backend="auto"):
         from .row_kernels import cpu_provider
 
         return cpu_provider("row_attention").attend_rows(query, cache.pool, rows, cache.config)
+
+
+@torch.inference_mode()
+def tree_row_attention(query, k, v, mask, cache, request_id, layer, topk, backend="auto"):
+    """row_attention for the drafted nodes of a request (query [nodes,
+    q_heads, head_dim]) over the rows of one selection that all nodes share
+    and over the drafted keys and values k, v [nodes, kv_heads, head_dim]
+    that mask [nodes] (int64, see row_kernels.tree_plan) lets each node see."""
+    if backend not in BACKENDS:
+        raise ValueError("invalid attention backend")
+    cfg = cache.config
+    if query.ndim != 3 or query.shape[2] != cfg.head_dim:
+        raise ValueError("invalid query shape")
+    if query.shape[1] % cfg.kv_heads or query.device != cache.pool.device:
+        raise ValueError("query GQA/device mismatch")
+    if k.shape != (len(query), cfg.kv_heads, cfg.head_dim) or v.shape != k.shape:
+        raise ValueError("expected one K/V row per node")
+    if topk.head_columns is not None:
+        raise ValueError("a tree's nodes and heads share one selection")
+    if backend == "triton" and not cache.storage.cuda:
+        raise ValueError("Triton requires CUDA")
+    with cache.resolve(request_id, layer, topk) as lease:
+        rows = lease.plan.physical_rows[None]
+        if cache.storage.cuda:
+            from .row_kernels import tree_attention
+        else:
+            from .row_kernels import cpu_provider
+
+            tree_attention = cpu_provider("tree_row_attention").tree_attention
+        return tree_attention(query[None], cache.pool, rows, k[None], v[None], mask[None], cfg.page_size)[0]

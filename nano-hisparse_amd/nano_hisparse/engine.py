@@ -10,8 +10,20 @@ from __future__ import annotations
 from collections import deque
 from dataclasses import dataclass, field
 
+from . import row_kernels as rk
 from .config import CapacityError
 from .model import Model
+
+
+@dataclass
+class TokenInfo:
+    """A generated token's log probability, the entropy of the distribution
+    that it was chosen from and the most likely tokens, (id, log probability)."""
+
+    token: int
+    logprob: float
+    entropy: float
+    top: list
 
 
 @dataclass
@@ -24,16 +36,31 @@ class Request:
     decode_count: int = 0
     finished: bool = False
     cancelled: bool = False
+    logprobs: list = field(default_factory=list)  # a TokenInfo per generated token (Engine(logprobs=...))
+    drafted_count: int = 0  # tokens that a draft proposed, and how many of them were accepted
+    accepted_count: int = 0
 
 
 class Engine:
     def __init__(self, model: Model, cache, top_k=None, backend="auto", eos_token_id=None, selector="quest",
-                 batch_decode=False, micro_batches=1, graph=False):
+                 batch_decode=False, micro_batches=1, graph=False, draft=None, logprobs=None):
         """batch_decode=True gives all running requests their decode turn in
         one Model.decode_batch call (GPU cache, Quest top_k; micro_batches=2
         pipelines two halves of the batch; graph=True replays each batch
         composition's step from a captured HIP graph); emission order and
-        admission are unchanged."""
+        admission are unchanged.
+
+        draft(request) may propose what follows a running request: (tokens,
+        parents), a tree of up to 63 tokens whose parents are earlier tokens
+        of the tree, or -1 for one that follows the request's last token. The
+        request's decode turn then verifies the whole tree in one pass
+        (Model.decode_tree) and emits every token of the path that greedy
+        decoding takes, and the one after it; without a proposal (None or no
+        tokens) it is an ordinary turn. Verified turns choose pages by the
+        query of the last token alone, as ordinary ones do.
+
+        logprobs=n records a TokenInfo with the n most likely tokens for
+        every generated token in its request's `logprobs`."""
         cfg, kv = model.config, cache.config
         if (cfg.num_key_value_heads, cfg.head_dim) != (kv.kv_heads, kv.head_dim):
             raise ValueError("model/cache head dimensions differ")
@@ -51,6 +78,12 @@ class Engine:
         self.graph = graph
         if graph and not batch_decode:
             raise ValueError("graph replay needs batch_decode")
+        if draft is not None and batch_decode:
+            raise ValueError("drafts are verified request by request, not with batch_decode")
+        if logprobs is not None and not 0 <= logprobs <= min(rk.MAX_TOP_LOGPROBS, cfg.vocab_size):
+            raise ValueError(f"logprobs must be None or 0 to {rk.MAX_TOP_LOGPROBS}, at most the vocabulary")
+        self.draft = draft
+        self.logprobs = logprobs
         self.requests: dict = {}
         self.waiting: deque = deque()
         self.running: deque = deque()
@@ -74,14 +107,61 @@ class Engine:
         self.waiting.append(request)
         return request
 
-    def _emit(self, request, logits=None, token=None):
-        if token is None:
-            token = int(logits.argmax().item())
+    def _choose(self, logits):
+        """(token, TokenInfo or None) for every row of logits [rows, vocab]."""
+        chosen = logits.argmax(-1)
+        if self.logprobs is None:
+            return [(token, None) for token in chosen.tolist()]
+        kernels = rk if logits.is_cuda else rk.cpu_provider("logprobs")
+        info = kernels.token_logprobs(logits, chosen, self.logprobs)
+        columns = (chosen, *info)
+        return [(token, TokenInfo(token, logprob, entropy, list(zip(ids, values))))
+                for token, logprob, entropy, ids, values in zip(*(c.tolist() for c in columns))]
+
+    def _emit(self, request, choice):
+        token, info = choice
         request.generated.append(token)
+        if info is not None:
+            request.logprobs.append(info)
         if token == self.eos_token_id or len(request.generated) >= request.max_new_tokens:
             request.finished = True
             self.cache.release_request(request.request_id, wait=False)
         return token
+
+    def _decode(self, request):
+        """One decode turn of a request: the tokens it emits."""
+        proposal = self.draft(request) if self.draft is not None else None
+        tokens, parents = proposal if proposal is not None else ((), ())
+        if len(tokens) != len(parents):
+            raise ValueError("a draft is a token list and a parent for each token")
+        if not len(tokens):
+            logits = self.model.decode(
+                request.generated[-1], request.request_id, self.cache, self.top_k, self.backend,
+                selector=self.selector,
+            )
+            request.decode_count += 1
+            return [self._emit(request, self._choose(logits[None])[0])]
+        tree = [request.generated[-1], *tokens]
+        above = [-1, *(p + 1 for p in parents)]
+        if min(above[1:]) < 0:
+            raise ValueError("a drafted token's parent is -1 or a token before it")
+        step = self.model.decode_tree(
+            tree, above, request.request_id, self.cache, self.top_k, self.backend, selector=self.selector,
+        )
+        choices = self._choose(step.logits)
+        request.decode_count += 1
+        request.drafted_count += len(tokens)
+        emitted, path, node = [], [], 0
+        while node is not None:
+            path.append(node)
+            emitted.append(self._emit(request, choices[node]))
+            if request.finished:
+                break
+            node = next((t for t in range(node + 1, len(tree)) if above[t] == node and tree[t] == emitted[-1]), None)
+        request.accepted_count += len(path) - 1
+        if not request.finished:
+            step.commit(path)
+        return emitted
 
     def _admit(self, request):
         layers = self.model.config.num_hidden_layers
@@ -99,7 +179,8 @@ class Engine:
             return True
 
     def step(self):
-        """Admit at most one prompt, then one decode turn per running request.
+        """Admit at most one prompt, then one decode turn per running request
+        (several tokens where a draft's were accepted).
 
         Returns [(request_id, token)] in emission order.
         """
@@ -109,7 +190,7 @@ class Engine:
             request = self.waiting.popleft()
             logits = self.model.prefill(request.prompt, self.cache, request.request_id)
             request.prefill_count += 1
-            emitted.append((request.request_id, self._emit(request, logits)))
+            emitted.append((request.request_id, self._emit(request, self._choose(logits[None])[0])))
             if not request.finished:
                 self.running.append(request)
         if self.batch_decode and self.running:
@@ -119,20 +200,16 @@ class Engine:
                 [r.generated[-1] for r in batch], [r.request_id for r in batch], self.cache, self.top_k,
                 micro_batches=self.micro_batches, graph=self.graph,
             )
-            for request, token in zip(batch, logits.argmax(-1).tolist()):
+            for request, choice in zip(batch, self._choose(logits)):
                 request.decode_count += 1
-                emitted.append((request.request_id, self._emit(request, token=token)))
+                emitted.append((request.request_id, self._emit(request, choice)))
                 if not request.finished:
                     self.running.append(request)
             return emitted
         for _ in range(len(self.running)):
-            request = self.running.popleft()
-            logits = self.model.decode(
-                request.generated[-1], request.request_id, self.cache, self.top_k, self.backend,
-                selector=self.selector,
-            )
-            request.decode_count += 1
-            emitted.append((request.request_id, self._emit(request, logits)))
+            request = self.running[0]  # stays there if its turn raises
+            emitted += [(request.request_id, token) for token in self._decode(request)]
+            self.running.popleft()
             if not request.finished:
                 self.running.append(request)
         return emitted

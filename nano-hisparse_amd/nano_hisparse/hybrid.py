@@ -609,6 +609,21 @@ class HybridKVCache:
         topk = LogicalTopK.from_selection(selection, query.device)
         return row_attention(query, self, request_id, layer, topk, backend)
 
+    def tree_attention(self, query, k, v, mask, request_id, layer, selection, backend="auto"):
+        """attention for a tree of drafted nodes: query [nodes, q_heads,
+        head_dim] over the selected rows (one selection for all nodes) and
+        the drafted keys and values k, v [nodes, kv_heads, head_dim], which
+        are not in the cache, as far as mask [nodes] lets each node see them."""
+        from .attention import tree_row_attention
+
+        length = self.storage.requests[request_id].lengths[layer]
+        if selection.length != length or selection.page_size != self.config.page_size:
+            raise ValueError("selection has stale length or wrong page size")
+        if query.ndim != 3 or selection.heads != query.shape[1]:
+            raise ValueError("selection must have one row per query head")
+        topk = LogicalTopK.from_selection(selection, query.device)
+        return tree_row_attention(query, k, v, mask, self, request_id, layer, topk, backend)
+
     def resolve(self, request_id, layer, topk: LogicalTopK):
         """Resolve `topk` for one layer and gather its misses; returns a
         RowLease whose `.plan` holds the physical rows (reference

@@ -25,6 +25,7 @@ from .selection import Selection, quest_selection, select_pages
 from .storage import upload
 
 
+SCORE_ROWS = 1024  # rows of logits that Model.score has at a time
 ROPE_TABLE_ROWS = 1 << 17  # longest cos/sin tables a model keeps (32 MB at head_dim 128 in 16 bits)
 
 
@@ -38,6 +39,7 @@ class ModelConfig:
     num_key_value_heads: int = 2
     rms_norm_eps: float = 1e-6
     rope_theta: float = 10000.0
+    qk_norm: bool = False  # RMSNorm of every query and key head before its rotation
 
     @property
     def head_dim(self):
@@ -71,6 +73,9 @@ class Projections(nn.Module):
         self.k_proj = nn.Linear(cfg.hidden_size, kv_width, bias=True)
         self.v_proj = nn.Linear(cfg.hidden_size, kv_width, bias=True)
         self.o_proj = nn.Linear(cfg.hidden_size, cfg.hidden_size, bias=False)
+        if cfg.qk_norm:
+            self.q_norm = RMSNorm(cfg.head_dim, cfg.rms_norm_eps)
+            self.k_norm = RMSNorm(cfg.head_dim, cfg.rms_norm_eps)
 
 
 class MLP(nn.Module):
@@ -123,7 +128,7 @@ class Model(nn.Module):
         hf = AutoModelForCausalLM.from_pretrained(name, torch_dtype=dtype).eval().to(device)
         model = cls.__new__(cls)
         nn.Module.__init__(model)
-        fields = {f: getattr(hf_cfg, f) for f in ModelConfig.__dataclass_fields__ if f != "rope_theta"}
+        fields = {f: getattr(hf_cfg, f) for f in ModelConfig.__dataclass_fields__ if f not in ("rope_theta", "qk_norm")}
         fields["rope_theta"] = rope.get("rope_theta", getattr(hf_cfg, "rope_theta", 10000.0))
         model.config = ModelConfig(**fields)
         model.model, model.lm_head = hf.model, hf.lm_head
@@ -144,12 +149,13 @@ class Model(nn.Module):
 
     def _project_at(self, layer, x, positions):
         """_project for rows at arbitrary positions (an int tensor [len(x)])."""
-        cfg, n = self.config, len(x)
-        h = layer.input_layernorm(x)
+        cfg = self.config
+        q, k, v = self._heads(layer, x)
         attn = layer.self_attn
-        q = attn.q_proj(h).view(n, cfg.num_attention_heads, cfg.head_dim)
-        k = attn.k_proj(h).view(n, cfg.num_key_value_heads, cfg.head_dim)
-        v = attn.v_proj(h).view(n, cfg.num_key_value_heads, cfg.head_dim)
+        if cfg.qk_norm:
+            if x.is_cuda and _plain_qk_norms(attn, x.dtype):
+                return *_norm_rope(attn, q, k, cfg, *_rope_rows(cfg, positions, x.dtype)), v
+            q, k = attn.q_norm(q), attn.k_norm(k)
         inv_freq = cfg.rope_theta ** (-torch.arange(0, cfg.head_dim, 2, device=x.device).float() / cfg.head_dim)
         angle = positions.float()[:, None] * inv_freq[None, :]
         angle = torch.cat((angle, angle), -1)[:, None, :]
@@ -160,6 +166,16 @@ class Model(nn.Module):
             return t * cos + torch.cat((-hi, lo), -1) * sin
 
         return rope(q), rope(k), v
+
+    def _heads(self, layer, x):
+        """RMSNorm and the q/k/v projections as heads [len(x), heads,
+        head_dim], q and k neither normalised nor rotated."""
+        cfg, n = self.config, len(x)
+        h = layer.input_layernorm(x)
+        attn = layer.self_attn
+        return (attn.q_proj(h).view(n, cfg.num_attention_heads, cfg.head_dim),
+                attn.k_proj(h).view(n, cfg.num_key_value_heads, cfg.head_dim),
+                attn.v_proj(h).view(n, cfg.num_key_value_heads, cfg.head_dim))
 
     @staticmethod
     def _finish(layer, residual, attention):
@@ -174,6 +190,13 @@ class Model(nn.Module):
             raise ValueError("prompt cannot be empty")
         if cache is not None and any(cache.storage.requests[request_id].lengths):
             raise ValueError("prefill is allowed exactly once per request")
+        x, delta = self._prompt_rows(tokens, cache, request_id)
+        return self._prompt_logits(x, delta, -1).float()
+
+    def _prompt_rows(self, tokens, cache=None, request_id=None):
+        """The decoder layers over a prompt, writing K/V to the cache if there
+        is one: the residual rows [tokens, hidden] and what the last layer
+        adds to them (None where it is in them)."""
         cfg = self.config
         groups = cfg.num_attention_heads // cfg.num_key_value_heads
         # bf16/fp16 models on a GPU run the causal attention as the MFMA
@@ -204,7 +227,18 @@ class Model(nn.Module):
                     is_causal=True,
                 ).transpose(0, 1)
             x = self._finish(layer, x, attention)
-        return self.lm_head(self.model.norm(x[-1])).float()
+        return x, None
+
+    def _prompt_logits(self, x, delta, rows):
+        """Logits, in the model's dtype, of the last row (-1) or some rows (a
+        slice) of what _prompt_rows returned."""
+        if delta is None:
+            return self.lm_head(self.model.norm(x[rows]))
+        if _plain_norm(self.model.norm, x.dtype) and _plain(self.lm_head, nn.Linear):
+            if rows == -1:
+                return self._head_logits([_Last(x[-1:], delta[-1:])])[0]
+            return self._head_logits([_Last(x[rows], delta[rows])])
+        return self.lm_head(self.model.norm(x[rows] + delta[rows]))
 
     def _prefill_layers(self, x, cache, request_id):
         """The prompt pass of a bf16/fp16 GPU model from its embedded tokens
@@ -222,16 +256,42 @@ class Model(nn.Module):
             attn, norm1, norm2 = layer.self_attn, layer.input_layernorm, layer.post_attention_layernorm
             h = rk.add_rmsnorm(x, delta, norm1.weight, _eps(norm1, cfg))
             q, k, v = attn.q_proj(h), attn.k_proj(h), attn.v_proj(h)
-            rk.rope_(q, Hq, D, cos, sin)
-            rk.rope_(k, Hkv, D, cos, sin)
+            if cfg.qk_norm:
+                q, k = _norm_rope_(attn, q.view(n, Hq, D), k.view(n, Hkv, D), cfg, cos, sin)
+            else:
+                rk.rope_(q, Hq, D, cos, sin)
+                rk.rope_(k, Hkv, D, cos, sin)
             q, k, v = q.view(n, Hq, D), k.view(n, Hkv, D), v.view(n, Hkv, D)
             if cache is not None:
                 cache.write(request_id, index, k, v)
             o = attn.o_proj(rk.prefill_attention(q, k, v).reshape(n, -1)).contiguous()
             delta = layer.mlp(rk.add_rmsnorm(x, o, norm2.weight, _eps(norm2, cfg))).contiguous()
-        if _plain_norm(self.model.norm, x.dtype) and _plain(self.lm_head, nn.Linear):
-            return self._head([_Last(x[-1:], delta[-1:])])[0]
-        return self.lm_head(self.model.norm(x[-1] + delta[-1])).float()
+        return x, delta
+
+    @torch.inference_mode()
+    def score(self, tokens: list[int], top: int = 0):
+        """Log probabilities of a text: for every token but the first, the
+        log probability of that token after those before it, the entropy of
+        the distribution it was drawn from and its `top` most likely tokens
+        (row_kernels.TokenLogprobs of len(tokens) - 1 rows)."""
+        from . import row_kernels as rk
+
+        if len(tokens) < 2:
+            raise ValueError("a score needs at least two tokens")
+        self._check_tokens(tokens)
+        targets = upload(tokens[1:], torch.int64, self.device)
+        x, delta = self._prompt_rows(tokens[:-1])
+        kernels = rk if self.device.type == "cuda" else rk.cpu_provider("score")
+        parts = []
+        for at in range(0, len(targets), SCORE_ROWS):  # the logits of a long text need not fit at once
+            rows = slice(at, min(at + SCORE_ROWS, len(targets)))
+            parts.append(kernels.token_logprobs(self._prompt_logits(x, delta, rows), targets[rows], top))
+        return parts[0] if len(parts) == 1 else rk.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
+
+    def _check_tokens(self, tokens):
+        embed = self.model.embed_tokens
+        if _plain(embed, nn.Embedding) and not 0 <= min(tokens) <= max(tokens) < len(embed.weight):
+            raise IndexError("token id outside the vocabulary")
 
     @torch.inference_mode()
     def decode(self, token: int, request_id, cache, top_k=None, backend="auto", selector="quest"):
@@ -260,6 +320,64 @@ class Model(nn.Module):
             attention = cache.attention(q[0], request_id, index, selection, backend)
             x = self._finish(layer, x, attention.unsqueeze(0))
         return self.lm_head(self.model.norm(x[0])).float()
+
+    @torch.inference_mode()
+    def decode_tree(self, tokens: list[int], parents: list[int], request_id, cache, top_k=None, backend="auto",
+                    selector="quest"):
+        """One pass over a tree of tokens that may follow a request's history:
+        tokens[t] comes after tokens[parents[t]] (parents[t] < t), or right
+        after the history where parents[t] is -1. Usually token 0, the only
+        root, is the last one emitted and the others are drafted; at most 64.
+
+        Every node attends to the history as decode() does (per layer one
+        selection, by the first node's query, of which all nodes read the
+        same rows) and to its own ancestors. Nothing is written to the cache:
+        the returned DraftStep holds every node's logits and keys and values,
+        and its commit() appends those of an accepted path."""
+        from . import row_kernels as rk
+
+        n = len(tokens)
+        if n != len(parents) or not 1 <= n <= rk.MAX_TREE_NODES:
+            raise ValueError(f"a tree has 1 to {rk.MAX_TREE_NODES} tokens and a parent for each")
+        if any(not -1 <= p < t for t, p in enumerate(parents)):
+            raise ValueError("a node's parent is -1 or a node before it")
+        lengths = list(cache.storage.requests[request_id].lengths)
+        if len(set(lengths)) != 1 or lengths[0] == 0:
+            raise ValueError("all layers must have the same nonempty history")
+        self._check_tokens(tokens)
+        gpu = self.device.type == "cuda"
+        kernels = rk if gpu else rk.cpu_provider("decode_tree")
+        mask, positions = kernels.tree_plan(upload([list(parents)], torch.int32, self.device),
+                                            upload([lengths[0]], torch.int64, self.device))
+        mask, positions = mask[0], positions[0]
+        tables = None
+        if gpu and self.config.qk_norm:  # every position is below lengths[0] + n
+            tables = self._rope_tables(lengths[0] + n)
+            if tables is None:
+                tables = _rope_rows(self.config, torch.arange(lengths[0] + n, device=self.device), self.dtype)
+        x = self.model.embed_tokens(upload(tokens, torch.int64, self.device))
+        drafted = []
+        for index, layer in enumerate(self.model.layers):
+            if tables is not None and _plain_qk_norms(layer.self_attn, x.dtype):
+                q, k, v = self._heads(layer, x)
+                q, k = _norm_rope(layer.self_attn, q, k, self.config, *tables, positions)
+            else:
+                q, k, v = self._project_at(layer, x, positions)
+            request = cache.storage.requests[request_id]
+            P = cache.config.page_size
+            if selector == "quest" and top_k is not None:
+                selection = quest_selection(
+                    q[0], request.minimum[index], request.maximum[index], request.lengths[index], P, top_k
+                )
+            elif selector in ("quest", "mean"):
+                pages = select_pages(cache, request_id, index, q[0], top_k)
+                selection = Selection.from_pages(pages, request.lengths[index], P, q.shape[1])
+            else:
+                raise ValueError("selector must be quest or mean")
+            attention = cache.tree_attention(q, k, v, mask, request_id, index, selection, backend)
+            x = self._finish(layer, x, attention)
+            drafted.append((k, v))
+        return DraftStep(self.lm_head(self.model.norm(x)).float(), drafted, list(parents), request_id, cache, lengths)
 
     def _fused_projections(self):
         """Per layer: the q/k/v weights and biases and the gate/up weights as
@@ -356,8 +474,11 @@ class Model(nn.Module):
         return self._head(groups)
 
     def _head(self, groups):
+        return self._head_logits(groups).float()
+
+    def _head_logits(self, groups):
         """The last residual add, the final norm and the lm_head of every
-        group's rows: fused kernels in place of a plain norm and head, else
+        group's rows (logits in the model's dtype): fused kernels in place of a plain norm and head, else
         the modules themselves."""
         from . import row_kernels as rk
 
@@ -368,7 +489,7 @@ class Model(nn.Module):
         x = rows[0] if len(rows) == 1 else torch.cat(rows)
         if not plain:
             x = norm(x)
-        return (_linear(x, head.weight, head.bias) if _plain(head, nn.Linear) else head(x)).float()
+        return _linear(x, head.weight, head.bias) if _plain(head, nn.Linear) else head(x)
 
     def _rope_tables(self, limit):
         """cos and sin [rows, head_dim / 2] in the model dtype of every
@@ -505,6 +626,38 @@ class Model(nn.Module):
         return entry["logits"].clone()
 
 
+class DraftStep:
+    """What decode_tree computed: `logits` [nodes, vocab] (fp32), the
+    distribution after each node."""
+
+    def __init__(self, logits, drafted, parents, request_id, cache, lengths):
+        self.logits = logits
+        self._drafted, self._parents = drafted, parents
+        self._request_id, self._cache, self._lengths = request_id, cache, lengths
+
+    def commit(self, nodes):
+        """Append the keys and values of a path of the tree (a root first,
+        then each node's child) to the request's history in the cache. Once
+        per step, while the history is the one that the step attended to."""
+        nodes = list(nodes)
+        for parent, node in zip([-1] + nodes, nodes):
+            if not 0 <= node < len(self._parents) or self._parents[node] != parent:
+                raise ValueError("commit takes a path: a root, then each node's child")
+        request = self._cache.storage.requests.get(self._request_id)
+        if self._drafted is None or request is None or list(request.lengths) != self._lengths:
+            raise ValueError("the request's history has changed since this step")
+        if self._lengths[0] + len(nodes) > request.max_tokens:
+            raise ValueError("commit would exceed the request's reserved tokens")
+        if not nodes:
+            return
+        drafted, self._drafted = self._drafted, None
+        path = nodes[0] == 0 and nodes == list(range(len(nodes)))
+        at = None if path else upload(nodes, torch.int64, drafted[0][0].device)
+        for layer, (k, v) in enumerate(drafted):
+            k, v = (t[: len(nodes)] if path else t.index_select(0, at) for t in (k, v))
+            self._cache.write(self._request_id, layer, k.contiguous(), v.contiguous())
+
+
 def _tree(module):
     """A module and every module below it."""
     modules = [module]
@@ -574,14 +727,17 @@ class _Group:
         qkv_w, qkv_b, _ = fused
         self.gu_w = fused[2]
         h = rk.add_rmsnorm(self.x, self.delta, layer.input_layernorm.weight, _eps(layer.input_layernorm, cfg))
-        if _small_m(h, qkv_w, qkv_b) and D % 16 == 0:  # projection and RoPE in one launch
+        if _small_m(h, qkv_w, qkv_b) and D % 16 == 0 and not cfg.qk_norm:  # projection and RoPE in one launch
             qkv = rk.linear_rope(h, qkv_w, qkv_b, Hq + Hkv, D, self.cos, self.sin)
         else:
             qkv = _linear(h, qkv_w, qkv_b)
-            rk.rope_(qkv, Hq + Hkv, D, self.cos, self.sin)
+            if not cfg.qk_norm:
+                rk.rope_(qkv, Hq + Hkv, D, self.cos, self.sin)
         q = qkv[:, : Hq * D].view(B, Hq, D)
         k = qkv[:, Hq * D: (Hq + Hkv) * D].view(B, Hkv, D)
         v = qkv[:, (Hq + Hkv) * D:].view(B, Hkv, D)
+        if cfg.qk_norm:
+            _norm_rope_(layer.self_attn, q, k, cfg, self.cos, self.sin)
         self.step.append(index, k, v)
         self.handle = self.step.select(index, q, top_k)
 
@@ -601,6 +757,28 @@ class _Group:
         else:
             act = rk.silu_mul(_linear(h, self.gu_w, None))
         self.delta = _linear(act, down.weight, down.bias)
+
+
+def _norm_rope(attn, q, k, cfg, cos, sin, positions=None, out=None):
+    """q and k [n, heads, head_dim] normalised per head by the plain norms
+    q_norm and k_norm and rotated, in one launch: row r by row positions[r]
+    (or r) of cos/sin."""
+    from . import row_kernels as rk
+
+    return rk.qk_norm_rope(q, k, attn.q_norm.weight, attn.k_norm.weight, _eps(attn.q_norm, cfg), cos, sin, positions,
+                           out)
+
+
+def _norm_rope_(attn, q, k, cfg, cos, sin):
+    """The same in place, with norms of any kind."""
+    from . import row_kernels as rk
+
+    if _plain_qk_norms(attn, q.dtype):
+        return _norm_rope(attn, q, k, cfg, cos, sin, out=(q, k))
+    for t, norm in ((q, attn.q_norm), (k, attn.k_norm)):
+        t.copy_(norm(t))
+        rk.rope_(t.flatten(1), t.shape[1], t.shape[2], cos, sin)  # (heads of a row lie side by side: a view)
+    return q, k
 
 
 def _decode_rows(embed, ids, positions, tables):
@@ -667,11 +845,18 @@ def _plain_layer(layer, dtype):
     and plain q and k projections, whose outputs it rotates in place."""
     attn = layer.self_attn
     return (_plain_norm(layer.input_layernorm, dtype) and _plain_norm(layer.post_attention_layernorm, dtype)
-            and _plain(attn.q_proj, nn.Linear) and _plain(attn.k_proj, nn.Linear))
+            and _plain(attn.q_proj, nn.Linear) and _plain(attn.k_proj, nn.Linear) and _plain_qk_norms(attn, dtype))
+
+
+def _plain_qk_norms(attn, dtype):
+    """Whether nhs_qk_norm_rope computes the layer's query and key norms (true
+    without any): plain ones of one eps."""
+    norms = [n for n in (getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)) if n is not None]
+    return all(_plain_norm(n, dtype) for n in norms) and len({_eps(n, None) for n in norms}) < 2
 
 
 def _eps(norm, cfg):
-    return getattr(norm, "eps", getattr(norm, "variance_epsilon", cfg.rms_norm_eps))
+    return getattr(norm, "eps", getattr(norm, "variance_epsilon", cfg and cfg.rms_norm_eps))
 
 
 def _fuse(modules, name):

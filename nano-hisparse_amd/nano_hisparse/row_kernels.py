@@ -46,7 +46,9 @@ def set_cpu_provider(provider):
     page_size) -> RowPlan, gather_rows(host, pool, plan, config),
     attend_rows(query, pool, rows, config), quest_positions(query, minimum,
     maximum, length, page_size, top_pages, keep_sink) -> position tensor and
-    mean_pages(query, summaries, length, page_size, top_pages) -> page list.
+    mean_pages(query, summaries, length, page_size, top_pages) -> page list;
+    for drafted tokens and log probabilities tree_plan, tree_attention and
+    token_logprobs as below.
     """
     global _cpu_provider
     _cpu_provider = provider
