@@ -204,17 +204,45 @@ __global__ __launch_bounds__(kTgThreads) void tree_general_kernel(TreeArgs a) {
     if (sub + 16 * i < D) store_elem(a.out, T::dtype, at + sub + 16 * i, some ? acc[i] / l : 0.f);
 }
 
-// ---- 16-bit heads of 64 and 128 on the matrix cores ----
+// ---- heads whose rows are 64 to 512 bytes, on the matrix cores ----
 
-constexpr int kTfStage = 2048;  // rows whose addresses are in LDS at a time
-__device__ __attribute__((aligned(256))) char tree_zeros[256];  // read in place of a masked row
+// rows whose addresses are in LDS at a time (rows of 128 bytes: so that two workgroups share a CU)
+constexpr int tf_stage(int row_bytes) { return row_bytes <= 128 ? 1024 : 2048; }
+constexpr int kTfRowBytes = 512;  // the longest row of a head
+__device__ __attribute__((aligned(kTfRowBytes))) char tree_zeros[kTfRowBytes];  // read in place of a masked row
+
+// LDS slot of 16-byte chunk c of K row r (C chunks a row): any 16 consecutive rows at one chunk fall on distinct banks
+template <int C>
+__device__ __forceinline__ int tf_k_slot(int r, int c) {
+  return C >= 16 ? c ^ (r & 15) : C == 8 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3);
+}
+// and of V row (key) r. 16 bits: the 4 rows of a transposing read fall on distinct banks; fp32: rows r and r + 4, of
+// which the halves of a wave read the same dims (two to a bank with 8 chunks a row).
+template <typename T, int C>
+__device__ __forceinline__ int tf_v_slot(int r, int c) {
+  if constexpr (T::dtype == NHS_F32) return C >= 16 ? c ^ (8 * ((r >> 2) & 1)) : c;
+  return C >= 16 ? c ^ (4 * (r & 3)) : C == 8 ? c ^ (4 * ((r >> 1) & 1)) : c;
+}
+
+// 16 bytes of K and Q each: one 32x32x16 product of 16-bit elements, or four 32x32x2 of fp32
+template <typename T>
+__device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
+  if constexpr (T::dtype != NHS_F32) {
+    return mfma32x32x16<T>(k, q, c);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(q.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(q.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.z), __uint_as_float(q.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.w), __uint_as_float(q.w), c, 0, 0, 0);
+  }
+}
 
 // QW waves hold 32 query rows each; KW such sets share the keys (KW tiles of
 // BN keys a round). The layouts are those of prefill_attention_kernel:
 // S^T = K Q^T and O^T = V^T P^T, tiles straight from global memory to LDS.
 //
 // Every row of a tile has an address of its own, so a stage of up to 2048 rows
-// is turned into addresses in LDS first (a masked row's is that of zeros, and
+// (tf_stage) is turned into addresses in LDS first (a masked row's is that of zeros, and
 // its bit of the tile's word is clear); the loads of a round then need one LDS
 // read each. The drafted keys are a last round of the last split. A masked
 // weight is 0, which a matrix core would multiply with whatever V holds, so
@@ -224,16 +252,25 @@ __device__ __attribute__((aligned(256))) char tree_zeros[256];  // read in place
 //
 // With QW = 1 a wave loads and reads its own tiles only and no barrier stands
 // in the loop.
+//
+// fp32 runs on v_mfma_f32_32x32x2_f32 (lane l: row l%32 of A at k = l/32). The
+// dims of a dot product may come in any order, so four of them take the
+// 16-byte chunks as they lie; for O^T a score register is the B operand as it
+// stands, its two keys (4 rows apart) against one V element per lane.
 template <typename T, int D, int QW, int KW, int BN>
 __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a) {
   constexpr int W = QW * KW, THREADS = W * kWave;
-  constexpr int KS = D / 16, DB = D / 32, C = D / 8, NB = BN / 32;
-  constexpr int kRows = 1024 / (D * 2);        // of a load instruction
+  constexpr bool F = T::dtype == NHS_F32;
+  constexpr int RB = D * T::bytes;             // bytes of a head's row
+  constexpr int KS = RB / 32, DB = D / 32, C = RB / 16, NB = BN / 32;
+  constexpr int kRows = 1024 / RB;             // of a load instruction
   constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
-  constexpr int kTile = BN * D * 2;            // bytes
+  constexpr int kTile = BN * RB;               // bytes
   constexpr int kRound = BN * KW;              // keys
-  constexpr unsigned kDraft = T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;  // exponent bits of NaN and infinities
-  static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1, "tile shape");
+  constexpr int kTfStage = tf_stage(RB);
+  // exponent bits of NaN and infinities
+  constexpr uint32_t kOdd = F ? 0x7f800000u : T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;
+  static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1 && RB <= kTfRowBytes, "tile shape");
   // Tiles under names of their own, used by rounds in turn: the compiler then knows that reads of one need not wait for
   // loads into the others.
   __shared__ __attribute__((aligned(16))) char k0[KW * kTile], k1[KW * kTile];
@@ -261,7 +298,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   const uint64_t word = live ? (uint64_t)mask[node] : 0;
   uint4 qf[KS];
   {
-    const char* qp = a.q + ((int64_t)b * a.q_b + (int64_t)node * a.q_n + (int64_t)head * a.q_h) * 2 + half * 16;
+    const char* qp = a.q + ((int64_t)b * a.q_b + (int64_t)node * a.q_n + (int64_t)head * a.q_h) * T::bytes + half * 16;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 32);
   }
@@ -273,15 +310,16 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     for (int i = 0; i < 16; ++i) o[x][i] = 0.f;
 
   const int lrow = lane / C, lchunk = lane % C;
-  const int k_row = n * (D * 2);
+  const int k_row = n * RB;
   const int j4 = (lane & 15) >> 2;
   int v_at[DB];
 #pragma unroll
   for (int x = 0; x < DB; ++x)
-    v_at[x] = (4 * half + j4) * (D * 2) +
-              pf_v_slot<D>(j4, x * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+    v_at[x] = F ? 4 * half * RB + tf_v_slot<T, C>(4 * half, x * 8 + n / 4) * 16 + n % 4 * 4
+                : (4 * half + j4) * RB +
+                      tf_v_slot<T, C>(j4, x * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
 
-  const int64_t head_bytes = (int64_t)kv * D * 2, plane = a.plane_bytes;
+  const int64_t head_bytes = (int64_t)kv * RB, plane = a.plane_bytes;
   const int64_t zeros = (int64_t)tree_zeros;
   auto load_tile = [&](int t, char* kb, char* vb) {  // this share's tile of the stage's round t
 #pragma unroll
@@ -289,8 +327,8 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
       const int row = (i * QW + wave) * kRows + lrow;
       const int64_t at = stage[t * kRound + share * BN + row];
       const int dst = share * kTile + (i * QW + wave) * 1024;
-      const char* ks = (const char*)at + pf_k_slot<D>(row, lchunk) * 16;
-      const char* vs = (const char*)(at == zeros ? at : at + plane) + pf_v_slot<D>(row, lchunk) * 16;
+      const char* ks = (const char*)at + tf_k_slot<C>(row, lchunk) * 16;
+      const char* vs = (const char*)(at == zeros ? at : at + plane) + tf_v_slot<T, C>(row, lchunk) * 16;
       pf_load_lds(ks, kb + dst);
       pf_load_lds(vs, vb + dst);
     }
@@ -308,10 +346,10 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     for (int st = 0; st < KS; ++st)
 #pragma unroll
       for (int x = 0; x < NB; ++x) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(kl + x * 32 * D * 2 + pf_k_slot<D>(n, 2 * st + half) * 16);
-        s[x] = mfma32x32x16<T>(kf, qf[st], s[x]);
+        const uint4 kf = *reinterpret_cast<const uint4*>(kl + x * 32 * RB + tf_k_slot<C>(n, 2 * st + half) * 16);
+        s[x] = tf_qk<T>(kf, qf[st], s[x]);
       }
-    if constexpr (D == 128 && NB == 2) {  // as in the prompt attention: eight K reads ahead of the MFMAs
+    if constexpr (!F && D == 128 && NB == 2) {  // as in the prompt attention: eight K reads ahead of the MFMAs
       __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -344,29 +382,49 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         for (int i = 0; i < 16; ++i) o[x][i] *= alpha;
     }
     const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
-    uint4 pb[2 * NB];
     float tile_sum = 0.f;
+    if constexpr (F) {
 #pragma unroll
-    for (int j = 0; j < 2 * NB; ++j) {
-      uint32_t w[4];
+      for (int x = 0; x < NB; ++x)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float e0 = s[j >> 1][(j & 1) * 8 + 2 * x], e1 = s[j >> 1][(j & 1) * 8 + 2 * x + 1];
-        w[x] = pf_pack<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(e0, a.scale_log2, -ref)),
-                          __builtin_amdgcn_exp2f(__builtin_fmaf(e1, a.scale_log2, -ref)));
-        tile_sum = pf_add_pair<T>(w[x], tile_sum);
+        for (int i = 0; i < 16; ++i) {
+          s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], a.scale_log2, -ref));
+          tile_sum += s[x][i];
+        }
+      l += tile_sum;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int y = 0; y < DB; ++y) {
+            const float vf = *reinterpret_cast<const float*>(vl + v_at[y] + (x * 32 + (i >> 2) * 8 + (i & 3)) * RB);
+            o[y] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[x][i], o[y], 0, 0, 0);
+          }
+    } else {
+      uint4 pb[2 * NB];
+#pragma unroll
+      for (int j = 0; j < 2 * NB; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float e0 = s[j >> 1][(j & 1) * 8 + 2 * x], e1 = s[j >> 1][(j & 1) * 8 + 2 * x + 1];
+          w[x] = pf_pack<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(e0, a.scale_log2, -ref)),
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(e1, a.scale_log2, -ref)));
+          tile_sum = pf_add_pair<T>(w[x], tile_sum);
+        }
+        pb[j] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      pb[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      l += tile_sum;
+#pragma unroll
+      for (int j = 0; j < 2 * NB; ++j)
+#pragma unroll
+        for (int x = 0; x < DB; ++x) {
+          const uint2 lo = pf_read_tr(vl + v_at[x] + (16 * j) * RB);
+          const uint2 hi = pf_read_tr(vl + v_at[x] + (16 * j + 8) * RB);
+          o[x] = mfma32x32x16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[j], o[x]);
+        }
     }
-    l += tile_sum;
-#pragma unroll
-    for (int j = 0; j < 2 * NB; ++j)
-#pragma unroll
-      for (int x = 0; x < DB; ++x) {
-        const uint2 lo = pf_read_tr(vl + v_at[x] + (16 * j) * (D * 2));
-        const uint2 hi = pf_read_tr(vl + v_at[x] + (16 * j + 8) * (D * 2));
-        o[x] = mfma32x32x16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[j], o[x]);
-      }
   };
 
   const int begin = split * a.rows_per_split, end = min(a.n_rows, begin + a.rows_per_split);
@@ -378,10 +436,10 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     for (int i = 0; i < kMine; ++i) {
       const int row = (i * QW + wave) * kRows + lrow, j = min(share * BN + row, a.nodes - 1);
       const int dst = share * kTile + (i * QW + wave) * 1024;
-      const char* ks = a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * 2;
-      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2;
-      pf_load_lds(ks + pf_k_slot<D>(row, lchunk) * 16, k0 + dst);
-      pf_load_lds(vs + pf_v_slot<D>(row, lchunk) * 16, v0 + dst);
+      const char* ks = a.k + ((int64_t)b * a.k_b + (int64_t)j * a.k_n + (int64_t)kv * a.k_h) * T::bytes;
+      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * T::bytes;
+      pf_load_lds(ks + tf_k_slot<C>(row, lchunk) * 16, k0 + dst);
+      pf_load_lds(vs + tf_v_slot<T, C>(row, lchunk) * 16, v0 + dst);
     }
     present = __ballot(lane < a.nodes && mask[min(lane, a.nodes - 1)] != 0);
     if (tid == 0) odd = 0;
@@ -413,9 +471,10 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         bool found = false;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const bool lo = (w[x] & kDraft) == kDraft, hi = (w[x] >> 16 & kDraft) == kDraft;
+          const bool lo = (w[x] & kOdd) == kOdd, hi = !F && (w[x] >> 16 & kOdd) == kOdd;
           found |= lo || hi;
-          w[x] = here ? w[x] & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u)) : 0u;
+          const uint32_t keep = F ? (lo ? 0u : ~0u) : (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          w[x] = here ? w[x] & keep : 0u;
         }
         if (found || !here) *p = make_uint4(w[0], w[1], w[2], w[3]);
         if (found && here) odd = 1;
@@ -496,14 +555,13 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   if (draft && odd) {
     for (int j = 0; j < a.nodes; ++j) {
       if (!((word & present) >> j & 1)) continue;
-      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * 2 + half * 8;
+      const char* vs = a.v + ((int64_t)b * a.v_b + (int64_t)j * a.v_n + (int64_t)kv * a.v_h) * T::bytes;
 #pragma unroll
       for (int x = 0; x < DB; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint32_t bits = *reinterpret_cast<const uint16_t*>(vs + x * 64 + (i >> 2) * 16 + (i & 3) * 2);
-          if ((bits & kDraft) == kDraft)
-            o[x][i] += T::dtype == NHS_BF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits);
+          const float value = load_elem(vs, T::dtype, x * 32 + (i >> 2) * 8 + half * 4 + (i & 3));
+          if (!(fabsf(value) < INFINITY)) o[x][i] += value;
         }
     }
   }
@@ -521,14 +579,19 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   }
   const bool some = word != 0 && m != -INFINITY;
   const float inv = some ? 1.f / l : 0.f;
-  char* op = a.out + ((int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h) * 2 + half * 8;
+  char* op = a.out + ((int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h) * T::bytes;
 #pragma unroll
   for (int x = 0; x < DB; ++x)
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const uint32_t w0 = pf_pack<T>(o[x][4 * y] * inv, o[x][4 * y + 1] * inv);
-      const uint32_t w1 = pf_pack<T>(o[x][4 * y + 2] * inv, o[x][4 * y + 3] * inv);
-      *reinterpret_cast<uint2*>(op + x * 64 + y * 16) = some ? make_uint2(w0, w1) : make_uint2(0u, 0u);
+    for (int y = 0; y < 4; ++y) {  // dims x*32 + y*8 + half*4 .. +3
+      float r4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r4[e] = some ? o[x][4 * y + e] * inv : 0.f;
+      char* to = op + (x * 32 + y * 8 + half * 4) * T::bytes;
+      if constexpr (F)
+        *reinterpret_cast<float4*>(to) = make_float4(r4[0], r4[1], r4[2], r4[3]);
+      else
+        *reinterpret_cast<uint2*>(to) = make_uint2(pf_pack<T>(r4[0], r4[1]), pf_pack<T>(r4[2], r4[3]));
     }
 }
 
@@ -647,18 +710,20 @@ struct TreeShape {
   int row_blocks, n_splits, rows_per_split;
 };
 
-// How a (request, KV head)'s query rows and keys are divided. `flash`: the
-// matrix-core kernel takes the call (16-bit heads of 64 or 128).
-static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim, bool flash) {
+// How a (request, KV head)'s query rows and keys are divided. `row_bytes`: of a
+// head's row where the matrix-core kernel takes the call, else 0.
+static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim,
+                            int row_bytes) {
+  const bool flash = row_bytes > 0;
   TreeShape s;
   const int query_rows = nodes * (q_heads / kv_heads);
   int block_rows = kTgRows, per_cu = 2, least = 64;
   s.waves = s.shares = 0;
   if (flash) {
-    s.waves = query_rows <= 32 ? 1 : query_rows <= 64 ? 2 : 4;
-    s.shares = s.waves == 1 ? 4 : 2;
+    s.waves = query_rows <= 32 ? 1 : query_rows <= 64 || head_dim == 256 ? 2 : 4;  // (256: four would spill)
+    s.shares = s.waves == 1 && row_bytes < 512 ? 4 : 2;  // (tiles of 64 KB in two buffers)
     block_rows = 32 * s.waves;
-    per_cu = 1;
+    per_cu = row_bytes <= 128 ? 2 : 1;
     least = 128;
   }
   s.row_blocks = (query_rows + block_rows - 1) / block_rows;
@@ -670,7 +735,11 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
   return s;
 }
 
-static bool tree_flash_head(int dtype, int head_dim) { return dtype != NHS_F32 && (head_dim == 64 || head_dim == 128); }
+// Bytes of a head's row if the matrix-core kernel has it, else 0.
+static int tree_flash_row(int dtype, int head_dim) {
+  const int bytes = head_dim * elem_size(dtype);
+  return (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256) && bytes <= kTfRowBytes ? bytes : 0;
+}
 
 static bool tree_valid(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim) {
   return batch >= 0 && nodes >= 1 && nodes <= kTreeNodes && n_rows >= 0 && q_heads >= 1 && kv_heads >= 1 &&
@@ -697,10 +766,8 @@ extern "C" int64_t nhs_tree_attention_workspace_bytes(int32_t batch, int32_t nod
                                                       int32_t kv_heads, int32_t head_dim) {
   if (!tree_valid(batch, nodes, n_rows, q_heads, kv_heads, head_dim)) return 0;
   int splits = 0;  // the most that any kernel makes of the shape: which one runs depends on dtype and alignment too
-  for (const bool flash : {false, true}) {
-    if (flash && !tree_flash_head(NHS_BF16, head_dim)) continue;
-    splits = std::max(splits, tree_shape(std::max(batch, 1), nodes, n_rows, q_heads, kv_heads, head_dim, flash).n_splits);
-  }
+  for (const int row : {0, tree_flash_row(NHS_BF16, head_dim), tree_flash_row(NHS_F32, head_dim)})
+    splits = std::max(splits, tree_shape(std::max(batch, 1), nodes, n_rows, q_heads, kv_heads, head_dim, row).n_splits);
   if (splits == 1) return 0;
   return (int64_t)splits * batch * nodes * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
 }
@@ -732,13 +799,14 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)pool) % esize ||
       ((uintptr_t)mask | (uintptr_t)rows) % 8)
     return fail(NHS_ERR_INVALID, "%s: misaligned pointer", who);
-  bool flash = tree_flash_head(dtype, head_dim) && pool_block_stride % 16 == 0 &&
+  bool flash = tree_flash_row(dtype, head_dim) > 0 && pool_block_stride % 16 == 0 &&
                ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)pool) % 16 == 0;
   for (const int64_t stride : {q_batch_stride, q_node_stride, q_head_stride, k_batch_stride, k_node_stride,
                                k_head_stride, v_batch_stride, v_node_stride, v_head_stride, out_batch_stride,
                                out_node_stride, out_head_stride})
-    flash = flash && stride % 8 == 0;
-  const TreeShape shape = tree_shape(batch, nodes, n_rows, q_heads, kv_heads, head_dim, flash);
+    flash = flash && stride * esize % 16 == 0;
+  const TreeShape shape =
+      tree_shape(batch, nodes, n_rows, q_heads, kv_heads, head_dim, flash ? tree_flash_row(dtype, head_dim) : 0);
   const int64_t need = nhs_tree_attention_workspace_bytes(batch, nodes, n_rows, q_heads, kv_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(NHS_ERR_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", who, (long long)need);
@@ -792,24 +860,38 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
       else
         run(kernel, tree_join_kernel<T, D, 1>, threads, 4);
     };
-    if (shape.waves == 1)
-      go(tree_flash_kernel<T, D, 1, 4, 32>);
-    else if (shape.waves == 2)
-      go(tree_flash_kernel<T, D, 2, 2, 64>);
-    else
-      go(tree_flash_kernel<T, D, 4, 2, 64>);
+    if constexpr (D * T::bytes < 512) {
+      if (shape.waves == 1)
+        go(tree_flash_kernel<T, D, 1, 4, 32>);
+      else if (shape.waves == 2)
+        go(tree_flash_kernel<T, D, 2, 2, 64>);
+      else
+        go(tree_flash_kernel<T, D, 4, 2, 64>);
+    } else {
+      if (shape.waves == 1)
+        go(tree_flash_kernel<T, D, 1, 2, 32>);
+      else if (shape.waves == 2)
+        go(tree_flash_kernel<T, D, 2, 2, 32>);
+      else if constexpr (D < 256)
+        go(tree_flash_kernel<T, D, 4, 2, 32>);
+    }
   };
-  using D64 = std::integral_constant<int, 64>;
-  using D128 = std::integral_constant<int, 128>;
-  if (flash && dtype == NHS_BF16)
-    head_dim == 128 ? on_mfma(BF16{}, D128{}) : on_mfma(BF16{}, D64{});
-  else if (flash)
-    head_dim == 128 ? on_mfma(F16{}, D128{}) : on_mfma(F16{}, D64{});
-  else if (dtype == NHS_BF16)
-    general(BF16{});
+  const auto by_dim = [&](auto tag) {
+    using T = decltype(tag);
+    if (!flash) return general(tag);
+    switch (head_dim) {
+      case 32: return on_mfma(tag, std::integral_constant<int, 32>());
+      case 64: return on_mfma(tag, std::integral_constant<int, 64>());
+      case 128: return on_mfma(tag, std::integral_constant<int, 128>());
+      default:
+        if constexpr (T::bytes == 2) on_mfma(tag, std::integral_constant<int, 256>());
+    }
+  };
+  if (dtype == NHS_BF16)
+    by_dim(BF16{});
   else if (dtype == NHS_F16)
-    general(F16{});
+    by_dim(F16{});
   else
-    general(F32{});
+    by_dim(F32{});
   return launch_status(who);
 }

@@ -326,7 +326,8 @@ SHAPES = [  # B, T, Hq, Hkv, D, P, N
     (2, 64, 8, 2, 128, 64, 1111), (1, 33, 14, 2, 64, 8, 700), (2, 7, 8, 8, 128, 5, 65), (1, 16, 32, 8, 128, 64, 2048),
     (1, 3, 16, 1, 128, 16, 300), (1, 64, 32, 1, 64, 16, 129), (5, 2, 4, 2, 32, 3, 40), (2, 9, 6, 3, 80, 7, 91),
     (1, 12, 4, 2, 256, 16, 150), (1, 4, 2, 1, 2, 4, 30), (2, 3, 3, 3, 17, 4, 33), (2, 2, 4, 2, 64, 16, 31),
-    (1, 20, 16, 4, 128, 16, 6000),
+    (1, 20, 16, 4, 128, 16, 6000), (2, 64, 4, 2, 256, 16, 400), (3, 40, 8, 2, 32, 16, 1300), (1, 17, 4, 2, 256, 8, 77),
+    (2, 30, 4, 1, 32, 32, 129), (1, 50, 7, 1, 64, 64, 3000),
 ]
 
 
