@@ -89,8 +89,12 @@ __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b) {
 // over the wave: every lane moves to the largest reference, then plain sums
 __device__ __forceinline__ LpSums lp_wave_join(LpSums t) {
   float ref = t.ref;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) ref = fmaxf(ref, __shfl_xor(ref, d));
+  ref = fmaxf(ref, dpp_f32<0xB1>(ref));   // lane ^ 1, ^ 2, then the mirrored 8 and 16 lanes, as group_sum goes
+  ref = fmaxf(ref, dpp_f32<0x4E>(ref));
+  ref = fmaxf(ref, dpp_f32<0x141>(ref));
+  ref = fmaxf(ref, dpp_f32<0x140>(ref));
+  ref = fmaxf(ref, __shfl_xor(ref, 16));
+  ref = fmaxf(ref, __shfl_xor(ref, 32));
   const float d = t.ref - ref, f = __builtin_amdgcn_exp2f(d);
   return {ref, group_sum(t.s * f, kWave), group_sum(f * __builtin_fmaf(fmaxf(d, -1e9f), t.s, t.w), kWave)};
 }
@@ -154,9 +158,9 @@ __device__ void lp_top_by_rounds(const LpRow<T>& row, const LpPart& part, int to
 }
 
 // The `top` largest of sh.found[0 .. n) in descending order to sh.sorted (0 beyond n): every key's place is the number
-// of larger ones. Sixteen keys are read at a time, so that the wait for LDS is paid once for them.
+// of larger ones. Eight keys are read at a time, so that the wait for LDS is paid once for them.
 __device__ __forceinline__ void lp_sort_found(int n, int top, LogprobShared& sh) {
-  constexpr int kStep = 16;
+  constexpr int kStep = 8;
   const int tid = threadIdx.x, padded = (n + kStep - 1) / kStep * kStep;
   if (tid < top) sh.sorted[tid] = 0;
   if (tid < padded - n) sh.found[n + tid] = 0;
@@ -178,8 +182,8 @@ __device__ __forceinline__ void lp_sort_found(int n, int top, LogprobShared& sh)
 
 // The `top` largest elements of the part, given each thread's largest (of chunks first + thread, + kLpThreads, ...):
 // the top-th largest of these is a lower bound, and only the few threads that reach it hold elements that count; their
-// chunks are read again and compared by the whole workgroup. Where more elements equal the bound than LDS holds (masked
-// vocabularies), those above it are kept and the equal ones counted off in index order.
+// chunks are read again and compared by the whole workgroup. Where many threads reach it (masked vocabularies) or more
+// elements than LDS holds, those above it are kept and the equal ones counted off in index order.
 template <typename T>
 __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool any, float thread_max,
                        LogprobShared& sh) {
@@ -192,7 +196,7 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
   // the threads with fewer than `top` larger ones; the least of them is the top-th largest
   int larger[2] = {0, 0};
   const uint4* all = reinterpret_cast<const uint4*>(sh.lane_max);
-#pragma unroll 16
+#pragma unroll 8
   for (int i = 0; i < kLpThreads / 4; ++i) {
     const uint4 v = all[i];
     larger[0] += (v.x > mine) + (v.z > mine);
@@ -205,9 +209,9 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
   __syncthreads();
   const uint32_t threshold = sh.threshold;
   const int per_thread = (part.last - part.first + kLpThreads - 1) / kLpThreads;
-  const int pairs = sh.n_hot * per_thread;  // at most 256 threads x their chunks: the part
   // pushes the elements whose order is at least `least`
   const auto collect = [&](uint32_t least) {
+    const int pairs = sh.n_hot * per_thread;  // at most 256 threads x their chunks: the part
     const auto push = [&](float x, int i) {
       if (lp_order(x) >= least) {
         const int at = atomicAdd(&sh.n_found, 1);
@@ -222,15 +226,24 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
 #pragma unroll
       for (int e = 0; e < E; ++e) push(x[e], row.index(chunk, e));
     }
-    if (part.lead && tid < row.lead) push(row.at(tid), tid);
-    if (part.tail)
-      for (int i = row.index(row.chunks, 0) + tid; i < row.vocab; i += kLpThreads) push(row.at(i), i);
+    const int behind = row.index(row.chunks, 0);
+    const int lead = part.lead ? row.lead : 0, around = lead + (part.tail ? row.vocab - behind : 0);
+    if (tid < around) {
+      const int i = tid < lead ? tid : behind + tid - lead;
+      push(row.at(i), i);
+    }
   };
-  collect(threshold);
-  __syncthreads();
-  if (sh.n_found > kLpCandidates) {
+  bool ties = sh.n_hot > 2 * top + 32;
+  if (!ties) {
+    collect(threshold);
     __syncthreads();
-    if (tid == 0) sh.n_found = 0;
+    ties = sh.n_found > kLpCandidates;
+  }
+  if (ties) {
+    __syncthreads();
+    if (tid == 0) sh.n_hot = sh.n_found = 0;
+    __syncthreads();
+    if (mine > threshold) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
     __syncthreads();
     collect(threshold + 1);
     __syncthreads();
@@ -403,7 +416,15 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     s += e;
     w = __builtin_fmaf(e, fmaxf(y, -1e9f), w);  // 0 and not NaN where x is -inf
   };
-  const auto block = [&](const uint4 (&v)[U]) {
+  // (one copy of the loop's body, also for the last block: a row is often shorter than the code that it runs is long)
+  for (int c = part.first + tid; c < part.last; c += U * kLpThreads) {
+    constexpr uint32_t none = T::dtype == NHS_F32 ? 0xff800000u : T::dtype == NHS_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // chunks past the end count as -inf
+      v[u] = make_uint4(none, none, none, none);
+      if (c + u * kLpThreads < part.last) v[u] = row.load(c + u * kLpThreads);
+    }
     float x[U][E], block_max = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -418,34 +439,14 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) add(x[u][e], s, w);
     t.s += s, t.w += w;
-  };
-  int c = part.first + tid;
-  for (; c + (U - 1) * kLpThreads < part.last; c += U * kLpThreads) {
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = row.load(c + u * kLpThreads);
-    block(v);
-  }
-  if (c < part.last) {  // the last block: chunks past the end count as -inf
-    constexpr uint32_t none = T::dtype == NHS_F32 ? 0xff800000u : T::dtype == NHS_BF16 ? 0xff80ff80u : 0xfc00fc00u;
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = make_uint4(none, none, none, none);
-      if (c + u * kLpThreads < part.last) v[u] = row.load(c + u * kLpThreads);
-    }
-    block(v);
   }
   const bool any = part.first + tid < part.last;
   const float thread_max = top;
-  // the elements around the chunks, which the search looks at in any case
-  if (part.lead && tid < row.lead) {
-    const float x = row.at(tid);
-    raise(x);
-    add(x, t.s, t.w);
-  }
-  if (part.tail && row.index(row.chunks, 0) + tid < row.vocab) {
-    const float x = row.at(row.index(row.chunks, 0) + tid);
+  // the elements before and after the chunks, which the search looks at in any case
+  const int behind = row.index(row.chunks, 0);
+  const int lead = part.lead ? row.lead : 0, around = lead + (part.tail ? row.vocab - behind : 0);
+  if (tid < around) {
+    const float x = row.at(tid < lead ? tid : behind + tid - lead);
     raise(x);
     add(x, t.s, t.w);
   }
