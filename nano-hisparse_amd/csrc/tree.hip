@@ -722,6 +722,12 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
   if (flash) {
     s.waves = query_rows <= 32 ? 1 : query_rows <= 64 || head_dim == 256 ? 2 : 4;  // (256: four would spill)
     s.shares = s.waves == 1 && row_bytes < 512 ? 4 : 2;  // (tiles of 64 KB in two buffers)
+    // Blocks of 256 rows where they fill the chip without splits (half the reads of the keys from L2; with splits their
+    // joining costs more than that). us with blocks of 128 / 256: 32 requests x 448 rows x 4 KV heads (256 of 256) x
+    // 2048 keys 118.5 / 98.5, 16 of them (128) x 4096 keys 105 / 116.
+    if (query_rows > 128 && head_dim == 128 && row_bytes == 256 &&
+        (int64_t)batch * kv_heads * ((query_rows + 255) / 256) >= 256)
+      s.waves = 8, s.shares = 1;
     block_rows = 32 * s.waves;
     per_cu = row_bytes <= 128 ? 2 : 1;
     least = 128;
@@ -865,8 +871,10 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
         go(tree_flash_kernel<T, D, 1, 4, 32>);
       else if (shape.waves == 2)
         go(tree_flash_kernel<T, D, 2, 2, 64>);
-      else
+      else if (shape.waves == 4)
         go(tree_flash_kernel<T, D, 4, 2, 64>);
+      else if constexpr (D == 128)
+        go(tree_flash_kernel<T, D, 8, 1, 64>);
     } else {
       if (shape.waves == 1)
         go(tree_flash_kernel<T, D, 1, 2, 32>);

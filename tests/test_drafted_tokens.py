@@ -328,6 +328,7 @@ SHAPES = [  # B, T, Hq, Hkv, D, P, N
     (1, 12, 4, 2, 256, 16, 150), (1, 4, 2, 1, 2, 4, 30), (2, 3, 3, 3, 17, 4, 33), (2, 2, 4, 2, 64, 16, 31),
     (1, 20, 16, 4, 128, 16, 6000), (2, 64, 4, 2, 256, 16, 400), (3, 40, 8, 2, 32, 16, 1300), (1, 17, 4, 2, 256, 8, 77),
     (2, 30, 4, 1, 32, 32, 129), (1, 50, 7, 1, 64, 64, 3000),
+    (32, 33, 32, 4, 128, 16, 100),
 ]
 
 
