@@ -206,8 +206,7 @@ __global__ __launch_bounds__(kTgThreads) void tree_general_kernel(TreeArgs a) {
 
 // ---- heads whose rows are 64 to 512 bytes, on the matrix cores ----
 
-// rows whose addresses are in LDS at a time (rows of 128 bytes: so that two workgroups share a CU)
-constexpr int tf_stage(int row_bytes) { return row_bytes <= 128 ? 1024 : 2048; }
+constexpr int kTfStage = 2048;  // rows whose addresses are in LDS at a time
 constexpr int kTfRowBytes = 512;  // the longest row of a head
 __device__ __attribute__((aligned(kTfRowBytes))) char tree_zeros[kTfRowBytes];  // read in place of a masked row
 
@@ -239,19 +238,37 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 
 // QW waves hold 32 query rows each; KW such sets share the keys (KW tiles of
 // BN keys a round). The layouts are those of prefill_attention_kernel:
-// S^T = K Q^T and O^T = V^T P^T, tiles straight from global memory to LDS.
+// S^T = K Q^T and O^T = V^T P^T, tiles straight from global memory to LDS. A
+// row of K and V is read once per block of 32 QW query rows, where a pass per
+// node would read it once per node.
 //
 // Every row of a tile has an address of its own, so a stage of up to 2048 rows
-// (tf_stage) is turned into addresses in LDS first (a masked row's is that of zeros, and
+// is turned into addresses in LDS first (a masked row's is that of zeros, and
 // its bit of the tile's word is clear); the loads of a round then need one LDS
-// read each. The drafted keys are a last round of the last split. A masked
-// weight is 0, which a matrix core would multiply with whatever V holds, so
-// what a mask hides must be finite: masked rows and absent nodes read zeros,
-// and NaN and infinities of drafted values are taken out of the tile, then
-// added to the outputs of the nodes that see them.
+// read each. The drafted keys are the first round of the last split, asked
+// for before the row indices are read. A masked weight is 0, which a matrix
+// core would multiply with whatever V holds, so what a mask hides must be
+// finite: masked rows read zeros, absent nodes' values are cleared in the tile,
+// and NaN and infinities of drafted values are taken out of it, then added to
+// the outputs of the nodes that see them.
+//
+// 16-bit weights are rounded to the type for the P.V product and the
+// denominator sums the same rounded weights, as in the prompt attention: the
+// output's error against float64 is 0.0022 of it in bf16, 0.0017 of which is
+// its own rounding. (A second product with the rounded rests, which leaves
+// that rounding alone, costs 5% at 8 requests x 2048 rows and 18% for the
+// widest trees.) fp32 weights are not rounded.
 //
 // With QW = 1 a wave loads and reads its own tiles only and no barrier stands
 // in the loop.
+//
+// Measured (MI355X, bf16, rows read from HBM, us with the join of the splits):
+// 8 requests x 16 nodes x 32/8 heads of 128 x 2048 rows 30 (23 without the
+// join; the rows stream at 5.5 TB/s once they flow, but 6 us pass before the
+// first are in, and 2.5 at the end); one request x 32 nodes x 32768 rows 50 (39);
+// 16 requests x 64 nodes x 28/4 heads x 4096 rows 107 (570 TFLOP/s): bound by
+// the matrix cores, LDS reads and softmax in about equal parts (85 without the
+// loads, 65 with them alone). With the general kernel 932, 3685 and 10818.
 //
 // fp32 runs on v_mfma_f32_32x32x2_f32 (lane l: row l%32 of A at k = l/32). The
 // dims of a dot product may come in any order, so four of them take the
@@ -267,7 +284,6 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
   constexpr int kTile = BN * RB;               // bytes
   constexpr int kRound = BN * KW;              // keys
-  constexpr int kTfStage = tf_stage(RB);
   // exponent bits of NaN and infinities
   constexpr uint32_t kOdd = F ? 0x7f800000u : T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;
   static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1 && RB <= kTfRowBytes, "tile shape");
@@ -597,7 +613,8 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
 
 // Joins the splits of every output row: the sums are scaled to the largest of
 // the splits' maxima, added and divided. WAVES waves of a workgroup share a row
-// (four where there are more than 16 splits: few rows, long chains of loads);
+// (four from 17 splits on, where the rows are few and the chains of loads long;
+// us of both launches with one / four: 32 splits 30.3 / 29.6, 8 splits 41.6 / 44.1);
 // LANES lanes of four dims read one split while the others read the next ones,
 // all the splits of a wave in flight at once.
 template <typename T, int D, int WAVES>
@@ -720,8 +737,12 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
   int block_rows = kTgRows, per_cu = 2, least = 64;
   s.waves = s.shares = 0;
   if (flash) {
-    s.waves = query_rows <= 32 ? 1 : query_rows <= 64 || head_dim == 256 ? 2 : 4;  // (256: four would spill)
-    s.shares = s.waves == 1 && row_bytes < 512 ? 4 : 2;  // (tiles of 64 KB in two buffers)
+    // One set of waves per 32 query rows. us at up to 32 rows with one / two sets: rows of 128 bytes, 16 requests x
+    // 16384 keys 38.3 / 41.3, fp32 heads of 32 x 528 keys 11.8 / 13.6; rows of 256 bytes, one request x 128 keys 11.9
+    // / 10.4, x 2048 15.7 / 14.5, x 32768 37.5 / 37.0, 16 requests x 8192 equal. At 64 rows x 2048 keys two / four sets
+    // 30.0 / 30.8. (Heads of 256: four would spill.)
+    s.waves = query_rows <= 32 && row_bytes <= 128 ? 1 : query_rows <= 64 || head_dim == 256 ? 2 : 4;
+    s.shares = s.waves == 1 ? 4 : 2;
     // Blocks of 256 rows where they fill the chip without splits (half the reads of the keys from L2; with splits their
     // joining costs more than that). us with blocks of 128 / 256: 32 requests x 448 rows x 4 KV heads (256 of 256) x
     // 2048 keys 118.5 / 98.5, 16 of them (128) x 4096 keys 105 / 116.
@@ -729,7 +750,10 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
         (int64_t)batch * kv_heads * ((query_rows + 255) / 256) >= 256)
       s.waves = 8, s.shares = 1;
     block_rows = 32 * s.waves;
-    per_cu = row_bytes <= 128 ? 2 : 1;
+    // One workgroup per CU, none of less than 128 keys. us with one / two per CU: one request of 8 nodes x 16384 keys
+    // 27.4 / 36.8, rows of 64 bytes x 32768 keys 15.5 / 18.9. With at least 64 / 128 / 256 keys: 8 nodes x 2048 keys
+    // 19.0 / 16.7 / 18.0, 32 nodes 26.7 / 17.9 / 19.5, x 512 keys 15.0 / 14.9 / 16.5.
+    per_cu = 1;
     least = 128;
   }
   s.row_blocks = (query_rows + block_rows - 1) / block_rows;
@@ -866,23 +890,14 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
       else
         run(kernel, tree_join_kernel<T, D, 1>, threads, 4);
     };
-    if constexpr (D * T::bytes < 512) {
-      if (shape.waves == 1)
-        go(tree_flash_kernel<T, D, 1, 4, 32>);
-      else if (shape.waves == 2)
-        go(tree_flash_kernel<T, D, 2, 2, 64>);
-      else if (shape.waves == 4)
-        go(tree_flash_kernel<T, D, 4, 2, 64>);
-      else if constexpr (D == 128)
-        go(tree_flash_kernel<T, D, 8, 1, 64>);
-    } else {
-      if (shape.waves == 1)
-        go(tree_flash_kernel<T, D, 1, 2, 32>);
-      else if (shape.waves == 2)
-        go(tree_flash_kernel<T, D, 2, 2, 32>);
-      else if constexpr (D < 256)
-        go(tree_flash_kernel<T, D, 4, 2, 32>);
-    }
+    constexpr int RB = D * T::bytes, BN = RB < 512 ? 64 : 32;  // (tiles of at most 64 KB in two buffers)
+    if (shape.waves == 2) return go(tree_flash_kernel<T, D, 2, 2, BN>);
+    if constexpr (RB <= 128)
+      if (shape.waves == 1) return go(tree_flash_kernel<T, D, 1, 4, 32>);
+    if constexpr (D < 256)
+      if (shape.waves == 4) return go(tree_flash_kernel<T, D, 4, 2, BN>);
+    if constexpr (D == 128 && RB == 256)
+      if (shape.waves == 8) return go(tree_flash_kernel<T, D, 8, 1, BN>);
   };
   const auto by_dim = [&](auto tag) {
     using T = decltype(tag);
