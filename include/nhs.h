@@ -458,7 +458,6 @@ int nhs_prefill_attention(const void* q, int64_t q_seq_stride, int64_t q_head_st
  * parents_stride elements apart; mask and positions are [batch, nodes].
  */
 #define NHS_MAX_TREE_NODES 64
-#define NHS_MAX_TREE_HEAD_DIM 256
 int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parents, int64_t parents_stride,
                   const int64_t* lengths, int64_t* mask, int64_t* positions, void* stream);
 
@@ -472,10 +471,13 @@ int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parents, int64_t 
  * node with mask word 0, like those that a mask hides, may hold anything.
  * One dtype for all tensors; strides in elements, dims of a head contiguous;
  * fp32 sums, one rounding of the output. head_dim up to
- * NHS_MAX_TREE_HEAD_DIM, nodes up to NHS_MAX_TREE_NODES. pool_block_stride as in nhs_attend_rows. The workspace
- * (nhs_tree_attention_workspace_bytes, 16-byte aligned, may be NULL where that is 0) holds
- * anything before and after a call.
+ * NHS_MAX_TREE_HEAD_DIM, nodes up to NHS_MAX_TREE_NODES, n_rows up to 2^30.
+ * Heads of 32, 64, 128 and (16 bits) 256 whose operands are 16-byte aligned,
+ * strides included, run on the matrix cores. pool_block_stride as in
+ * nhs_attend_rows. The workspace (nhs_tree_attention_workspace_bytes, 16-byte
+ * aligned, may be NULL where that is 0) holds anything before and after a call.
  */
+#define NHS_MAX_TREE_HEAD_DIM 256
 int64_t nhs_tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t n_rows, int32_t q_heads,
                                            int32_t kv_heads, int32_t head_dim);
 int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_node_stride, int64_t q_head_stride,
@@ -515,10 +517,10 @@ int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, int32_t hea
  * logits of each row, equal ones by ascending index, a NaN above every
  * number: top_ids and top_logprobs [rows, top]. A row that holds a NaN or
  * +inf, or nothing above -inf, has no distribution: its log probabilities
- * and entropy are NaN. The workspace
- * (nhs_token_logprobs_workspace_bytes, 16-byte aligned, may be NULL where that is 0) holds
- * anything before and after a call. No counterpart in the reference, which takes the argmax of its logits
- * (engine.py:68-74).
+ * and entropy are NaN. vocab up to 2^30. The workspace
+ * (nhs_token_logprobs_workspace_bytes, 16-byte aligned, may be NULL where that
+ * is 0) holds anything before and after a call. No counterpart in the
+ * reference, which takes the argmax of its logits (engine.py:68-74).
  */
 #define NHS_MAX_TOP_LOGPROBS 64
 int64_t nhs_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype, int32_t top);

@@ -422,7 +422,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
          k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && rows.size(0) == B &&
          rows.scalar_type() == at::kLong && mask.size(0) == B && mask.size(1) == T && mask.stride(1) == 1 &&
          mask.scalar_type() == at::kLong && q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1 &&
-         T <= NHS_MAX_TREE_NODES && D <= NHS_MAX_TREE_HEAD_DIM && pool.size(0) * P < (int64_t(1) << 31));
+         T <= NHS_MAX_TREE_NODES && D <= NHS_MAX_TREE_HEAD_DIM && N <= (1 << 30) && pool.size(0) * P < (int64_t(1) << 31));
     const int64_t stride = pool_block_stride(pool);
     Tensor out;
     if (a[7] != Py_None) {
@@ -516,7 +516,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int32_t top = integer32(a[2]);
     const int code = dtype_code(logits);
     need(logits.stride(1) == 1 && tokens.size(0) == R && tokens.scalar_type() == at::kLong && tokens.is_contiguous() &&
-         top >= 0 && top <= NHS_MAX_TOP_LOGPROBS && top <= V);
+         top >= 0 && top <= NHS_MAX_TOP_LOGPROBS && top <= V && V <= (1 << 30));
     Tensor logprobs, entropy, ids, values;
     int st;
     {

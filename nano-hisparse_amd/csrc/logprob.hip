@@ -310,7 +310,8 @@ __device__ __forceinline__ LpToken lp_token(const LogprobArgs& a, int64_t r, con
 }
 
 // The outputs of a row from its sums and sh.sorted. The sums are those of x * (1 + beta), where kLog2e rounds to
-// log2 e * (1 + beta): to first order lse(x) = lse(x (1 + beta)) - beta * sum p x.
+// log2 e * (1 + beta): to first order lse(x) = lse(x (1 + beta)) - beta * sum p x. (No rounding makes a probability more
+// than 1 or an entropy less than 0.)
 template <typename F>
 __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t r, const LpSums& t, const LpToken& first,
                                           F logit, LogprobShared& sh) {
@@ -318,14 +319,14 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t r, const
   const double bits = (double)log2f(t.s), mean = (double)t.w / (double)t.s;
   const double lse = ((double)t.ref + bits - beta * (mean + (double)t.ref)) * kLn2;
   const int tid = threadIdx.x;
-  if (tid == 0) a.entropy[r] = (float)((bits - mean) * kLn2);
+  if (tid == 0) a.entropy[r] = (float)fmax((bits - mean) * kLn2, 0.0);
   for (int g = tid; g < a.per_row; g += kLpThreads) {
     const LpToken token = g == tid ? first : logit(g);
-    a.logprobs[r * a.per_row + g] = token.known ? (float)((double)token.x - lse) : -INFINITY;
+    a.logprobs[r * a.per_row + g] = token.known ? (float)fmin((double)token.x - lse, 0.0) : -INFINITY;
   }
   if (tid < a.top) {
     a.top_ids[r * a.top + tid] = lp_index(sh.sorted[tid]);
-    a.top_logprobs[r * a.top + tid] = (float)((double)lp_value(sh.sorted[tid]) - lse);
+    a.top_logprobs[r * a.top + tid] = (float)fmin((double)lp_value(sh.sorted[tid]) - lse, 0.0);
   }
 }
 
@@ -364,16 +365,17 @@ __device__ void lp_unusual_row(const LogprobArgs& a, int64_t r, const LpRow<T>& 
   s = w = 0.f;
 #pragma unroll
   for (int i = 0; i < kLpWaves; ++i) s += sh.s[i], w += sh.w[i];
-  const float log_s = logf(s);
-  if (tid == 0) a.entropy[r] = log_s - w / s * (float)kLn2;
+  const float log_s = logf(s), entropy = log_s - w / s * (float)kLn2;
+  const auto at_most_0 = [](float x) { return x > 0.f ? 0.f : x; };  // a NaN stays
+  if (tid == 0) a.entropy[r] = -at_most_0(-entropy);
   for (int g = tid; g < a.per_row; g += kLpThreads) {
     const LpToken token = lp_token(a, r, row, g);
-    a.logprobs[r * a.per_row + g] = token.known ? token.x - m - log_s : s == s ? -INFINITY : NAN;
+    a.logprobs[r * a.per_row + g] = token.known ? at_most_0(token.x - m - log_s) : s == s ? -INFINITY : NAN;
   }
   lp_top_by_rounds(row, LpPart{0, row.chunks, true, true}, a.top, sh);
   if (tid < a.top) {
     a.top_ids[r * a.top + tid] = lp_index(sh.sorted[tid]);
-    a.top_logprobs[r * a.top + tid] = lp_value(sh.sorted[tid]) - m - log_s;
+    a.top_logprobs[r * a.top + tid] = at_most_0(lp_value(sh.sorted[tid]) - m - log_s);
   }
 }
 
@@ -526,6 +528,7 @@ extern "C" int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_
   if (!valid_dtype(dtype) || rows < 0 || vocab < 1 || tokens_per_row < 0 || top < 0 || top > vocab)
     return fail(NHS_ERR_INVALID, "%s: invalid shape or dtype", who);
   if (top > kLpMaxTop) return fail(NHS_ERR_UNSUPPORTED, "%s: at most %d alternatives", who, kLpMaxTop);
+  if (vocab > (1 << 30)) return fail(NHS_ERR_UNSUPPORTED, "%s: vocab up to 2^30", who);
   if (rows == 0) return NHS_OK;
   if (!logits || !entropy || (tokens_per_row > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs)))
     return fail(NHS_ERR_INVALID, "%s: null pointer", who);

@@ -772,7 +772,7 @@ static int tree_flash_row(int dtype, int head_dim) {
 }
 
 static bool tree_valid(int batch, int nodes, int n_rows, int q_heads, int kv_heads, int head_dim) {
-  return batch >= 0 && nodes >= 1 && nodes <= kTreeNodes && n_rows >= 0 && q_heads >= 1 && kv_heads >= 1 &&
+  return batch >= 0 && nodes >= 1 && nodes <= kTreeNodes && n_rows >= 0 && n_rows <= (1 << 30) && q_heads >= 1 && kv_heads >= 1 &&
          q_heads % kv_heads == 0 && head_dim >= 1 && q_heads <= 65536 && batch <= (1 << 20);
 }
 

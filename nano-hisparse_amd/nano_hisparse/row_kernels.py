@@ -943,6 +943,8 @@ def tree_attention(query, pool, rows, k, v, mask, page_size, out=None):
         raise ValueError("tree_attention: mask [B, T] int64")
     if T > MAX_TREE_NODES or D > MAX_TREE_HEAD_DIM:
         raise ValueError(f"tree_attention: at most {MAX_TREE_NODES} nodes and heads of {MAX_TREE_HEAD_DIM}")
+    if rows.shape[1] > 2**30:
+        raise ValueError("tree_attention: at most 2^30 rows")
     if any(t.stride(3) != 1 for t in (query, k, v)):
         raise ValueError("tree_attention: head dims must be contiguous")
     stride = pool_block_stride(pool)
@@ -1046,6 +1048,8 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError("token_logprobs: logits [rows, vocab], tokens int64 [rows] or [rows, n]")
     code, top = dtype_code(logits.dtype), int(top)
     R, V = logits.shape
+    if V > 2**30:
+        raise ValueError("token_logprobs: a vocabulary of at most 2^30 tokens")
     if V < 1 or not 0 <= top <= min(MAX_TOP_LOGPROBS, V):
         raise ValueError(f"token_logprobs: top must be 0 to {MAX_TOP_LOGPROBS}, and no more than the vocabulary")
     if logits.stride(1) != 1 and V > 1:

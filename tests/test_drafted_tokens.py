@@ -210,7 +210,7 @@ def attention_status(lib, **change):
 
 @pytest.mark.parametrize("change,status", [
     (dict(nodes=65), -1), (dict(nodes=0), -1), (dict(batch=-1), -1), (dict(n_rows=-1), -1), (dict(kv_heads=3), -1),
-    (dict(head_dim=0), -1), (dict(page=0), -1), (dict(dtype=3), -1), (dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1),
+    (dict(n_rows=(1 << 30) + 1), -1), (dict(head_dim=0), -1), (dict(page=0), -1), (dict(dtype=3), -1), (dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1),
     (dict(mask=0), -1), (dict(out=0), -1), (dict(pool=0), -1), (dict(rows=0), -1), (dict(q=257), -1),
     (dict(mask=260), -1), (dict(pool_rows=-1), -1), (dict(block=16), -1), (dict(head_dim=258), -2),
     (dict(pool_rows=1 << 31), -2), (dict(n_rows=100000), -3), (dict(n_rows=100000, ws=256, ws_bytes=64), -3),
@@ -248,7 +248,7 @@ def test_token_logprobs_refuses(lib):
                                       ids, 256, 256, 1 << 30, None)
 
     assert status(rows=0) == 0
-    assert status(top=65) == -2
+    assert status(top=65) == -2 and status(vocab=(1 << 30) + 1) == -2
     for bad in (dict(rows=-1), dict(vocab=0, top=0), dict(top=-1), dict(top=6, vocab=5), dict(dtype=4),
                 dict(logits=None), dict(tokens=None), dict(ids=None), dict(entropy=None), dict(logits=258),
                 dict(tokens=260), dict(per_row=-1)):
@@ -687,6 +687,57 @@ def test_token_logprobs_layouts(gpu, dtype):
     assert torch.equal(none.top_ids, rk.token_logprobs(logits, tokens, 3).top_ids)
     empty = rk.token_logprobs(logits[:0], tokens[:0], 3)
     assert empty.logprobs.shape == (0, 4) and empty.top_ids.shape == (0, 3) and empty.entropy.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [bf16, f16, f32])
+def test_certain_tokens(gpu, dtype):
+    """One token alone, or far above the others: no rounding puts its log probability above 0 or the entropy below."""
+    V = 5001
+    logits = torch.full((40, V), -math.inf)
+    logits[20:] = -60000.0
+    at = torch.randint(0, V, (40,), generator=torch.Generator().manual_seed(0))
+    logits[torch.arange(40), at] = torch.linspace(-700, 900, 40)
+    got = check_logprobs(logits.to(dtype).to(gpu), at.to(gpu), 3)
+    assert (got.logprobs <= 0).all() and (got.entropy >= 0).all() and (got.top_logprobs <= 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_a_whole_verification_in_one_graph(gpu, dtype):
+    """Plan, norm + rotation, attention and log probabilities one after the
+    other, captured and replayed with other inputs, against the eager calls."""
+    B, T, Hq, Hkv, D, P, N, V = 2, 12, 8, 2, 64, 16, 400, 3000
+    g = torch.Generator().manual_seed(0)
+    c = tree_case(gpu, dtype, B, T, Hq, Hkv, D, P, N)
+    parents = random_parents(B, T, g).to(gpu)
+    lengths = torch.tensor([400, 380], device=gpu)
+    table = torch.rand(512, D // 2, generator=g).to(gpu)
+    weights = [torch.rand(D, generator=g).to(dtype).to(gpu) for _ in range(2)]
+    head = (torch.randn(Hq * D, V, generator=g) * 0.1).to(dtype).to(gpu)
+    tokens = torch.randint(0, V, (B * T,), generator=g).to(gpu)
+
+    def verify():
+        mask, positions = rk.tree_plan(parents, lengths)
+        q, k = rk.qk_norm_rope(c["q"].reshape(B * T, Hq, D), c["k"].reshape(B * T, Hkv, D), *weights, 1e-6, table.cos(),
+                               table.sin(), positions.view(-1))
+        out = rk.tree_attention(q.view(B, T, Hq, D), c["pool"], c["rows"], k.view(B, T, Hkv, D), c["v"], mask, P)
+        return (mask, positions, q, k, out) + tuple(rk.token_logprobs(out.view(B * T, -1) @ head, tokens, 4))
+
+    verify()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = verify()
+    for i in range(3):
+        parents.copy_(random_parents(B, T, g))
+        lengths += 7
+        c["q"].mul_(-1)
+        c["rows"].copy_(c["rows"].roll(3, 1))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, verify())), i
 
 
 @pytest.mark.gpu

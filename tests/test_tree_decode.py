@@ -287,9 +287,9 @@ def test_engine_options_are_checked(where):
             Engine(model, cache_for(model), top_k=2, batch_decode=True, draft=lambda r: None)
 
 
-@pytest.mark.parametrize("drafts", [False, True])
-def test_log_probabilities_of_the_generated_tokens(where, drafts):
-    model = tiny(where, seed=7)
+@pytest.mark.parametrize("drafts,qk_norm", [(False, False), (True, False), (True, True)])
+def test_log_probabilities_of_the_generated_tokens(where, drafts, qk_norm):
+    model = tiny(where, seed=7, qk_norm=qk_norm)
     expected = generate(model, PROMPTS).requests
 
     def draft(request):
