@@ -131,6 +131,8 @@ class Engine:
     def _decode(self, request):
         """One decode turn of a request: the tokens it emits."""
         proposal = self.draft(request) if self.draft is not None else None
+        if request.finished:  # cancelled meanwhile
+            return []
         tokens, parents = proposal if proposal is not None else ((), ())
         if len(tokens) != len(parents):
             raise ValueError("a draft is a token list and a parent for each token")
@@ -206,10 +208,12 @@ class Engine:
                 if not request.finished:
                     self.running.append(request)
             return emitted
-        for _ in range(len(self.running)):
-            request = self.running[0]  # stays there if its turn raises
+        for request in list(self.running):
+            if request.finished:  # cancelled while another one's draft was made
+                continue
             emitted += [(request.request_id, token) for token in self._decode(request)]
-            self.running.popleft()
+            if not request.cancelled:  # (it stays the first one if its turn raises)
+                self.running.popleft()
             if not request.finished:
                 self.running.append(request)
         return emitted

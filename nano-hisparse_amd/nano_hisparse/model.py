@@ -634,6 +634,7 @@ class DraftStep:
         self.logits = logits
         self._drafted, self._parents = drafted, parents
         self._request_id, self._cache, self._lengths = request_id, cache, lengths
+        self._request = cache.storage.requests[request_id]
 
     def commit(self, nodes):
         """Append the keys and values of a path of the tree (a root first,
@@ -644,7 +645,7 @@ class DraftStep:
             if not 0 <= node < len(self._parents) or self._parents[node] != parent:
                 raise ValueError("commit takes a path: a root, then each node's child")
         request = self._cache.storage.requests.get(self._request_id)
-        if self._drafted is None or request is None or list(request.lengths) != self._lengths:
+        if self._drafted is None or request is not self._request or list(request.lengths) != self._lengths:
             raise ValueError("the request's history has changed since this step")
         if self._lengths[0] + len(nodes) > request.max_tokens:
             raise ValueError("commit would exceed the request's reserved tokens")

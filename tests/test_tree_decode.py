@@ -277,6 +277,39 @@ def test_bad_proposals_leave_the_request_running(where):
     assert engine.run() == {"a": generate(model, {"a": [1, 2, 3]}, limit=4).requests["a"].generated}
 
 
+def test_drafts_may_cancel_requests(where):
+    """Their own one and others, before and after them in the turn."""
+    model = tiny(where, seed=2)
+    prompts = {"a": [1, 2, 3], "b": [4, 5], "c": [6], "d": [7, 8]}
+    expected = {n: r.generated for n, r in generate(model, prompts).requests.items()}
+    plan = {("b", 2): ["b"], ("c", 3): ["a", "c"]}  # by whose draft, with how many tokens: who is cancelled
+
+    def draft(request):
+        for name in plan.pop((request.request_id, len(request.generated)), []):
+            engine.cancel(name)
+        return None
+
+    engine = Engine(model, cache_for(model, gpu_pages=512, host_pages=512), draft=draft)
+    for name, prompt in prompts.items():
+        engine.add_request(name, prompt, 12)
+    out = engine.run()
+    assert not plan and out["d"] == expected["d"]
+    assert len(out["b"]) == 2 and len(out["c"]) == 3 and len(out["a"]) < 12
+    assert all(out[n] == expected[n][: len(out[n])] for n in prompts)
+    assert not engine.cache.storage.requests
+
+
+def test_a_commit_needs_the_request_that_the_step_was_of(where):
+    model = tiny(where)
+    cache, _ = started(model, [1, 2, 3])
+    step = model.decode_tree([4], [-1], "r", cache)
+    cache.release_request("r")
+    cache.reserve("r", 19, model.config.num_hidden_layers)
+    model.prefill([5, 6, 7], cache, "r")
+    with pytest.raises(ValueError, match="history"):
+        step.commit([0])
+
+
 def test_engine_options_are_checked(where):
     model = tiny(where)
     for bad in (dict(logprobs=-1), dict(logprobs=65)):
