@@ -466,12 +466,13 @@ int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parents, int64_t 
  * h / (q_heads / kv_heads),
  *   out[b, t, h] = softmax_x(q[b, t, h] . K[x] * head_dim^-0.5) . V[x]
  * over the pool rows rows[b, c] in [0, pool_rows) (others are masked) and the
- * drafted nodes j whose bit mask[b, t] holds (k[b, j], v[b, j], not in the
- * pool). A node with mask word 0 yields zeros, and the keys and values of a
- * node with mask word 0, like those that a mask hides, may hold anything.
+ * drafted nodes j whose bit mask[b, t] holds and whose own word is not 0
+ * (k[b, j], v[b, j], not in the pool). A node with mask word 0 yields zeros,
+ * and its keys and values, like those that a mask hides, may hold anything.
  * One dtype for all tensors; strides in elements, dims of a head contiguous;
- * fp32 sums, one rounding of the output. head_dim up to
- * NHS_MAX_TREE_HEAD_DIM, nodes up to NHS_MAX_TREE_NODES, n_rows up to 2^30.
+ * fp32 sums, one rounding of the output, which overlaps no input. head_dim up
+ * to NHS_MAX_TREE_HEAD_DIM, nodes up to NHS_MAX_TREE_NODES, n_rows up to 2^30,
+ * batch up to 2^20.
  * Heads of 32, 64, 128 and (16 bits) 256 whose operands are 16-byte aligned,
  * strides included, run on the matrix cores. pool_block_stride as in
  * nhs_attend_rows. The workspace (nhs_tree_attention_workspace_bytes, 16-byte

@@ -591,7 +591,7 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
     const bool wide = (int64_t)rows * per_wave >= kNormRopeWide;
     const int u = wide ? 2 : 1;
     const int64_t parts = (per_wave + u - 1) / u, waves = rows * parts;
-    if (waves <= 0x7fffffff) {
+    if (waves <= 0x3fffffc) {  // (a launch has 32 bits of threads)
       const dim3 grid((unsigned)((waves + 3) / 4)), block(kRopeThreads);
       const auto run_vec = [&](auto t, auto table, auto l) {
         using T = decltype(t);
@@ -631,7 +631,7 @@ extern "C" int nhs_qk_norm_rope(int32_t rows, int32_t q_heads, int32_t k_heads, 
     }
   }
   const int64_t items = (int64_t)rows * a.heads, blocks = (items + kRopeThreads / kWave - 1) / (kRopeThreads / kWave);
-  if (blocks > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  if (blocks * kRopeThreads > 0xffffffffll) return fail(NHS_ERR_UNSUPPORTED, "%s: too many workgroups", who);
   const auto run = [&](auto kernel) {
     launch(kernel, dim3((unsigned)blocks), dim3(kRopeThreads), 0, s, ev.start, ev.stop, a);
   };

@@ -539,6 +539,7 @@ extern "C" int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_
   const int64_t need = nhs_token_logprobs_workspace_bytes(rows, vocab, dtype, top), parts = (int64_t)rows * shape.splits;
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(NHS_ERR_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", who, (long long)need);
+  if (parts * kLpThreads > 0xffffffffll) return fail(NHS_ERR_UNSUPPORTED, "%s: too many rows", who);
   LogprobArgs a{static_cast<const char*>(logits), row_stride, vocab, top, tokens_per_row, tokens, tokens_stride,
                 logprobs, entropy, top_ids, top_logprobs, shape.splits, shape.split_chunks,
                 static_cast<float4*>(workspace), nullptr};

@@ -69,8 +69,8 @@ struct TreeArgs {
   float scale_log2;  // D^-1/2 * log2(e)
   char* out;
   int64_t o_b, o_n, o_h;
-  float* stats;    // n_splits > 1: [n_splits, batch * nodes * q_heads, 2] (max in base 2, sum)
-  float* partial;  // and [n_splits, batch * nodes * q_heads, head_dim], not divided by the sum
+  float* partial;  // n_splits > 1: [n_splits, batch * nodes * q_heads, head_dim], not divided by the sum
+  float* stats;    // and [n_splits, batch * nodes * q_heads, 2] (max in base 2, sum)
   int64_t out_rows;  // batch * nodes * q_heads
 };
 
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kTgThreads) void tree_general_kernel(TreeArgs a) {
     return;
   }
   const int64_t at = (int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h;
-  const bool some = word != 0 && m != -INFINITY;
+  const bool some = word != 0 && l != 0.f;  // (a NaN among the scores makes l one)
 #pragma unroll
   for (int i = 0; i < DIMS / 16; ++i)
     if (sub + 16 * i < D) store_elem(a.out, T::dtype, at + sub + 16 * i, some ? acc[i] / l : 0.f);
@@ -397,7 +397,17 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[x][i] *= alpha;
     }
-    const float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
+    float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
+    // Scores are scaled and made relative to the maximum in one step, which is off by the rounding of ref. Where that
+    // could exceed a power or two of 2 (and overflow the weights), they are made relative first.
+    const bool large = fabsf(ref) > 0x1p26f;
+    if (__any(large)) {
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] -= large ? m : 0.f;
+      ref = large ? 0.f : ref;
+    }
     float tile_sum = 0.f;
     if constexpr (F) {
 #pragma unroll
@@ -593,7 +603,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
             make_float4(o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]);
     return;
   }
-  const bool some = word != 0 && m != -INFINITY;
+  const bool some = word != 0 && l != 0.f;  // (a NaN among the scores makes l one)
   const float inv = some ? 1.f / l : 0.f;
   char* op = a.out + ((int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h) * T::bytes;
 #pragma unroll
@@ -685,7 +695,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     }
   }
   if (side) return;
-  const bool some = present && top != -INFINITY;
+  const bool some = present && total != 0.f;
   const int64_t at = (int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h + d;
 #pragma unroll
   for (int e = 0; e < 4; ++e) store_elem(a.out, T::dtype, at + e, some ? o[e] / total : 0.f);
@@ -705,12 +715,12 @@ __global__ __launch_bounds__(256) void tree_join_general_kernel(TreeArgs a) {
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float ref = top == -INFINITY ? 0.f : top;
-  const bool some = a.mask[(int64_t)b * a.mask_b + node] != 0 && top != -INFINITY;
   for (int s = lane; s < a.n_splits; s += kWave) {
     const float* st = a.stats + 2 * ((int64_t)s * a.out_rows + out_row);
     total = __builtin_fmaf(__builtin_amdgcn_exp2f(st[0] - ref), st[1], total);
   }
   total = group_sum(total, kWave);
+  const bool some = a.mask[(int64_t)b * a.mask_b + node] != 0 && total != 0.f;
   const int64_t at = (int64_t)b * a.o_b + (int64_t)node * a.o_n + (int64_t)head * a.o_h;
   for (int d = lane; d < D; d += kWave) {
     float o = 0.f;
@@ -787,6 +797,7 @@ extern "C" int nhs_tree_plan(int32_t batch, int32_t nodes, const int32_t* parent
   if (batch < 0 || nodes < 1) return fail(NHS_ERR_INVALID, "nhs_tree_plan: invalid shape");
   if (nodes > kTreeNodes) return fail(NHS_ERR_UNSUPPORTED, "nhs_tree_plan: at most %d nodes", kTreeNodes);
   if (batch == 0) return NHS_OK;
+  if (batch > 0x3ffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_tree_plan: too many trees");
   launch(tree_plan_kernel, dim3((unsigned)batch), dim3(kWave), 0, (hipStream_t)stream, ev.start, ev.stop, parents,
          parents_stride, nodes, lengths, mask, positions);
   return launch_status("nhs_tree_plan");
@@ -841,7 +852,8 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(NHS_ERR_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", who, (long long)need);
   const int64_t blocks = (int64_t)batch * kv_heads * shape.row_blocks * shape.n_splits;
-  if (blocks > 0x7fffffff || (int64_t)batch * nodes * q_heads > 0x7fffffff)
+  const int threads = flash ? shape.waves * shape.shares * kWave : kTgThreads;
+  if (blocks * threads > 0xffffffffll || (int64_t)batch * nodes * q_heads > 0x7fffffff)  // (a launch has 32 bits of threads)
     return fail(NHS_ERR_UNSUPPORTED, "%s: too many workgroups", who);
   TreeArgs a;
   a.q = static_cast<const char*>(q), a.k = static_cast<const char*>(k), a.v = static_cast<const char*>(v);
@@ -863,11 +875,11 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   a.out = static_cast<char*>(out);
   a.o_b = out_batch_stride, a.o_n = out_node_stride, a.o_h = out_head_stride;
   a.out_rows = (int64_t)batch * nodes * q_heads;
-  a.stats = static_cast<float*>(workspace);
-  a.partial = a.stats + 2 * a.out_rows * shape.n_splits;
+  a.partial = static_cast<float*>(workspace);
+  a.stats = a.partial + a.out_rows * shape.n_splits * head_dim;
   hipStream_t s = (hipStream_t)stream;
   const hipEvent_t none = nullptr;
-  const auto run = [&](auto kernel, auto join, int threads, int rows_each) {
+  const auto run = [&](auto kernel, auto join, int rows_each) {
     const bool joined = shape.n_splits > 1;
     launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, s, ev.start, joined ? none : ev.stop, a);
     if (joined)
@@ -876,19 +888,18 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   const auto general = [&](auto tag) {
     using T = decltype(tag);
     if (head_dim <= 128)
-      run(tree_general_kernel<T, 32, 128>, tree_join_general_kernel<T>, kTgThreads, 4);
+      run(tree_general_kernel<T, 32, 128>, tree_join_general_kernel<T>, 4);
     else
-      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_general_kernel<T>, kTgThreads, 4);
+      run(tree_general_kernel<T, 16, kTgMaxDim>, tree_join_general_kernel<T>, 4);
   };
   const auto on_mfma = [&](auto tag, auto dim) {
     using T = decltype(tag);
     constexpr int D = decltype(dim)::value;
-    const int threads = shape.waves * shape.shares * kWave;
     const auto go = [&](auto kernel) {
       if (shape.n_splits > 16)
-        run(kernel, tree_join_kernel<T, D, 4>, threads, 1);
+        run(kernel, tree_join_kernel<T, D, 4>, 1);
       else
-        run(kernel, tree_join_kernel<T, D, 1>, threads, 4);
+        run(kernel, tree_join_kernel<T, D, 1>, 4);
     };
     constexpr int RB = D * T::bytes, BN = RB < 512 ? 64 : 32;  // (tiles of at most 64 KB in two buffers)
     if (shape.waves == 2) return go(tree_flash_kernel<T, D, 2, 2, BN>);

@@ -112,6 +112,12 @@ def _check_out(who, out, shape, dtype, device):
         raise ValueError(f"{who}: out's head dims must be contiguous and its elements distinct")
 
 
+def _check_counts(who, *counts):
+    """Sizes reach the library as 32-bit numbers."""
+    if max(counts) >= 2**31:
+        raise ValueError(f"{who}: sizes must be < 2^31")
+
+
 def timing_events():
     """A (start, stop) pair of timing events usable with set_launch_events."""
     start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -900,6 +906,7 @@ def tree_plan(parents, lengths):
             or lengths.shape != parents.shape[:1]:
         raise ValueError("tree_plan: parents [B, T] int32, lengths [B] int64")
     B, T = parents.shape
+    _check_counts("tree_plan", B)
     if T > MAX_TREE_NODES:
         raise ValueError(f"tree_plan: at most {MAX_TREE_NODES} nodes")
     if parents.stride(1) != 1:
@@ -921,6 +928,7 @@ def tree_attention(query, pool, rows, k, v, mask, page_size, out=None):
     outside the pool, such as -1, are masked) and over the drafted keys and
     values k, v [B, T, Hkv, D] whose bits mask [B, T] (int64, as tree_plan
     makes it) holds. Returns [B, T, Hq, D]; a node with mask 0 yields zeros.
+    `out` may be given and overlaps no input.
     One dtype (bf16, fp16 or fp32) for all, D up to 256."""
     if query.is_cuda:
         done = (_launch or _load_launch()).tree_attention(query, pool, rows, k, v, mask, page_size, out)
@@ -945,6 +953,7 @@ def tree_attention(query, pool, rows, k, v, mask, page_size, out=None):
         raise ValueError(f"tree_attention: at most {MAX_TREE_NODES} nodes and heads of {MAX_TREE_HEAD_DIM}")
     if rows.shape[1] > 2**30:
         raise ValueError("tree_attention: at most 2^30 rows")
+    _check_counts("tree_attention", B, Hq, Hkv)
     if any(t.stride(3) != 1 for t in (query, k, v)):
         raise ValueError("tree_attention: head dims must be contiguous")
     stride = pool_block_stride(pool)
@@ -987,6 +996,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps, cos, sin, positions=None, out=No
     if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype:
         raise ValueError("qk_norm_rope: q [n, Hq, D] and k [n, Hkv, D] of one dtype")
     n, Hq, D = q.shape
+    _check_counts("qk_norm_rope", n, Hq, k.shape[1], D)
     code = dtype_code(q.dtype)
     if D < 2 or D % 2 or Hq < 1 or k.shape[1] < 1:
         raise ValueError("qk_norm_rope: heads of an even number of dims")
@@ -1048,6 +1058,7 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError("token_logprobs: logits [rows, vocab], tokens int64 [rows] or [rows, n]")
     code, top = dtype_code(logits.dtype), int(top)
     R, V = logits.shape
+    _check_counts("token_logprobs", R, tokens[:1].numel())
     if V > 2**30:
         raise ValueError("token_logprobs: a vocabulary of at most 2^30 tokens")
     if V < 1 or not 0 <= top <= min(MAX_TOP_LOGPROBS, V):

@@ -75,7 +75,7 @@ def tree_oracle(q, pool, rows, k, v, mask, page, rounded):
         for t in range(T):
             if mask[b, t] == 0:
                 continue
-            seen = seen_nodes(mask[b])[t]
+            seen = seen_nodes(mask[b])[t] & (mask[b] != 0)  # an absent node is no one's ancestor
             keys = torch.cat((past_k, k[b, seen].double()))
             values = torch.cat((past_v, v[b, seen].double()))
             keys, values = (x.repeat_interleave(g, 1) for x in (keys, values))
@@ -224,6 +224,7 @@ def test_tree_attention_refuses(lib, change, status):
     ((0, 4, 256, 4, 256, 256, 256, None), 0), ((1, 0, 256, 4, 256, 256, 256, None), -1),
     ((-1, 4, 256, 4, 256, 256, 256, None), -1), ((1, 65, 256, 65, 256, 256, 256, None), -2),
     ((1, 4, None, 4, 256, 256, 256, None), -1), ((1, 4, 256, 4, 256, None, 256, None), -1),
+    ((1 << 26, 4, 256, 4, 256, 256, 256, None), -2),
 ])
 def test_tree_plan_refuses(lib, args, status):
     assert lib.nhs_tree_plan(*args) == status
@@ -240,6 +241,8 @@ def test_qk_norm_rope_refuses(lib):
                 dict(table=2), dict(q=None), dict(w=None), dict(cos=None), dict(out=None), dict(table_rows=1),
                 dict(table_rows=0, positions=256), dict(q=257), dict(positions=260)):
         assert status(**bad) == -1, bad
+    for dim in (64, 66):  # more heads than a launch has waves
+        assert status(rows=1 << 26, positions=256, dim=dim, q_heads=62) == -2
 
 
 def test_token_logprobs_refuses(lib):
@@ -248,7 +251,7 @@ def test_token_logprobs_refuses(lib):
                                       ids, 256, 256, 1 << 30, None)
 
     assert status(rows=0) == 0
-    assert status(top=65) == -2 and status(vocab=(1 << 30) + 1) == -2
+    assert status(top=65) == -2 and status(vocab=(1 << 30) + 1) == -2 and status(rows=1 << 24) == -2
     for bad in (dict(rows=-1), dict(vocab=0, top=0), dict(top=-1), dict(top=6, vocab=5), dict(dtype=4),
                 dict(logits=None), dict(tokens=None), dict(ids=None), dict(entropy=None), dict(logits=258),
                 dict(tokens=260), dict(per_row=-1)):
@@ -278,7 +281,11 @@ def test_bad_arguments_raise(gpu):
     for bad in ((p.long(), n), (p, n.int()), (p, n[:1]), (p[0], n), (p.expand(2, 3).new_zeros(2, 65), n)):
         with pytest.raises(ValueError):
             rk.tree_plan(*bad)
+    with pytest.raises(ValueError, match="sizes"):
+        rk.tree_plan(p[:1].expand(2**31, 3), n[:1].expand(2**31))
     x, t = torch.zeros(2, 10, device=gpu), torch.zeros(2, dtype=torch.int64, device=gpu)
+    with pytest.raises(ValueError, match="sizes"):
+        rk.token_logprobs(x[:1].expand(2**31, 10), t[:1].expand(2**31))
     for bad in ((x.double(), t), (x, t.int()), (x, t[:1]), (x[0], t), (x, t, 11), (x, t, -1),
                 (x.new_zeros(2, 100), t, 65), (x.t().contiguous().t(), t), (x[:, :0], t)):
         with pytest.raises(ValueError):
@@ -295,6 +302,8 @@ def test_bad_arguments_raise(gpu):
                 (q, k, w, w, 1e-6, cos[:0], cos[:0], at), (q.cpu(), k, w, w, 1e-6, cos, cos)):
         with pytest.raises(ValueError):
             rk.qk_norm_rope(*bad)
+    with pytest.raises(ValueError, match="sizes"):
+        rk.qk_norm_rope(q[:1].expand(2**31, 4, 8), k[:1].expand(2**31, 2, 8), w, w, 1e-6, cos, cos, at[:1].expand(2**31))
 
 
 # ---- tree_plan ---------------------------------------------------------------------------------
@@ -346,6 +355,39 @@ def test_tree_attention(gpu, dtype, shape):
 def test_tree_attention_peaky_scores(gpu, dtype, D):
     c = tree_case(gpu, dtype, 2, 16, 8, 2, D, 16, 500, seed=5, spread=3.0)
     check_tree(c, run_tree(c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(bf16, 128), (f16, 64), (f32, 32), (bf16, 80)])
+@pytest.mark.parametrize("N", [40, 1500])
+def test_scores_of_billions(gpu, dtype, D, N):
+    """Keys of one number each, queries of another: the scores are exact in
+    fp32 and thousands of powers of two apart, so the output is the mean of the
+    values whose keys are the largest."""
+    print("case:", dict(dtype=dtype, D=D, N=N), flush=True)
+    c = tree_case(gpu, dtype, 2, 5, 4, 2, D, 16, N, seed=N + D, fused=False)
+    blocks, total = len(c["pool"]), c["pool"].shape[0] * 16
+    c["pool"][:, 0] = 128.0 * (torch.arange(total, device=gpu) % 150).view(blocks, 16, 1, 1).to(dtype)
+    c["q"].fill_(2.0 ** (14 if dtype == f16 else 17))
+    c["k"].copy_(128.0 * torch.arange(130, 150, 2, device=gpu).view(2, 5, 1, 1).expand(c["k"].shape))
+    expected, _ = tree_oracle(*(c[n] for n in ("q", "pool", "rows", "k", "v", "mask", "page")), False)
+    # weights of 1 or 0; up to 64 equal keys added and divided
+    check(run_tree(c), expected, HALF[dtype] * expected.abs() + 2.0 ** -25 + 66 * U * 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(bf16, 128), (f16, 64), (f32, 32), (bf16, 80)])
+@pytest.mark.parametrize("N", [0, 40, 1500])
+def test_a_query_that_is_not_a_number_has_no_answer(gpu, dtype, D, N):
+    print("case:", dict(dtype=dtype, D=D, N=N), flush=True)
+    c = tree_case(gpu, dtype, 2, 7, 8, 2, D, 16, N, seed=N + D, fused=False)
+    c["mask"][1, 3] = 0
+    expected, tol = tree_oracle(*(c[n] for n in ("q", "pool", "rows", "k", "v", "mask", "page")), dtype != f32)
+    for b, t, h in ((0, 2, 5), (1, 0, 0), (1, 3, 1)):  # (the last node is absent: zeros)
+        c["q"][b, t, h, D - 1] = float("nan")
+        if (b, t) != (1, 3):
+            expected[b, t, h] = float("nan")
+    check(run_tree(c), expected, tol)
 
 
 @pytest.mark.gpu
