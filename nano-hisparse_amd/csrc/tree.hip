@@ -833,7 +833,7 @@ extern "C" int nhs_tree_attention(const void* q, int64_t q_batch_stride, int64_t
   if (head_dim > kTgMaxDim) return fail(NHS_ERR_UNSUPPORTED, "%s: head_dim up to %d", who, kTgMaxDim);
   if (pool_rows >= (1ll << 31)) return fail(NHS_ERR_UNSUPPORTED, "%s: pool rows must be < 2^31", who);
   const int esize = elem_size(dtype);
-  const int64_t row_bytes = (int64_t)kv_heads * head_dim * esize, block = 2 * page_size * row_bytes;
+  const int64_t row_bytes = (int64_t)kv_heads * head_dim * esize, block = 2ll * page_size * row_bytes;
   if (pool_block_stride == 0) pool_block_stride = block;
   if (pool_block_stride < block || pool_block_stride % esize)
     return fail(NHS_ERR_INVALID, "%s: pool_block_stride is 0 or at least one block of whole elements", who);
