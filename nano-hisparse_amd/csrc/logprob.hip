@@ -19,6 +19,10 @@ namespace nhs {
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave, kLpMaxTop = NHS_MAX_TOP_LOGPROBS;
 constexpr int kLpCandidates = 1024;  // keys held in LDS
 constexpr int kLpMaxSplits = 64;
+// The most alternatives for which the search compares the maxima of four threads each: a quarter of the comparisons, but
+// four times as many chunks to look through. us with one thread / four: one fp32 row of 128256, top 5 10.7 / 9.5, 16 bf16
+// rows, top 8 12.0 / 11.5; 128 rows of 32001, top 20 11.9 / 13.8, 1000 rows, top 60 26.6 / 41.4.
+constexpr int kLpQuadTop = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.693147180559945309417;
 
@@ -181,29 +185,38 @@ __device__ __forceinline__ void lp_sort_found(int n, int top, LogprobShared& sh)
 }
 
 // The `top` largest elements of the part, given each thread's largest (of chunks first + thread, + kLpThreads, ...):
-// the top-th largest of these is a lower bound, and only the few threads that reach it hold elements that count; their
-// chunks are read again and compared by the whole workgroup. Where many threads reach it (masked vocabularies) or more
-// elements than LDS holds, those above it are kept and the equal ones counted off in index order.
+// the top-th largest of these (or of those of four threads each) is a lower bound, and only the few threads that reach
+// it hold elements that count; their chunks are read again and compared by the whole workgroup. Where many threads
+// reach it (masked vocabularies) or more elements than LDS holds, those above it are kept and the equal ones counted
+// off in index order.
 template <typename T>
 __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool any, float thread_max,
                        LogprobShared& sh) {
   constexpr int E = LpRow<T>::E;
   const int tid = threadIdx.x, lane = tid & 63;
   const uint32_t mine = any ? lp_order(thread_max) : 0u;
-  sh.lane_max[tid] = mine;
+  const bool quads = top <= kLpQuadTop;
+  uint32_t best = mine;
+  if (quads) {  // the four threads of a quad stand for one
+    best = max(best, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)best, 0xB1, 0xF, 0xF, false));
+    best = max(best, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)best, 0x4E, 0xF, 0xF, false));
+    if (tid % 4 == 0) sh.lane_max[tid / 4] = best;
+  } else {
+    sh.lane_max[tid] = mine;
+  }
   if (tid == 0) sh.n_hot = sh.n_found = 0, sh.threshold = 0xffffffffu;
   __syncthreads();
-  // the threads with fewer than `top` larger ones; the least of them is the top-th largest
+  // the threads (or quads) with fewer than `top` larger ones; the least of them is the top-th largest
   int larger[2] = {0, 0};
   const uint4* all = reinterpret_cast<const uint4*>(sh.lane_max);
 #pragma unroll 8
-  for (int i = 0; i < kLpThreads / 4; ++i) {
+  for (int i = 0; i < (quads ? kLpThreads / 16 : kLpThreads / 4); ++i) {
     const uint4 v = all[i];
-    larger[0] += (v.x > mine) + (v.z > mine);
-    larger[1] += (v.y > mine) + (v.w > mine);
+    larger[0] += (v.x > best) + (v.z > best);
+    larger[1] += (v.y > best) + (v.w > best);
   }
   if (larger[0] + larger[1] < top) {
-    atomicMin(&sh.threshold, mine);
+    atomicMin(&sh.threshold, best);
     if (mine) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
   }
   __syncthreads();
@@ -234,7 +247,7 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
     }
   };
   // (a row of 128256 with half of it masked: 15 us, where looking through all that reach the bound first took 20)
-  bool ties = sh.n_hot > 2 * top + 32;
+  bool ties = sh.n_hot > (quads ? 8 : 2) * top + 32;
   if (!ties) {
     collect(threshold);
     __syncthreads();
@@ -389,8 +402,8 @@ __device__ __forceinline__ bool lp_usual(const LpSums& t) { return t.s > 0.f && 
 // alternatives starts from. Long prompts are bound by memory: 4000 bf16 rows
 // of 128256, read once, 188 us (5.5 TB/s; with a maximum, a sum and a search
 // in passes of their own 1626). Short ones by the chain of steps, each waiting
-// for the last: one row of 128256 takes 5.5 us without alternatives and 11 with
-// five, 128 rows of 32001 6.7 and 12 (a launch that does nothing, 2).
+// for the last: one row of 128256 takes 5.5 us without alternatives and 9.5 with
+// five, 128 rows of 32001 6.7 and 10 (a launch that does nothing, 2).
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
   constexpr int E = LpRow<T>::E, U = 4;
