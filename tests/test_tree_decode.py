@@ -277,6 +277,26 @@ def test_bad_proposals_leave_the_request_running(where):
     assert engine.run() == {"a": generate(model, {"a": [1, 2, 3]}, limit=4).requests["a"].generated}
 
 
+def test_what_followed_the_same_tokens_before_as_a_draft(where):
+    """The loops that small random models fall into are found by looking them up."""
+
+    def draft(request):
+        text = request.prompt + request.generated
+        for at in range(len(text) - 3, 0, -1):
+            if text[at - 1: at + 1] == text[-2:]:
+                tokens = text[at + 1: at + 6]
+                return tokens, list(range(-1, len(tokens) - 1))
+
+    model = tiny(where, seed=4)
+    prompts = {"a": [7, 3, 9, 4] * 4, "b": [1, 2, 3]}
+    plain = generate(model, prompts, limit=40)
+    engine = generate(model, prompts, limit=40, draft=draft)
+    for name, r in engine.requests.items():
+        assert r.generated == plain.requests[name].generated
+        assert r.decode_count + r.accepted_count == 39
+    assert sum(r.drafted_count for r in engine.requests.values()) > 0
+
+
 def test_drafts_may_cancel_requests(where):
     """Their own one and others, before and after them in the turn."""
     model = tiny(where, seed=2)
