@@ -19,10 +19,10 @@ namespace nhs {
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave, kLpMaxTop = NHS_MAX_TOP_LOGPROBS;
 constexpr int kLpCandidates = 1024;  // keys held in LDS
 constexpr int kLpMaxSplits = 64;
-// The most alternatives for which the search compares the maxima of four threads each: a quarter of the comparisons, but
-// four times as many chunks to look through. us with one thread / four: one fp32 row of 128256, top 5 10.7 / 9.5, 16 bf16
-// rows, top 8 12.0 / 11.5; 128 rows of 32001, top 20 11.9 / 13.8, 1000 rows, top 60 26.6 / 41.4.
-constexpr int kLpQuadTop = 8;
+// The most alternatives for which the bound comes from the maxima of four threads each: a quarter of the comparisons, but
+// a lower bound, which more threads reach. us with one thread / four: one bf16 row of 32001, top 5 9.0 / 8.1, 128 of
+// them, top 10 10.7 / 9.8, top 20 11.9 / 11.3, top 32 12.8 / 13.1.
+constexpr int kLpQuadTop = 24;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.693147180559945309417;
 
@@ -215,16 +215,15 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
     larger[0] += (v.x > best) + (v.z > best);
     larger[1] += (v.y > best) + (v.w > best);
   }
-  if (larger[0] + larger[1] < top) {
-    atomicMin(&sh.threshold, best);
-    if (mine) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
-  }
+  if (larger[0] + larger[1] < top) atomicMin(&sh.threshold, best);
   __syncthreads();
   const uint32_t threshold = sh.threshold;
+  if (mine && mine >= threshold) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
+  __syncthreads();
   const int per_thread = (part.last - part.first + kLpThreads - 1) / kLpThreads;
   // pushes the elements whose order is at least `least`
   const auto collect = [&](uint32_t least) {
-    const int pairs = sh.n_hot * per_thread;  // at most 256 threads x their chunks: the part
+    const int log = 32 - __clz(max(per_thread, 1) - 1), pairs = sh.n_hot << log;  // (chunks of a thread, to a power of two)
     const auto push = [&](float x, int i) {
       if (lp_order(x) >= least) {
         const int at = atomicAdd(&sh.n_found, 1);
@@ -232,7 +231,7 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
       }
     };
     for (int p = tid; p < pairs; p += kLpThreads) {
-      const int chunk = part.first + sh.hot[p / per_thread] + (p % per_thread) * kLpThreads;
+      const int chunk = part.first + sh.hot[p >> log] + (p & ((1 << log) - 1)) * kLpThreads;
       if (chunk >= part.last) continue;
       float x[E];
       LpRow<T>::unpack(row.load(chunk), x);
@@ -247,7 +246,7 @@ __device__ void lp_top(const LpRow<T>& row, const LpPart& part, int top, bool an
     }
   };
   // (a row of 128256 with half of it masked: 15 us, where looking through all that reach the bound first took 20)
-  bool ties = sh.n_hot > (quads ? 8 : 2) * top + 32;
+  bool ties = sh.n_hot > 2 * top + 32;
   if (!ties) {
     collect(threshold);
     __syncthreads();
@@ -400,10 +399,10 @@ __device__ __forceinline__ bool lp_usual(const LpSums& t) { return t.s > 0.f && 
 // relative to it, and references only ever meet as these numbers), S and W
 // over blocks of four chunks, and its largest logit, which the search for the
 // alternatives starts from. Long prompts are bound by memory: 4000 bf16 rows
-// of 128256, read once, 188 us (5.5 TB/s; with a maximum, a sum and a search
+// of 128256, read once, 185 us (5.5 TB/s; with a maximum, a sum and a search
 // in passes of their own 1626). Short ones by the chain of steps, each waiting
 // for the last: one row of 128256 takes 5.5 us without alternatives and 9.5 with
-// five, 128 rows of 32001 6.7 and 10 (a launch that does nothing, 2).
+// five, 128 rows of 32001 6.7 and 9.5 (a launch that does nothing, 2).
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
   constexpr int E = LpRow<T>::E, U = 4;
