@@ -260,7 +260,8 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 // widest trees.) fp32 weights are not rounded.
 //
 // With QW = 1 a wave loads and reads its own tiles only and no barrier stands
-// in the loop.
+// in the loop (the four shares are joined in two steps: one share after the
+// other took 8.0 us where two steps take 7.5, one request of 128 rows).
 //
 // Measured (MI355X, bf16, rows read from HBM, us with the join of the splits):
 // 8 requests x 16 nodes x 32/8 heads of 128 x 2048 rows 30 (23 without the
@@ -546,14 +547,15 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
 
   l += __shfl_xor(l, 32);
   if constexpr (KW > 1) {
-    // the waves of the other shares hand their sums over through the tile buffers, one share at a time (registers by
-    // lane: the partners hold the same query rows and dims)
-    float* part = reinterpret_cast<float*>(wave == 0 ? k0 : wave == 1 ? v0 : wave == 2 ? k1 : v1) + lane;
-    float* stat = reinterpret_cast<float*>(stage) + wave * 2 * kWave + lane;
-    static_assert(QW <= 4 && DB * 16 * kWave * 4 <= KW * kTile && QW * 2 * kWave * 4 <= kTfStage * 8, "merge space");
-    for (int from = 1; from < KW; ++from) {
+    // the upper half of the shares hands its sums over to the lower half through the tile buffers, until one is left
+    // (registers by lane: the partners hold the same query rows and dims)
+    static_assert(W <= 8 && DB * 16 * kWave * 4 <= KW * kTile && W * kWave * 4 <= kTfStage * 8, "merge space");
+    for (int step = KW / 2; step > 0; step /= 2) {
+      const int area = wave * (KW / 2) + share % step;  // below W / 2
+      float* part = reinterpret_cast<float*>(area == 0 ? k0 : area == 1 ? v0 : area == 2 ? k1 : v1) + lane;
+      float* stat = reinterpret_cast<float*>(stage) + area * 2 * kWave + lane;
       __syncthreads();
-      if (share == from) {
+      if (share / step == 1) {
 #pragma unroll
         for (int x = 0; x < DB; ++x)
 #pragma unroll
@@ -562,7 +564,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         stat[kWave] = l;
       }
       __syncthreads();
-      if (share == 0) {
+      if (share < step) {
         const float m2 = stat[0], l2 = stat[kWave];
         const float both = fmaxf(m, m2), ref = both == -INFINITY ? 0.f : both;
         const float f1 = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2);
