@@ -267,7 +267,7 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 // 8 requests x 16 nodes x 32/8 heads of 128 x 2048 rows 30 (23 without the
 // join; the rows stream at 5.5 TB/s once they flow, but 6 us pass before the
 // first are in, and 2.5 at the end); one request x 32 nodes x 32768 rows 50 (39);
-// 16 requests x 64 nodes x 28/4 heads x 4096 rows 107 (570 TFLOP/s): bound by
+// 16 requests x 64 nodes x 28/4 heads x 4096 rows 102 (595 TFLOP/s): bound by
 // the matrix cores, LDS reads and softmax in about equal parts (85 without the
 // loads, 65 with them alone). With the general kernel 932, 3685 and 10818.
 //
@@ -319,6 +319,8 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 32);
   }
+  // a wave past the last query row only loads (448 rows in blocks of 128: 105.5 -> 102 us, widest trees)
+  const bool alive = (block * QW + wave) * 32 < a.query_rows;
   float m = -INFINITY, l = 0.f;  // running max (of the unscaled scores) and this lane's share of the denominator
   pf_f32x16 o[DB];
 #pragma unroll
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         for (int x = 0; x < NB; ++x)
           seen[x] = some ? (uint32_t)((word & present) >> (share * BN + 32 * x)) : 0u;
       }
-      if (some) tile(kb, vb, seen);
+      if (some && alive) tile(kb, vb, seen);
     };
     for (int t = -1; t < rounds; t += 2) {
       if (t >= 0 || with_draft) round(t, k0, v0, k1, v1);
