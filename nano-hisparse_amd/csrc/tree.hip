@@ -764,8 +764,8 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
         (int64_t)batch * kv_heads * ((query_rows + 255) / 256) >= 256)
       s.waves = 8, s.shares = 1;
     block_rows = 32 * s.waves;
-    // One workgroup per CU, none of less than 128 keys. us with one / two per CU: one request of 8 nodes x 16384 keys
-    // 27.4 / 36.8, rows of 64 bytes x 32768 keys 15.5 / 18.9. With at least 64 / 128 / 256 keys: 8 nodes x 2048 keys
+    // One workgroup per CU, of rounds of 128 keys. us with one / two per CU: one request of 8 nodes x 16384 keys
+    // 27.4 / 36.8, rows of 64 bytes x 32768 keys 15.5 / 18.9. In rounds of 64 / 128 / 256: 8 nodes x 2048 keys
     // 19.0 / 16.7 / 18.0, 32 nodes 26.7 / 17.9 / 19.5, x 512 keys 15.0 / 14.9 / 16.5.
     per_cu = 1;
     least = 128;
@@ -773,6 +773,23 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
   s.row_blocks = (query_rows + block_rows - 1) / block_rows;
   const int64_t items = (int64_t)batch * kv_heads * s.row_blocks;
   const int64_t wanted = std::max<int64_t>(1, 256 * per_cu / items), most = std::max(1, n_rows / least);
+  if (flash) {
+    // The draft is a round too, of the last split, so the longest split has `longest` rounds, it among them, and the
+    // last one may have nothing else. us with splits of equal numbers of keys, the draft on top / so: 16 nodes x 512
+    // keys 14.3 / 12.5, 4 requests of them 16.6 / 14.4, x 960 keys 19.2 / 16.6, fp32 heads of 32 x 448 keys 13.2 / 9.9.
+    // Splitting pays where it saves more than the join costs, which is about 2.3 us and the partial sums at 5.5 TB/s; a
+    // round takes 1.6 us. us whole / split: 256 keys, 8 requests of 16 nodes 14.5 / 17.8, one request 13.3 / 12.3.
+    const int rounds = (n_rows + least - 1) / least, total = rounds + 1;
+    const int longest = (int)((total + wanted - 1) / wanted), splits = (total + longest - 1) / longest;
+    const double joined = longest * 1.6 + 2.3 + (double)splits * batch * nodes * q_heads * head_dim * 8 / 5.5e6;
+    s.n_splits = 1, s.rows_per_split = std::max(n_rows, 1);
+    if (splits > 1 && joined < total * 1.6) {
+      s.n_splits = splits;
+      s.rows_per_split =
+          std::max((rounds - longest + splits - 1) / (splits - 1), (rounds + splits - 1) / splits) * least;
+    }
+    return s;
+  }
   s.n_splits = (int)std::min(wanted, most);
   s.rows_per_split = std::max(((n_rows + s.n_splits - 1) / s.n_splits + least - 1) / least * least, 1);
   s.n_splits = std::max(1, (n_rows + s.rows_per_split - 1) / s.rows_per_split);
