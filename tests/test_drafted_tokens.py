@@ -351,6 +351,17 @@ def test_tree_attention(gpu, dtype, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(bf16, 128), (f32, 32)])
+@pytest.mark.parametrize("B,T", [(1, 16), (5, 64)])
+@pytest.mark.parametrize("N", [1, 127, 128, 129, 256, 257, 384, 500, 512, 513, 640, 2049])
+def test_tree_attention_around_the_borders_of_splits(gpu, dtype, D, B, T, N):
+    """Whole, split, and with splits that have the draft alone."""
+    print("case:", dict(dtype=dtype, D=D, B=B, T=T, N=N), flush=True)
+    c = tree_case(gpu, dtype, B, T, 4, 2, D, 16, N, seed=N + B)
+    check_tree(c, run_tree(c))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,D", [(bf16, 128), (f16, 64), (f32, 32), (bf16, 80)])
 def test_tree_attention_peaky_scores(gpu, dtype, D):
     c = tree_case(gpu, dtype, 2, 16, 8, 2, D, 16, 500, seed=5, spread=3.0)
