@@ -151,19 +151,26 @@ class Engine:
             tree, above, request.request_id, self.cache, self.top_k, self.backend, selector=self.selector,
         )
         choices = self._choose(step.logits)
+        room = request.max_new_tokens - len(request.generated)
+        path = self._accepted(tree, above, choices, room)
+        if len(path) < room and choices[path[-1]][0] != self.eos_token_id:  # the request goes on
+            step.commit(path)  # before anything is emitted: an append may be refused
         request.decode_count += 1
         request.drafted_count += len(tokens)
-        emitted, path, node = [], [], 0
-        while node is not None:
-            path.append(node)
-            emitted.append(self._emit(request, choices[node]))
-            if request.finished:
-                break
-            node = next((t for t in range(node + 1, len(tree)) if above[t] == node and tree[t] == emitted[-1]), None)
         request.accepted_count += len(path) - 1
-        if not request.finished:
-            step.commit(path)
-        return emitted
+        return [self._emit(request, choices[node]) for node in path]
+
+    def _accepted(self, tree, above, choices, room):
+        """The path of a verified tree that greedy decoding takes, of at most
+        `room` nodes, up to the one after which the text ends."""
+        path = [0]
+        while len(path) < room and choices[path[-1]][0] != self.eos_token_id:
+            node = path[-1]
+            node = next((t for t in range(node + 1, len(tree)) if above[t] == node and tree[t] == choices[node][0]), None)
+            if node is None:
+                break
+            path.append(node)
+        return path
 
     def _admit(self, request):
         layers = self.model.config.num_hidden_layers

@@ -1,0 +1,53 @@
+"""Turns of the engine with drafts that do not go as planned: appends that
+are refused. The text has to be that of plain decoding."""
+
+import pytest
+
+from nano_hisparse.engine import Engine
+from nano_hisparse.storage import PageLease
+from test_tree_decode import PROMPTS, cache_for, generate, tiny, where  # noqa: F401 (where is a fixture)
+
+
+def texts(engine):
+    return {name: r.generated for name, r in engine.requests.items()}
+
+
+def chain(tokens):
+    """A draft of tokens that follow one another."""
+    return list(tokens), list(range(-1, len(tokens) - 1))
+
+
+def lease_of(engine, name, layers):
+    store = engine.cache.storage
+    return PageLease(store, [p for key, p in store.pages.items() if key[0] == name and key[1] in layers])
+
+
+# ---- appends that are refused ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("layers", [(0,), (0, 1)])
+@pytest.mark.parametrize("drafted", [1, 3])
+def test_a_turn_whose_append_is_refused_emits_nothing_and_is_made_again(where, layers, drafted):  # noqa: F811
+    """The store refuses to append to a layer that a reader holds."""
+    model = tiny(where, seed=2)
+    expected = texts(generate(model, PROMPTS))["a"]
+    engine = Engine(model, cache_for(model),
+                    draft=lambda r: chain(expected[len(r.generated):][:drafted]))
+    request = engine.add_request("a", PROMPTS["a"], 12)
+    engine.step()
+    while not request.finished:
+        before = list(request.generated)
+        if len(before) + drafted + 1 < 12:  # (a turn that ends the request appends nothing)
+            lease = lease_of(engine, "a", layers)
+            with pytest.raises(RuntimeError, match="lease"):
+                engine.step()
+            lease.release()
+            assert request.generated == before and not request.logprobs
+            lengths = engine.cache.storage.requests["a"].lengths
+            assert lengths == [len(PROMPTS["a"]) + len(before) - 1] * 2
+        engine.step()
+        assert len(request.generated) > len(before)
+    assert request.generated == expected
+    engine.cache.collect(wait=True)
+    assert not engine.cache.storage.requests
+    engine.cache.assert_invariants()
