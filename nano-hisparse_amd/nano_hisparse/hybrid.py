@@ -586,6 +586,14 @@ class HybridKVCache:
         self.pending_clean.add(page.key)
         self.update_residency(*page.key[:2])
 
+    def check_unleased(self, request_id):
+        """Raises as write does if any layer of a request has active leases."""
+        layers = range(self.storage.requests[request_id].layers)
+        if any(self.tables[request_id, layer].busy for layer in layers):
+            raise RuntimeError("cannot append during a row lease")
+        if any(key[0] == request_id for key in self.storage.pinned):
+            raise RuntimeError("cannot append while a layer has active attention leases")
+
     def write(self, request_id, layer, k, v):
         if self.tables[request_id, layer].busy:
             raise RuntimeError("cannot append during a row lease")

@@ -639,7 +639,9 @@ class DraftStep:
     def commit(self, nodes):
         """Append the keys and values of a path of the tree (a root first,
         then each node's child) to the request's history in the cache. Once
-        per step, while the history is the one that the step attended to."""
+        per step, while the history is the one that the step attended to; a
+        commit that a reader's lease on any layer refuses has appended nothing
+        and may be repeated."""
         nodes = list(nodes)
         for parent, node in zip([-1] + nodes, nodes):
             if not 0 <= node < len(self._parents) or self._parents[node] != parent:
@@ -651,6 +653,7 @@ class DraftStep:
             raise ValueError("commit would exceed the request's reserved tokens")
         if not nodes:
             return
+        self._cache.check_unleased(self._request_id)
         drafted, self._drafted = self._drafted, None
         path = nodes[0] == 0 and nodes == list(range(len(nodes)))
         at = None if path else upload(nodes, torch.int64, drafted[0][0].device)

@@ -25,7 +25,7 @@ def lease_of(engine, name, layers):
 # ---- appends that are refused ------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("layers", [(0,), (0, 1)])
+@pytest.mark.parametrize("layers", [(0,), (1,), (0, 1)])
 @pytest.mark.parametrize("drafted", [1, 3])
 def test_a_turn_whose_append_is_refused_emits_nothing_and_is_made_again(where, layers, drafted):  # noqa: F811
     """The store refuses to append to a layer that a reader holds."""
@@ -50,4 +50,24 @@ def test_a_turn_whose_append_is_refused_emits_nothing_and_is_made_again(where, l
     assert request.generated == expected
     engine.cache.collect(wait=True)
     assert not engine.cache.storage.requests
+    engine.cache.assert_invariants()
+
+
+def test_a_refused_commit_may_be_repeated(where):  # noqa: F811
+    model = tiny(where)
+    engine = Engine(model, cache_for(model))
+    engine.add_request("r", [1, 2, 3], 12)
+    engine.step()
+    step = model.decode_tree([4, 5], [-1, 0], "r", engine.cache)
+    lengths = list(engine.cache.storage.requests["r"].lengths)
+    for layers in ((0,), (1,)):
+        lease = lease_of(engine, "r", layers)
+        with pytest.raises(RuntimeError, match="lease"):
+            step.commit([0, 1])
+        lease.release()
+        assert engine.cache.storage.requests["r"].lengths == lengths
+    step.commit([0, 1])
+    assert engine.cache.storage.requests["r"].lengths == [n + 2 for n in lengths]
+    with pytest.raises(ValueError, match="has changed"):
+        step.commit([0])
     engine.cache.assert_invariants()
