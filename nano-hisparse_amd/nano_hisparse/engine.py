@@ -189,7 +189,9 @@ class Engine:
 
     def step(self):
         """Admit at most one prompt, then one decode turn per running request
-        (several tokens where a draft's were accepted).
+        (several tokens where a draft's were accepted). A request whose turn
+        raises stays, behind the others, whose turns come first in the next
+        step.
 
         Returns [(request_id, token)] in emission order.
         """
@@ -218,11 +220,13 @@ class Engine:
         for request in list(self.running):
             if request.finished:  # cancelled while another one's draft was made
                 continue
-            emitted += [(request.request_id, token) for token in self._decode(request)]
-            if not request.cancelled:  # (it stays the first one if its turn raises)
-                self.running.popleft()
-            if not request.finished:
-                self.running.append(request)
+            try:
+                emitted += [(request.request_id, token) for token in self._decode(request)]
+            finally:  # (a request whose turn raises goes behind the others too)
+                if not request.cancelled:
+                    self.running.popleft()
+                if not request.finished:
+                    self.running.append(request)
         return emitted
 
     def run(self):

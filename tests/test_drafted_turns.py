@@ -71,3 +71,79 @@ def test_a_refused_commit_may_be_repeated(where):  # noqa: F811
     with pytest.raises(ValueError, match="has changed"):
         step.commit([0])
     engine.cache.assert_invariants()
+
+
+# ---- turns that raise ----------------------------------------------------------------------------
+
+
+def failing(model, monkeypatch, name, times=None, after=False):
+    """Makes the decode turns of one request raise (its first `times` ones),
+    before they compute anything or after."""
+    left = [times]
+    for method in ("decode", "decode_tree"):
+        real = getattr(model, method)
+
+        def call(tokens, *a, real=real, tree=method == "decode_tree", **kw):
+            of = a[1] if tree else a[0]
+            fails = of == name and left[0] != 0
+            if fails and left[0] is not None:
+                left[0] -= 1
+            if fails and not after:
+                raise RuntimeError("planned")
+            result = real(tokens, *a, **kw)
+            if fails:
+                raise RuntimeError("planned")
+            return result
+
+        monkeypatch.setattr(model, method, call)
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("bad", ["a", "b", "c"])
+def test_a_request_whose_turns_raise_holds_up_no_other(where, monkeypatch, bad, drafts):  # noqa: F811
+    model = tiny(where, seed=2)
+    prompts = {"a": [1, 2, 3], "b": [4, 5], "c": [6, 7, 8, 9]}
+    expected = texts(generate(model, prompts, gpu_pages=512, host_pages=512))
+    draft = (lambda r: chain(expected[r.request_id][len(r.generated):][:2])) if drafts else None
+    engine = Engine(model, cache_for(model, gpu_pages=512, host_pages=512), draft=draft)
+    for name, prompt in prompts.items():
+        engine.add_request(name, prompt, 12)
+    for _ in range(3):
+        engine.step()  # every prompt is in
+    at = len(engine.requests[bad].generated)
+    failing(model, monkeypatch, bad)
+    raised = 0
+    for _ in range(25):
+        try:
+            engine.step()
+        except RuntimeError as e:
+            assert str(e) == "planned"
+            raised += 1
+    assert raised >= 5  # it is tried again and again
+    for name in prompts:
+        assert engine.requests[name].generated == (expected[name] if name != bad else expected[name][:at])
+    monkeypatch.undo()
+    assert engine.run() == expected
+    engine.cache.assert_invariants()
+
+
+def test_a_request_that_ends_while_it_is_read_takes_no_more_turns(where):  # noqa: F811
+    """Its blocks cannot be released then; it is done all the same."""
+    model = tiny(where, seed=2)
+    expected = texts(generate(model, PROMPTS))
+    engine = Engine(model, cache_for(model), draft=lambda r: chain(expected[r.request_id][len(r.generated):])
+                    if r.request_id == "a" or len(r.generated) > 1 else None)
+    for name, prompt in PROMPTS.items():
+        engine.add_request(name, prompt, 12)
+    engine.step()
+    engine.step()
+    assert engine.requests["a"].finished and not engine.requests["b"].finished
+    lease = lease_of(engine, "b", (0,))
+    with pytest.raises(RuntimeError, match="lease"):
+        engine.step()
+    for _ in range(3):
+        assert engine.step() == []
+    assert texts(engine) == expected and not engine.running
+    lease.release()
+    engine.cache.release_request("b")
+    engine.cache.assert_invariants()
