@@ -191,7 +191,8 @@ class Engine:
         """Admit at most one prompt, then one decode turn per running request
         (several tokens where a draft's were accepted). A request whose turn
         raises stays, behind the others, whose turns come first in the next
-        step.
+        step. If the turn had appended keys and values it cannot be made again
+        and the request takes no more turns (cancel() releases it).
 
         Returns [(request_id, token)] in emission order.
         """
@@ -225,9 +226,15 @@ class Engine:
             finally:  # (a request whose turn raises goes behind the others too)
                 if not request.cancelled:
                     self.running.popleft()
-                if not request.finished:
+                if not request.finished and self._whole(request):
                     self.running.append(request)
         return emitted
+
+    def _whole(self, request):
+        """Whether a request's history is that of its tokens: every one but
+        the last in every layer."""
+        tokens = len(request.prompt) + len(request.generated) - 1
+        return all(n == tokens for n in self.cache.storage.requests[request.request_id].lengths)
 
     def run(self):
         while self.waiting or self.running:
@@ -242,6 +249,7 @@ class Engine:
         if request in self.waiting:
             self.waiting.remove(request)
         else:
-            self.running.remove(request)
+            if request in self.running:
+                self.running.remove(request)
             self.cache.release_request(request_id, wait=False)
         request.finished = request.cancelled = True

@@ -147,3 +147,44 @@ def test_a_request_that_ends_while_it_is_read_takes_no_more_turns(where):  # noq
     lease.release()
     engine.cache.release_request("b")
     engine.cache.assert_invariants()
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+def test_a_turn_that_raises_after_it_has_appended_is_not_made_again(where, monkeypatch, drafts):  # noqa: F811
+    """The last token's keys would be in the history twice. (A tree appends nothing before its commit.)"""
+    model = tiny(where, seed=2)
+    expected = texts(generate(model, PROMPTS))
+    draft = (lambda r: chain(expected[r.request_id][len(r.generated):][:2])) if drafts else None
+    engine = Engine(model, cache_for(model, gpu_pages=512, host_pages=512), draft=draft)
+    for name, prompt in PROMPTS.items():
+        engine.add_request(name, prompt, 12)
+    for _ in range(2):
+        engine.step()
+    failing(model, monkeypatch, "a", times=1, after=True)
+    with pytest.raises(RuntimeError, match="planned"):
+        engine.step()
+    at = len(engine.requests["a"].generated)
+    out = engine.run()
+    assert out["b"] == expected["b"]
+    assert out["a"] == (expected["a"] if drafts else expected["a"][:at])
+    if not drafts:
+        engine.cancel("a")
+    engine.cache.collect(wait=True)
+    assert not engine.cache.storage.requests
+    engine.cache.assert_invariants()
+
+
+def test_a_cancelled_request_may_have_left(where, monkeypatch):  # noqa: F811
+    """A layer of it written and the next one refused: the request waits for its cancellation."""
+    model = tiny(where, seed=2)
+    engine = Engine(model, cache_for(model))
+    engine.add_request("a", PROMPTS["a"], 12)
+    engine.step()
+    lease = lease_of(engine, "a", (1,))
+    with pytest.raises(RuntimeError, match="lease"):
+        engine.step()
+    lease.release()
+    assert not engine.running and not engine.requests["a"].finished and engine.step() == []
+    engine.cancel("a")
+    assert engine.requests["a"].cancelled and not engine.cache.storage.requests
+    engine.cache.assert_invariants()
