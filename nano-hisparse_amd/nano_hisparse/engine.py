@@ -87,6 +87,8 @@ class Engine:
         self.requests: dict = {}
         self.waiting: deque = deque()
         self.running: deque = deque()
+        self._events: list = []  # emitted in this step, or in steps that raised
+        self._failed: set = set()  # requests whose turns raised since a step returned
 
     def add_request(self, request_id, prompt, max_new_tokens=16):
         if request_id in self.requests or not prompt or max_new_tokens < 1:
@@ -121,18 +123,18 @@ class Engine:
     def _emit(self, request, choice):
         token, info = choice
         request.generated.append(token)
+        self._events.append((request.request_id, token))
         if info is not None:
             request.logprobs.append(info)
         if token == self.eos_token_id or len(request.generated) >= request.max_new_tokens:
             request.finished = True
             self.cache.release_request(request.request_id, wait=False)
-        return token
 
     def _decode(self, request):
-        """One decode turn of a request: the tokens it emits."""
+        """One decode turn of a request."""
         proposal = self.draft(request) if self.draft is not None else None
         if request.finished:  # cancelled meanwhile
-            return []
+            return
         tokens, parents = proposal if proposal is not None else ((), ())
         if len(tokens) != len(parents):
             raise ValueError("a draft is a token list and a parent for each token")
@@ -142,7 +144,7 @@ class Engine:
                 selector=self.selector,
             )
             request.decode_count += 1
-            return [self._emit(request, self._choose(logits[None])[0])]
+            return self._emit(request, self._choose(logits[None])[0])
         tree = [request.generated[-1], *tokens]
         above = [-1, *(p + 1 for p in parents)]
         if min(above[1:]) < 0:
@@ -158,7 +160,8 @@ class Engine:
         request.decode_count += 1
         request.drafted_count += len(tokens)
         request.accepted_count += len(path) - 1
-        return [self._emit(request, choices[node]) for node in path]
+        for node in path:
+            self._emit(request, choices[node])
 
     def _accepted(self, tree, above, choices, room):
         """The path of a verified tree that greedy decoding takes, of at most
@@ -194,15 +197,22 @@ class Engine:
         step. If the turn had appended keys and values it cannot be made again
         and the request takes no more turns (cancel() releases it).
 
-        Returns [(request_id, token)] in emission order.
+        Returns [(request_id, token)] in emission order, those of steps that
+        raised before it among them; so that they are not kept for long, the
+        step after one that raised leaves out the requests whose turns did.
         """
-        emitted = []
+        self._turns()
+        events, self._events = self._events, []
+        self._failed = set()
+        return events
+
+    def _turns(self):
         self.cache.collect()
         if self.waiting and self._admit(self.waiting[0]):
             request = self.waiting.popleft()
             logits = self.model.prefill(request.prompt, self.cache, request.request_id)
             request.prefill_count += 1
-            emitted.append((request.request_id, self._emit(request, self._choose(logits[None])[0])))
+            self._emit(request, self._choose(logits[None])[0])
             if not request.finished:
                 self.running.append(request)
         if self.batch_decode and self.running:
@@ -214,27 +224,33 @@ class Engine:
             )
             for request, choice in zip(batch, self._choose(logits)):
                 request.decode_count += 1
-                emitted.append((request.request_id, self._emit(request, choice)))
+                self._emit(request, choice)
                 if not request.finished:
                     self.running.append(request)
-            return emitted
+            return
+        others = {r.request_id for r in self.running} | {name for name, _ in self._events}
+        left_out = self._failed if self._events and len(others) > 1 else ()
         for request in list(self.running):
             if request.finished:  # cancelled while another one's draft was made
                 continue
             try:
-                emitted += [(request.request_id, token) for token in self._decode(request)]
+                if request.request_id not in left_out:
+                    self._decode(request)
+            except BaseException:
+                self._failed = self._failed | {request.request_id}
+                raise
             finally:  # (a request whose turn raises goes behind the others too)
                 if not request.cancelled:
                     self.running.popleft()
                 if not request.finished and self._whole(request):
                     self.running.append(request)
-        return emitted
 
     def _whole(self, request):
         """Whether a request's history is that of its tokens: every one but
         the last in every layer."""
         tokens = len(request.prompt) + len(request.generated) - 1
-        return all(n == tokens for n in self.cache.storage.requests[request.request_id].lengths)
+        stored = self.cache.storage.requests.get(request.request_id)
+        return stored is not None and all(n == tokens for n in stored.lengths)
 
     def run(self):
         while self.waiting or self.running:

@@ -141,8 +141,8 @@ def test_a_request_that_ends_while_it_is_read_takes_no_more_turns(where):  # noq
     lease = lease_of(engine, "b", (0,))
     with pytest.raises(RuntimeError, match="lease"):
         engine.step()
-    for _ in range(3):
-        assert engine.step() == []
+    assert engine.step() == [("b", token) for token in expected["b"][2:]]
+    assert engine.step() == []
     assert texts(engine) == expected and not engine.running
     lease.release()
     engine.cache.release_request("b")
@@ -188,3 +188,59 @@ def test_a_cancelled_request_may_have_left(where, monkeypatch):  # noqa: F811
     engine.cancel("a")
     assert engine.requests["a"].cancelled and not engine.cache.storage.requests
     engine.cache.assert_invariants()
+
+
+def steps_until_done(engine, limit=200):
+    """Every event that step() returns, whatever it raises in between."""
+    events = []
+    for _ in range(limit):
+        if not engine.waiting and not engine.running:
+            return events
+        try:
+            events += engine.step()
+        except (RuntimeError, ValueError):
+            pass
+    raise AssertionError("not done")
+
+
+@pytest.mark.parametrize("bad", ["a", "b", "c"])
+def test_steps_that_raise_lose_no_events(where, bad):  # noqa: F811
+    """Proposals that are refused now and then: what step() returns is still every token in order."""
+    model = tiny(where, seed=2)
+    prompts = {"a": [1, 2, 3], "b": [4, 5], "c": [6, 7, 8, 9]}
+    expected = texts(generate(model, prompts, gpu_pages=512, host_pages=512))
+    calls = dict.fromkeys(prompts, 0)
+
+    def draft(r):
+        calls[r.request_id] += 1
+        if r.request_id == bad and calls[bad] % 3:
+            return [1], [0]
+        return chain(expected[r.request_id][len(r.generated):][: calls[r.request_id] % 3])
+
+    engine = Engine(model, cache_for(model, gpu_pages=512, host_pages=512), draft=draft)
+    for name, prompt in prompts.items():
+        engine.add_request(name, prompt, 12)
+    events = steps_until_done(engine)
+    assert texts(engine) == expected
+    for name in prompts:
+        assert [token for of, token in events if of == name] == expected[name]
+
+
+def test_events_are_returned_while_requests_fail(where, monkeypatch):  # noqa: F811
+    """Two of three fail for good: the third one's tokens come out, its last ones too."""
+    model = tiny(where, seed=2)
+    prompts = {"a": [1, 2, 3], "b": [4, 5], "c": [6, 7, 8, 9]}
+    expected = texts(generate(model, prompts, gpu_pages=512, host_pages=512))
+    engine = Engine(model, cache_for(model, gpu_pages=512, host_pages=512))
+    for name, prompt in prompts.items():
+        engine.add_request(name, prompt, 12)
+    failing(model, monkeypatch, "a")
+    failing(model, monkeypatch, "c")
+    events = []
+    for _ in range(40):
+        try:
+            events += engine.step()
+        except RuntimeError:
+            pass
+    assert [token for of, token in events if of == "b"] == expected["b"]
+    assert [token for of, token in events if of != "b"] == [expected["a"][0], expected["c"][0]]
