@@ -165,15 +165,14 @@ class Engine:
 
     def _accepted(self, tree, above, choices, room):
         """The path of a verified tree that greedy decoding takes, of at most
-        `room` nodes, up to the one after which the text ends."""
-        path = [0]
-        while len(path) < room and choices[path[-1]][0] != self.eos_token_id:
-            node = path[-1]
-            node = next((t for t in range(node + 1, len(tree)) if above[t] == node and tree[t] == choices[node][0]), None)
-            if node is None:
-                break
-            path.append(node)
-        return path
+        `room` nodes, up to the one after which the text ends. Among nodes
+        that stand for the same text it is the one with the longest way on."""
+        paths = [[0]]
+        for t in range(1, len(tree)):
+            way = paths[above[t]]
+            taken = way and tree[t] == choices[above[t]][0] != self.eos_token_id and len(way) < room
+            paths.append([*way, t] if taken else None)
+        return max(filter(None, paths), key=len)
 
     def _admit(self, request):
         layers = self.model.config.num_hidden_layers

@@ -244,3 +244,54 @@ def test_events_are_returned_while_requests_fail(where, monkeypatch):  # noqa: F
             pass
     assert [token for of, token in events if of == "b"] == expected["b"]
     assert [token for of, token in events if of != "b"] == [expected["a"][0], expected["c"][0]]
+
+
+# ---- trees with the same text twice ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("first", [0, 1, 2])
+def test_candidates_that_begin_alike_are_all_followed(where, first):  # noqa: F811
+    """Several chains under one root, the right one among them: as many tokens are accepted wherever it stands."""
+    model = tiny(where, seed=2)
+    expected = texts(generate(model, PROMPTS))
+
+    def draft(r):
+        right = expected[r.request_id][len(r.generated):][:4]
+        wrong = [[*right[:1], (right[-1] + 1) % 64], [*right[:2], (right[-1] + 3) % 64, 5]]
+        chains = [*wrong[:first], right, *wrong[first:]]
+        tokens, parents = [], []
+        for c in chains:
+            for i, token in enumerate(c):
+                parents.append(len(tokens) - 1 if i else -1)
+                tokens.append(token)
+        return tokens, parents
+
+    engine = generate(model, PROMPTS, draft=draft)
+    assert texts(engine) == expected
+    for r in engine.requests.values():
+        assert r.decode_count == 3 and r.accepted_count == 8  # 11 tokens after the prompt's, in turns of up to 5
+
+
+def test_every_mix_of_equal_nodes_accepts_the_longest_way():
+    """The walk alone, against every path of random trees of few tokens."""
+    import random
+
+    rng = random.Random(0)
+    engine = Engine.__new__(Engine)
+    for _ in range(500):
+        n = rng.randrange(1, 16)
+        engine.eos_token_id = rng.choice([None, 2])
+        tree = [rng.randrange(3) for _ in range(n)]
+        above = [-1] + [rng.randrange(t) for t in range(1, n)]
+        choices = [(rng.randrange(3), None) for _ in range(n)]
+        room = rng.randrange(1, 6)
+        good = []
+        for t in range(n):
+            path = [t]
+            while above[path[0]] >= 0:
+                path.insert(0, above[path[0]])
+            steps = list(zip(path, path[1:]))
+            if len(path) <= room and all(tree[b] == choices[a][0] != engine.eos_token_id for a, b in steps):
+                good.append(path)
+        got = engine._accepted(tree, above, choices, room)
+        assert got in good and len(got) == max(map(len, good))
