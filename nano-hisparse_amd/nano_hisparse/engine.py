@@ -56,8 +56,10 @@ class Engine:
         request's decode turn then verifies the whole tree in one pass
         (Model.decode_tree) and emits every token of the path that greedy
         decoding takes, and the one after it; without a proposal (None or no
-        tokens) it is an ordinary turn. Verified turns choose pages by the
-        query of the last token alone, as ordinary ones do.
+        tokens) it is an ordinary turn. With a top_k, a verified turn selects
+        pages once, as an ordinary turn of the request's last token does; the
+        tokens accepted after it may have read other pages than turns of
+        their own would have selected.
 
         logprobs=n records a TokenInfo with the n most likely tokens for
         every generated token in its request's `logprobs`."""

@@ -21,7 +21,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .selection import Selection, quest_selection, select_pages
+from .selection import Selection, draft_selection, quest_selection, select_pages
 from .storage import upload
 
 
@@ -329,11 +329,13 @@ class Model(nn.Module):
         after the history where parents[t] is -1. Usually token 0, the only
         root, is the last one emitted and the others are drafted; at most 64.
 
-        Every node attends to the history as decode() does (per layer one
-        selection, by the first node's query, of which all nodes read the
-        same rows) and to its own ancestors. Nothing is written to the cache:
-        the returned DraftStep holds every node's logits and keys and values,
-        and its commit() appends those of an accepted path."""
+        Every node attends to its own ancestors and to the history's rows
+        that decode() would select for the first node (per layer one
+        selection, which all nodes share: with a top_k, a node below the
+        first may read other pages than it would have selected itself).
+        Nothing is written to the cache: the returned DraftStep holds every
+        node's logits and keys and values, and its commit() appends those of
+        an accepted path."""
         from . import row_kernels as rk
 
         n = len(tokens)
@@ -363,17 +365,7 @@ class Model(nn.Module):
                 q, k = _norm_rope(layer.self_attn, q, k, self.config, *tables, positions)
             else:
                 q, k, v = self._project_at(layer, x, positions)
-            request = cache.storage.requests[request_id]
-            P = cache.config.page_size
-            if selector == "quest" and top_k is not None:
-                selection = quest_selection(
-                    q[0], request.minimum[index], request.maximum[index], request.lengths[index], P, top_k
-                )
-            elif selector in ("quest", "mean"):
-                pages = select_pages(cache, request_id, index, q[0], top_k)
-                selection = Selection.from_pages(pages, request.lengths[index], P, q.shape[1])
-            else:
-                raise ValueError("selector must be quest or mean")
+            selection = draft_selection(cache, request_id, index, q[0], top_k, selector)
             attention = cache.tree_attention(q, k, v, mask, request_id, index, selection, backend)
             x = self._finish(layer, x, attention)
             drafted.append((k, v))

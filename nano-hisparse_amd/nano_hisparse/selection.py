@@ -144,7 +144,10 @@ def select_pages(cache, request_id: str, layer: int, query: torch.Tensor, top_k:
     page (the last only, for a one-page budget) are always kept. None keeps
     the whole causal history."""
     request = cache.storage.requests[request_id]
-    length = request.lengths[layer]
+    return _mean_pages(cache, query, request.summaries[layer], request.lengths[layer], top_k)
+
+
+def _mean_pages(cache, query, summaries, length, top_k):
     count = ceil(length / cache.config.page_size)
     if count == 0:
         raise ValueError("cannot attend to empty KV")
@@ -158,12 +161,44 @@ def select_pages(cache, request_id: str, layer: int, query: torch.Tensor, top_k:
     if query.device.type != "cuda":
         from .row_kernels import cpu_provider
 
-        return cpu_provider("select_pages").mean_pages(query, request.summaries[layer], length,
-                                                       cache.config.page_size, top_k)
+        return cpu_provider("select_pages").mean_pages(query, summaries, length, cache.config.page_size, top_k)
     from . import row_kernels as rk
 
-    pages, _, _ = rk.mean_batched(query[None], request.summaries[layer][None], length, cache.config.page_size, top_k)
+    pages, _, _ = rk.mean_batched(query[None], summaries[None], length, cache.config.page_size, top_k)
     return pages[0].tolist()  # a host list, as the reference returns
+
+
+def draft_selection(cache, request_id: str, layer: int, query: torch.Tensor, top_k: int | None, selector="quest"):
+    """What a token that is not in the cache yet reads of a request's
+    history: the selection that Model.decode makes for it, query [q_heads,
+    head_dim], once its key is appended, without the token itself. (The
+    reference appends every token before it selects.)
+
+    The last page, which is always kept, is then the token's own. Where the
+    history fills its last page, that is a page more, which counts among the
+    top_k and has nothing of the history in it.
+    """
+    request, P, heads = cache.storage.requests[request_id], cache.config.page_size, query.shape[0]
+    length, tables = request.lengths[layer], (request.minimum, request.maximum, request.summaries)
+    full = length // P
+    new = full * P == length  # the token opens a page, whose bounds and mean nothing reads
+    lo, hi, mean = (t[layer] if full < t.shape[1] else torch.cat((t[layer], t[layer, -1:])) for t in tables)
+    if selector == "quest" and top_k is not None:
+        chosen = quest_selection(query, lo, hi, length + new, P, top_k)
+        if not new:
+            return chosen
+        if chosen.shared_positions is not None:
+            positions = chosen.shared_positions
+            return Selection.from_device(torch.where(positions < length, positions, -1), length, P, heads, "quest")
+        pages = range(full)
+    elif selector in ("quest", "mean"):
+        pages = [p for p in _mean_pages(cache, query, mean, length + new, top_k) if p * P < length]
+    else:
+        raise ValueError("selector must be quest or mean")
+    if not pages:
+        return Selection.from_device(torch.full((1,), -1, dtype=torch.int32, device=query.device), length, P, heads,
+                                     selector)
+    return Selection.from_pages(list(pages), length, P, heads)
 
 
 def selection_oracle(query, k, v, selection):

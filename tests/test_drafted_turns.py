@@ -2,10 +2,12 @@
 are refused. The text has to be that of plain decoding."""
 
 import pytest
+import torch
 
 from nano_hisparse.engine import Engine
+from nano_hisparse.selection import draft_selection
 from nano_hisparse.storage import PageLease
-from test_tree_decode import PROMPTS, cache_for, generate, tiny, where  # noqa: F401 (where is a fixture)
+from test_tree_decode import ATOL, PROMPTS, cache_for, generate, started, tiny, where  # noqa: F401 (where is a fixture)
 
 
 def texts(engine):
@@ -295,3 +297,81 @@ def test_every_mix_of_equal_nodes_accepts_the_longest_way():
                 good.append(path)
         got = engine._accepted(tree, above, choices, room)
         assert got in good and len(got) == max(map(len, good))
+
+
+# ---- page budgets ----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("selector", ["quest", "mean"])
+@pytest.mark.parametrize("top_k", [1, 2, 3, 4, 5, 6, 9])
+@pytest.mark.parametrize("length", [1, 3, 4, 5, 8, 15, 16, 17, 18, 19, 20, 21, 24])
+def test_the_first_node_reads_the_pages_that_decoding_would(where, length, top_k, selector):  # noqa: F811
+    """On both sides of the pages' borders (4 tokens each), budgets below, at and above the pages there are."""
+    model = tiny(where, seed=6)
+    prompt = [(7 * i + 3) % 64 for i in range(length)]
+    cache, _ = started(model, prompt)
+    step = model.decode_tree([5, 9], [-1, 0], "r", cache, top_k, selector=selector)
+    logits = model.decode(5, "r", cache, top_k, selector=selector)
+    assert (step.logits[0] - logits).abs().max().item() <= ATOL
+    cache.assert_invariants()
+
+
+@pytest.mark.parametrize("selector", ["quest", "mean"])
+@pytest.mark.parametrize("length", [15, 16, 17])
+def test_a_history_that_fills_its_reservation_can_be_drafted_upon(where, length, selector):  # noqa: F811
+    """No page, and no bounds, are reserved for the tree's first token. (Up to a border, decoding's logits come from a
+    cache with room.)"""
+    model = tiny(where, seed=6)
+    prompt = [(7 * i + 3) % 64 for i in range(length)]
+    for top_k in (1, 2, 3, 4, 5, 6):
+        full, _ = started(model, prompt, room=0)
+        roomy, _ = started(model, prompt)
+        step = model.decode_tree([5], [-1], "r", full, top_k, selector=selector)
+        logits = model.decode(5, "r", roomy, top_k, selector=selector)
+        assert (step.logits[0] - logits).abs().max().item() <= ATOL
+        with pytest.raises(ValueError, match="reserved tokens"):
+            step.commit([0])
+
+
+@pytest.mark.parametrize("selector", ["quest", "mean"])
+@pytest.mark.parametrize("top_k", [1, 2, 3])
+def test_drafts_that_are_never_accepted_change_no_token(where, top_k, selector):  # noqa: F811
+    model = tiny(where, seed=2)
+    for start in range(4):
+        prompts = {"a": [(5 * i + 1 + start) % 64 for i in range(17 + start)]}
+
+        def engine(draft):
+            e = Engine(model, cache_for(model), top_k=top_k, draft=draft, selector=selector)
+            for name, prompt in prompts.items():
+                e.add_request(name, prompt, 14)
+            e.run()
+            return e
+
+        expected = texts(engine(None))
+
+        def wrong(r):
+            following = expected[r.request_id][len(r.generated)]
+            return [(following + 1) % 64, 5, (following + 2) % 64], [-1, 0, -1]
+
+        drafted = engine(wrong)
+        assert texts(drafted) == expected
+        assert all(r.accepted_count == 0 and r.decode_count == 13 for r in drafted.requests.values())
+
+
+def test_selections_for_a_token_that_is_not_there_yet(where):  # noqa: F811
+    """Positions: those of the history in the pages that are kept, the token's own page among them while it is empty."""
+    model = tiny(where, seed=6)
+    q = torch.randn(4, 8, device=where)
+    for length in (15, 16):
+        cache, _ = started(model, list(range(length)))
+        for selector in ("quest", "mean"):
+            for top_k in (1, 2, 3, 4, 5, 6, None):
+                s = draft_selection(cache, "r", 0, q, top_k, selector)
+                assert s.length == length and s.heads == 4 and s.page_size == 4
+                kept = 4 if top_k is None else min(top_k - (length == 16), 4)
+                assert len(s.pages) == kept and len(s.positions[0]) == 4 * kept - (kept > 0 and length == 15)
+                assert not kept or top_k == 1 or s.pages[0] == 0
+                assert length == 16 or s.pages[-1] == 3
+        for bad in (dict(top_k=0), dict(top_k=2, selector="best")):
+            with pytest.raises(ValueError):
+                draft_selection(cache, "r", 0, q, **bad)
