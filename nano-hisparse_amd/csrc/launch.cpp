@@ -20,8 +20,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <new>
 #include <stdexcept>
+#include <utility>
 #include <vector>
 
 #include "nhs.h"
@@ -374,7 +376,15 @@ struct OnDevice {
 void check_out(const Tensor& out, const Tensor& like) {
   on_gpu(out, like.dim(), like);
   need(same_sizes(out, like.sizes()) && out.scalar_type() == like.scalar_type() && out.stride(-1) == 1);
-  for (int64_t d = 0; d < out.dim(); ++d) need(out.stride(d) != 0 || out.size(d) == 1);
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t d = 0; d < out.dim(); ++d)
+    if (out.size(d) > 1) dims.emplace_back(out.stride(d), out.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;  // elements that the dimensions of smaller strides reach over
+  for (const auto& [stride, size] : dims) {
+    need(stride >= span);
+    span += stride * (size - 1);
+  }
 }
 
 // Scratch memory of a call (nothing for 0 bytes): on the current stream's allocator, freed with the tensor.
@@ -487,6 +497,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       k_out = tensor(PyTuple_GET_ITEM(a[8], 1));
       check_out(q_out, q);
       check_out(k_out, k);
+      need(q_out.data_ptr() != k_out.data_ptr());
     }
     int st;
     {

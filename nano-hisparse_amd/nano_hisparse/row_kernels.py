@@ -108,8 +108,15 @@ def _check_out(who, out, shape, dtype, device):
     contiguous, no element twice."""
     if out.shape != shape or out.dtype != dtype or out.device != device:
         raise ValueError(f"{who}: out must be {list(shape)} {dtype} on {device}")
-    if out.numel() and (out.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape))):
-        raise ValueError(f"{who}: out's head dims must be contiguous and its elements distinct")
+    if not out.numel():
+        return
+    span = 1  # elements that the dimensions of smaller strides reach over
+    for s, n in sorted((s, n) for s, n in zip(out.stride(), out.shape) if n > 1):
+        if s < span:
+            raise ValueError(f"{who}: out's elements must be distinct")
+        span += s * (n - 1)
+    if out.stride(-1) != 1:
+        raise ValueError(f"{who}: out's head dims must be contiguous")
 
 
 def _check_counts(who, *counts):
@@ -987,7 +994,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps, cos, sin, positions=None, out=No
     k_weight [D]) and their rotary embedding, one pass, fp32 with one
     rounding. cos/sin [rows, D/2] in q's dtype or float32; row r's position
     is positions[r] (int64 [n], clamped to the tables) or r. Returns new
-    (q, k), or writes to `out`, a pair that may be (q, k) itself."""
+    (q, k), or writes to `out`, a pair that may be (q, k) itself and overlaps
+    nothing else."""
     if q.is_cuda:
         done = (_launch or _load_launch()).qk_norm_rope(q, k, q_weight, k_weight, float(eps), cos, sin, positions, out)
         if done is not None:
@@ -1019,6 +1027,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps, cos, sin, positions=None, out=No
             raise ValueError("qk_norm_rope: out is a pair (q, k)")
         for t, o in zip((q, k), outs):
             _check_out("qk_norm_rope", o, t.shape, t.dtype, device)
+        if n and outs[0].data_ptr() == outs[1].data_ptr():
+            raise ValueError("qk_norm_rope: out's elements must be distinct")
     if n == 0:
         return outs
     if positions is not None:
