@@ -365,8 +365,8 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(NormRopeArgs
 // and its sum of squares never leave them; a wave takes U x 64 / LANES heads
 // of one row, whose cos/sin chunks it loads once, and asks for every head
 // before it computes the first. Bound by memory (each element moves once):
-// 16001 rows of 32 + 8 heads of 128 in bf16, 332 MB, 62 us (5.3 TB/s, the
-// rate of a large copy); an element per lane took 216.
+// 16001 rows of 32 + 8 heads of 128 in bf16, 332 MB, 62 us (5.3 TB/s, where
+// a large copy moves 4.85); an element per lane took 216.
 template <typename T, typename TT, int LANES, int U>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_vec_kernel(NormRopeArgs a, FastDiv parts) {
   constexpr int GROUPS = kWave / LANES;

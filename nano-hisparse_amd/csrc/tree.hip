@@ -263,13 +263,16 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 // in the loop (the four shares are joined in two steps: one share after the
 // other took 8.0 us where two steps take 7.5, one request of 128 rows).
 //
-// Measured (MI355X, bf16, rows read from HBM, us with the join of the splits):
-// 8 requests x 16 nodes x 32/8 heads of 128 x 2048 rows 30 (23 without the
-// join; the rows stream at 5.5 TB/s once they flow, but 6 us pass before the
-// first are in, and 2.5 at the end); one request x 32 nodes x 32768 rows 50 (39);
-// 16 requests x 64 nodes x 28/4 heads x 4096 rows 102 (595 TFLOP/s): bound by
-// the matrix cores, LDS reads and softmax in about equal parts (85 without the
-// loads, 65 with them alone). With the general kernel 932, 3685 and 10818.
+// Measured (MI355X, bf16, rows read from HBM, graphs replayed for a second, us
+// with the join of the splits): 8 requests x 16 nodes x 32/8 heads of 128 x
+// 2048 rows 28.8 (the rows stream at 5.5 TB/s once they flow, but 6 us pass
+// before the first are in, and 2.5 at the end; the join is 5); one request x
+// 32 nodes x 32768 rows 46.6 (join 6.7); 16 requests x 64 nodes x 28/4 heads x
+// 4096 rows 93 (652 TFLOP/s): bound by the matrix cores, LDS reads and softmax
+// in about equal parts. The pairs of figures in this file compare variants in
+// short runs after an idle card, which take 5 to 14% longer (30.6, 51.9 and
+// 108 here; of the 102 measured then, 85 were left without the loads and 65
+// with the loads alone). With the general kernel 932, 3685 and 10818.
 //
 // fp32 runs on v_mfma_f32_32x32x2_f32 (lane l: row l%32 of A at k = l/32). The
 // dims of a dot product may come in any order, so four of them take the
@@ -778,7 +781,8 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
     // last one may have nothing else. us with splits of equal numbers of keys, the draft on top / so: 16 nodes x 512
     // keys 14.3 / 12.5, 4 requests of them 16.6 / 14.4, x 960 keys 19.2 / 16.6, fp32 heads of 32 x 448 keys 13.2 / 9.9.
     // Splitting pays where it saves more than the join costs, which is about 2.3 us and the partial sums at 5.5 TB/s; a
-    // round takes 1.6 us. us whole / split: 256 keys, 8 requests of 16 nodes 14.5 / 17.8, one request 13.3 / 12.3.
+    // round takes 1.6 us (16-bit heads of up to 128 and fp32 heads of 32; the products of a round of fp32 heads of 128
+    // alone take about 6.8 us, and rounds of 512-byte rows are half as long, so for those the rule is only a guess). us whole / split: 256 keys, 8 requests of 16 nodes 14.5 / 17.8, one request 13.3 / 12.3.
     const int rounds = (n_rows + least - 1) / least, total = rounds + 1;
     const int longest = (int)((total + wanted - 1) / wanted), splits = (total + longest - 1) / longest;
     const double joined = longest * 1.6 + 2.3 + (double)splits * batch * nodes * q_heads * head_dim * 8 / 5.5e6;
