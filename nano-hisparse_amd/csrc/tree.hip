@@ -223,6 +223,15 @@ __device__ __forceinline__ int tf_v_slot(int r, int c) {
   return C >= 16 ? c ^ (4 * (r & 3)) : C == 8 ? c ^ (4 * ((r >> 1) & 1)) : c;
 }
 
+// a packed pair as fp32
+template <typename T>
+__device__ __forceinline__ float2 tf_unpack(uint32_t pair) {
+  if constexpr (T::dtype == NHS_BF16)
+    return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u));
+  else
+    return make_float2(f16_bits_to_f32(pair & 0xffffu), f16_bits_to_f32(pair >> 16));
+}
+
 // 16 bytes of K and Q each: one 32x32x16 product of 16-bit elements, or four 32x32x2 of fp32
 template <typename T>
 __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
@@ -252,12 +261,13 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 // and NaN and infinities of drafted values are taken out of it, then added to
 // the outputs of the nodes that see them.
 //
-// 16-bit weights are rounded to the type for the P.V product and the
-// denominator sums the same rounded weights, as in the prompt attention: the
-// output's error against float64 is 0.0022 of it in bf16, 0.0017 of which is
-// its own rounding. (A second product with the rounded rests, which leaves
-// that rounding alone, costs 5% at 8 requests x 2048 rows and 18% for the
-// widest trees.) fp32 weights are not rounded.
+// 16-bit weights go to the matrix cores as the nearest value of the type and,
+// in a second product against the same V, the rest of that rounding; the
+// denominator sums them as they are. The output is the exact one rounded once
+// (error against float64 0.0017 in bf16; with the rounded weights alone, which
+// the prompt attention takes, 0.0022). us without / with the rests: one request
+// x 16 nodes x 2048 rows 15.5 / 15.8, eight of them 28.8 / 30.0, the long
+// history and the widest trees below 44.0 / 48.7 and 89.7 / 108.5.
 //
 // With QW = 1 a wave loads and reads its own tiles only and no barrier stands
 // in the loop (the four shares are joined in two steps: one share after the
@@ -265,14 +275,15 @@ __device__ __forceinline__ pf_f32x16 tf_qk(uint4 k, uint4 q, pf_f32x16 c) {
 //
 // Measured (MI355X, bf16, rows read from HBM, graphs replayed for a second, us
 // with the join of the splits): 8 requests x 16 nodes x 32/8 heads of 128 x
-// 2048 rows 28.8 (the rows stream at 5.5 TB/s once they flow, but 6 us pass
+// 2048 rows 30.0 (the rows stream at 5.5 TB/s once they flow, but 6 us pass
 // before the first are in, and 2.5 at the end; the join is 5); one request x
-// 32 nodes x 32768 rows 46.6 (join 6.7); 16 requests x 64 nodes x 28/4 heads x
-// 4096 rows 93 (652 TFLOP/s): bound by the matrix cores, LDS reads and softmax
-// in about equal parts. The pairs of figures in this file compare variants in
-// short runs after an idle card, which take 5 to 14% longer (30.6, 51.9 and
-// 108 here; of the 102 measured then, 85 were left without the loads and 65
-// with the loads alone). With the general kernel 932, 3685 and 10818.
+// 32 nodes x 32768 rows 48.7 (join 6.7); 16 requests x 64 nodes x 28/4 heads x
+// 4096 rows 108.5 (559 TFLOP/s, 838 with the rests' products): bound by the
+// matrix cores, LDS reads and softmax together, which follow each other in a
+// wave. With the general kernel 932, 3685 and 10818. Other figures of this file
+// compare variants without the rests, in short runs after an idle card, which
+// take 5 to 14% longer (the widest trees 102, 85 of them without the loads, 65
+// with the loads alone).
 //
 // fp32 runs on v_mfma_f32_32x32x2_f32 (lane l: row l%32 of A at k = l/32). The
 // dims of a dot product may come in any order, so four of them take the
@@ -288,6 +299,9 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
   constexpr int kTile = BN * RB;               // bytes
   constexpr int kRound = BN * KW;              // keys
+  // fp16 weights, denominators and sums are all 2^10 times too large, so that a weight of 2^-34 of the largest is still a
+  // number (the largest is below 2^11; where ref is below `large`, ref - 10 is exact)
+  constexpr float kLift = T::dtype == NHS_F16 ? 10.f : 0.f;
   // exponent bits of NaN and infinities
   constexpr uint32_t kOdd = F ? 0x7f800000u : T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;
   static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1 && RB <= kTfRowBytes, "tile shape");
@@ -405,8 +419,8 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     }
     float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
     // Scores are scaled and made relative to the maximum in one step, which is off by the rounding of ref. Where that
-    // could exceed a power or two of 2 (and overflow the weights), they are made relative first.
-    const bool large = fabsf(ref) > 0x1p26f;
+    // could exceed half a power of 2 (and overflow the weights in the end), they are made relative first.
+    const bool large = fabsf(ref) > 0x1p24f;
     if (__any(large)) {
 #pragma unroll
       for (int x = 0; x < NB; ++x)
@@ -414,6 +428,7 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
         for (int i = 0; i < 16; ++i) s[x][i] -= large ? m : 0.f;
       ref = large ? 0.f : ref;
     }
+    ref -= kLift;
     float tile_sum = 0.f;
     if constexpr (F) {
 #pragma unroll
@@ -434,28 +449,33 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
             o[y] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[x][i], o[y], 0, 0, 0);
           }
     } else {
-      uint4 pb[2 * NB];
 #pragma unroll
-      for (int j = 0; j < 2 * NB; ++j) {
-        uint32_t w[4];
+      for (int j = 0; j < 2 * NB; ++j) {  // 16 keys
+        uint32_t w[4], r[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float e0 = s[j >> 1][(j & 1) * 8 + 2 * x], e1 = s[j >> 1][(j & 1) * 8 + 2 * x + 1];
-          w[x] = pf_pack<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(e0, a.scale_log2, -ref)),
-                            __builtin_amdgcn_exp2f(__builtin_fmaf(e1, a.scale_log2, -ref)));
-          tile_sum = pf_add_pair<T>(w[x], tile_sum);
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(e0, a.scale_log2, -ref));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(e1, a.scale_log2, -ref));
+          w[x] = pf_pack<T>(p0, p1);
+          const float2 rounded = tf_unpack<T>(w[x]);
+          r[x] = pf_pack<T>(p0 - rounded.x, p1 - rounded.y);
+          tile_sum += p0 + p1;
         }
-        pb[j] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      l += tile_sum;
-#pragma unroll
-      for (int j = 0; j < 2 * NB; ++j)
+        const uint4 pb = make_uint4(w[0], w[1], w[2], w[3]), rest = make_uint4(r[0], r[1], r[2], r[3]);
+        uint4 vf[DB];
 #pragma unroll
         for (int x = 0; x < DB; ++x) {
           const uint2 lo = pf_read_tr(vl + v_at[x] + (16 * j) * RB);
           const uint2 hi = pf_read_tr(vl + v_at[x] + (16 * j + 8) * RB);
-          o[x] = mfma32x32x16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[j], o[x]);
+          vf[x] = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
+#pragma unroll
+        for (int x = 0; x < DB; ++x) o[x] = mfma32x32x16<T>(vf[x], pb, o[x]);
+#pragma unroll
+        for (int x = 0; x < DB; ++x) o[x] = mfma32x32x16<T>(vf[x], rest, o[x]);
+      }
+      l += tile_sum;
     }
   };
 
@@ -762,7 +782,7 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
     s.shares = s.waves == 1 ? 4 : 2;
     // Blocks of 256 rows where they fill the chip without splits (half the reads of the keys from L2; with splits their
     // joining costs more than that). us with blocks of 128 / 256: 32 requests x 448 rows x 4 KV heads (256 of 256) x
-    // 2048 keys 118.5 / 98.5, 16 of them (128) x 4096 keys 105 / 116.
+    // 2048 keys 118.5 / 98.5 (long runs with the rests 130 / 110), 16 of them (128) x 4096 keys 105 / 116.
     if (query_rows > 128 && head_dim == 128 && row_bytes == 256 &&
         (int64_t)batch * kv_heads * ((query_rows + 255) / 256) >= 256)
       s.waves = 8, s.shares = 1;
@@ -782,7 +802,8 @@ static TreeShape tree_shape(int batch, int nodes, int n_rows, int q_heads, int k
     // keys 14.3 / 12.5, 4 requests of them 16.6 / 14.4, x 960 keys 19.2 / 16.6, fp32 heads of 32 x 448 keys 13.2 / 9.9.
     // Splitting pays where it saves more than the join costs, which is about 2.3 us and the partial sums at 5.5 TB/s; a
     // round takes 1.6 us (16-bit heads of up to 128 and fp32 heads of 32; the products of a round of fp32 heads of 128
-    // alone take about 6.8 us, and rounds of 512-byte rows are half as long, so for those the rule is only a guess). us whole / split: 256 keys, 8 requests of 16 nodes 14.5 / 17.8, one request 13.3 / 12.3.
+    // alone take about 6.8 us, and rounds of 512-byte rows are half as long, so for those the rule is only a guess). us
+    // whole / split: 256 keys, 8 requests of 16 nodes 14.5 / 17.8, one request 13.3 / 12.3.
     const int rounds = (n_rows + least - 1) / least, total = rounds + 1;
     const int longest = (int)((total + wanted - 1) / wanted), splits = (total + longest - 1) / longest;
     const double joined = longest * 1.6 + 2.3 + (double)splits * batch * nodes * q_heads * head_dim * 8 / 5.5e6;

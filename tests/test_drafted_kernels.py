@@ -148,6 +148,36 @@ def test_tree_attention_of_splits_of_several_stages(gpu, dtype, D, T, g):
     check_requests(c, run_tree(c), (0, 1, 2, 3, 4, B - 1))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D,T,g", [(bf16, 128, 8, 4), (f16, 64, 7, 4), (bf16, 32, 30, 2), (f16, 128, 33, 7),
+                                         (bf16, 256, 5, 2), (f16, 64, 64, 4), (bf16, 128, 20, 4)])
+def test_weights_of_sixteen_bit_heads_keep_their_rests(gpu, dtype, D, T, g):
+    """Outputs are the exact ones, rounded once. The exact values' neighbours
+    would be taken for a third of them if the weights were rounded to the type
+    (each off by up to 2^-9 relative in bf16 and independent of the others, so
+    an output by about as much, where its steps are 2^-8 to 2^-7 of it; fp16
+    likewise); with the rests of that rounding, rounded themselves, an output
+    is off by some 2^-17 (2^-20 in fp16, whose scores and sums are what is
+    left), which takes the neighbour for less than one in a hundred."""
+    print("case:", dict(dtype=dtype, D=D, T=T, g=g), flush=True)
+    B, Hkv, N, P = 4, 4, 1500, 16
+    c = tree_case(gpu, dtype, B, T, g * Hkv, Hkv, D, P, N, seed=D + T, spread=0.5)
+    got = run_tree(c)
+    differ = total = 0
+    for b in range(B):
+        at = c["rows"][b][c["rows"][b] >= 0]
+        for t in range(T):
+            word = int(c["mask"][b, t])
+            nodes = [j for j in range(T) if word >> j & 1]
+            keys, values = (torch.cat((c["pool"][at // P, i, at % P], c[n][b, nodes])).double().repeat_interleave(g, 1)
+                            for i, n in ((0, "k"), (1, "v")))
+            w = ((c["q"][b, t].double() * keys).sum(-1) / math.sqrt(D)).softmax(0)
+            exact = (w[..., None] * values).sum(0) if word else torch.zeros_like(got[b, t])
+            differ += (got[b, t] != exact.to(dtype)).sum().item()
+            total += exact.numel()
+    assert differ <= 0.02 * total, f"{differ} of {total}"
+
+
 # ---- long prompts --------------------------------------------------------------------------------
 
 
