@@ -299,9 +299,9 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
   constexpr int kMine = BN / kRows / QW;       // instructions of a wave per tile, for K and for V each
   constexpr int kTile = BN * RB;               // bytes
   constexpr int kRound = BN * KW;              // keys
-  // fp16 weights, denominators and sums are all 2^10 times too large, so that a weight of 2^-34 of the largest is still a
-  // number (the largest is below 2^11; where ref is below `large`, ref - 10 is exact)
-  constexpr float kLift = T::dtype == NHS_F16 ? 10.f : 0.f;
+  // fp16 weights, denominators and sums are all 2^15 times too large: what both products leave of a weight is then
+  // 2^-40 of the largest at most (which itself is below 2^15.2 and fp16's numbers end at 2^16, see `large`)
+  constexpr float kLift = T::dtype == NHS_F16 ? 15.f : 0.f;
   // exponent bits of NaN and infinities
   constexpr uint32_t kOdd = F ? 0x7f800000u : T::dtype == NHS_BF16 ? 0x7f80u : 0x7c00u;
   static_assert(kRound >= kTreeNodes && kTfStage % kRound == 0 && kMine >= 1 && RB <= kTfRowBytes, "tile shape");
@@ -419,8 +419,8 @@ __global__ __launch_bounds__(QW * KW * kWave) void tree_flash_kernel(TreeArgs a)
     }
     float ref = m == -INFINITY ? 0.f : m * a.scale_log2;
     // Scores are scaled and made relative to the maximum in one step, which is off by the rounding of ref. Where that
-    // could exceed half a power of 2 (and overflow the weights in the end), they are made relative first.
-    const bool large = fabsf(ref) > 0x1p24f;
+    // could exceed a thirtieth of a power of 2 (and overflow the weights in the end), they are made relative first.
+    const bool large = fabsf(ref) > 0x1p20f;
     if (__any(large)) {
 #pragma unroll
       for (int x = 0; x < NB; ++x)

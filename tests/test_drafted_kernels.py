@@ -11,7 +11,7 @@ import torch
 from nano_hisparse import _hip
 from nano_hisparse import row_kernels as rk
 from test_drafted_tokens import (HALF, U, bf16, check, check_norm, check_tree, f16, f32, norm_case, plan_oracle,
-                                 random_parents, run_tree, seen_nodes, tree_case)
+                                 random_parents, run_tree, seen_nodes, tree_case, tree_oracle)
 
 
 @pytest.mark.gpu
@@ -176,6 +176,33 @@ def test_weights_of_sixteen_bit_heads_keep_their_rests(gpu, dtype, D, T, g):
             differ += (got[b, t] != exact.to(dtype)).sum().item()
             total += exact.numel()
     assert differ <= 0.02 * total, f"{differ} of {total}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(f16, 32), (f16, 64), (f16, 128), (f16, 256), (bf16, 128), (f32, 64), (f16, 48)])
+@pytest.mark.parametrize("power", [18, 21])
+@pytest.mark.parametrize("B,N", [(1, 8000), (40, 1200)])
+def test_many_small_weights_add_up(gpu, dtype, D, power, B, N):
+    """One key with all but a little of the weight, thousands with exp(-18) or
+    exp(-21) of it each (below fp16's numbers) and the only values that are not
+    0. fp16 weights are multiples of 2^-39 of the largest, half of which per key
+    comes to the tolerance."""
+    print("case:", dict(dtype=dtype, D=D, power=power, B=B, N=N), flush=True)
+    c = tree_case(gpu, dtype, B, 2, 4, 2, D, 16, N, seed=D, fused=False)
+    for x in (c["q"], c["k"], c["pool"]):
+        x.zero_()
+    c["q"][..., 0] = 8.0
+    c["k"][:, 0, :, 0] = round(power * math.sqrt(D)) / 8
+    c["v"].zero_()
+    c["pool"][:, 1] = 1024.0
+    c["pool"][:, 1, :, :, 1::2] = -512.0
+    c["mask"].copy_(torch.tensor([[1, 3]], device=gpu).expand(B, 2))
+    some = dict(c, **{n: c[n][-1:] for n in ("q", "rows", "k", "v", "mask")})
+    expected, tol = tree_oracle(*(some[n] for n in ("q", "pool", "rows", "k", "v", "mask", "page")), False)
+    assert expected.abs().min() > 2.0 ** -13  # (a number in every type)
+    if dtype == f16:
+        tol += 2.0 ** -40 * N * 1024.0
+    check(run_tree(c)[-1:], expected, tol)
 
 
 # ---- long prompts --------------------------------------------------------------------------------
