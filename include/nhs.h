@@ -539,6 +539,84 @@ int nhs_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, in
 int nhs_expand_columns(const int64_t* shared_rows, int64_t n, const int64_t* columns,
                        int64_t heads, int64_t width, int64_t* out, void* stream);
 
+/*
+ * A KV cache held in 8 bits. A row is, in each of its two planes, kv_heads x
+ * head_dim codes of one type, then (at the next multiple of 4 bytes) an fp32
+ * scale for every KV head, padded to a multiple of 16 bytes:
+ *   pool  [blocks, 2, page_size, nhs_row8_bytes]     K plane 0, V plane 1
+ *   host  [host_pages, 2, page_size, nhs_row8_bytes] (pinned, contiguous)
+ * so nhs_gather_rows moves such rows with plane_bytes = nhs_row8_bytes. Of the
+ * head_dim elements x of one token, plane and KV head, with Q = 127 (int8) or
+ * 448 (e4m3fn):
+ *   scale = max(fp32(max|x| / Q), 2^-80)
+ *   code  = the type's value nearest to the exact quotient x / scale, ties to even
+ *   value = fp32(code * scale)
+ * Where an element is not finite, the scale is NaN and the codes are 0: the
+ * whole slice reads as NaN. Pools and hosts are 16-byte aligned, and
+ * pool_block_stride (bytes; 0: contiguous blocks) is a multiple of 16.
+ * head_dim <= NHS_MAX_HEAD_DIM8. No counterpart in the reference, whose cache
+ * holds the model's type (nano_hisparse/config.py:8-30).
+ */
+enum { NHS_CODE_I8 = 0, NHS_CODE_E4M3 = 1 };
+#define NHS_MAX_HEAD_DIM8 1024
+
+/* Bytes of a plane's row. */
+int64_t nhs_row8_bytes(int32_t kv_heads, int32_t head_dim);
+
+/*
+ * nhs_append_page into rows in 8 bits: the new rows of k and v (kv_dtype,
+ * kv_heads * head_dim elements, token_stride elements apart) are quantised
+ * into pool block `block` and, with a host_alias, host block `host_page`, the
+ * same bytes in both. minimum and maximum [kv_heads, head_dim] (kv_dtype) fold
+ * in the keys as given (NaN propagates); summary (fp32) becomes the mean of
+ * code * scale over the page's keys, earlier ones included, summed in 64 bits
+ * and rounded once. The pad bytes of a row are not written.
+ */
+int nhs_append_page8(const void* k, const void* v, int64_t token_stride, int32_t kv_dtype, int32_t code,
+                     int32_t kv_heads, int32_t head_dim, int32_t page_size, void* pool,
+                     int64_t pool_block_stride, int64_t block, int32_t within, int32_t count,
+                     void* host_alias, int64_t host_page, float* summary, void* minimum, void* maximum,
+                     void* stream);
+
+/*
+ * nhs_append_items into rows in 8 bits: one token per item, results as
+ * nhs_append_page8's. An item whose page is beyond its tables or not bound
+ * (resident < 0) is left alone; one without a host page gets no mirror.
+ */
+int nhs_append_items8(int32_t batch, const void* k, const void* v, int64_t token_stride, int32_t kv_dtype,
+                      int32_t code, int32_t kv_heads, int32_t head_dim, int32_t page_size, void* pool,
+                      int64_t pool_block_stride, void* host_alias, const nhs_layer_item* items,
+                      const int64_t* lengths, void* stream);
+
+/*
+ * Reads rows back: k_out[i] and v_out[i] (kv_heads * head_dim elements of
+ * out_dtype, k_stride and v_stride elements apart) are the values of pool row
+ * rows[i * rows_stride], i < n, rounded to out_dtype; zeros for a row outside
+ * [0, pool_rows).
+ */
+int nhs_read_rows8(const void* pool, int64_t pool_rows, int64_t pool_block_stride, int32_t code,
+                   int32_t kv_heads, int32_t head_dim, int32_t page_size, const int64_t* rows,
+                   int64_t rows_stride, int64_t n, int32_t out_dtype, void* k_out, int64_t k_stride,
+                   void* v_out, int64_t v_stride, void* stream);
+
+/*
+ * nhs_attend_rows over rows in 8 bits: out[b,h] = softmax_r(q[b,h] . K[r] *
+ * head_dim^-0.5) . V[r] over the rows rows[b, h, c] in [0, pool_rows); zeros
+ * for a head without any. Scores and sums are fp32; query and out have
+ * q_dtype. The workspace (16-byte aligned; may be NULL where 0 bytes are
+ * needed) holds anything before and after a call; calls that may overlap need
+ * different ones.
+ */
+int64_t nhs_attend_rows8_workspace_bytes(int32_t batch, int32_t n_rows, int32_t q_heads, int32_t kv_heads,
+                                         int32_t head_dim);
+int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_batch_stride, int64_t q_head_stride,
+                     const void* pool, int64_t pool_rows, int64_t pool_block_stride, int32_t code,
+                     const int64_t* rows, int64_t rows_batch_stride, int64_t rows_head_stride,
+                     int64_t rows_col_stride, int32_t batch, int32_t n_rows, int32_t q_heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t page_size, void* out,
+                     int64_t out_batch_stride, int64_t out_head_stride, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

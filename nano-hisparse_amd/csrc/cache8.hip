@@ -1,0 +1,378 @@
+// A KV cache held in 8 bits (rows8.h): K and V rows quantised as they are
+// appended to a pool page and its host mirror, with the page's key bounds and
+// mean (nhs_append_page8, nhs_append_items8), and pool rows read back in a
+// model's type (nhs_read_rows8).
+#include <math.h>
+
+#include <type_traits>
+
+#include "rows8.h"
+
+namespace nhs {
+
+constexpr int kA8Threads = 256;
+constexpr int kA8Waves = kA8Threads / kWave;
+constexpr int kA8Held = 16;     // new rows whose codes are in LDS at a time
+constexpr int kA8Batch = 16;    // earlier rows loaded together for the page's mean
+constexpr int kA8MaxDim = NHS_MAX_HEAD_DIM8;
+
+struct Append8Args {
+  const char* k;
+  const char* v;
+  int64_t token_stride;  // elements between consecutive tokens of k and v
+  Row8 form;
+  int page_size;
+  char* pool_block;  // the page's pool block [2, page_size, form.bytes]
+  char* host_block;  // its host block, or null
+  int within, count;
+  float* summary;
+  void* minimum;
+  void* maximum;
+};
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d));
+  return x;
+}
+
+// torch.minimum and torch.maximum: a NaN stays
+__device__ __forceinline__ float least(float a, float b) { return (a != a || b != b) ? a + b : fminf(a, b); }
+__device__ __forceinline__ float most(float a, float b) { return (a != a || b != b) ? a + b : fmaxf(a, b); }
+
+// One plane of one KV head of a page: a wave quantises a row at a time (lane
+// l its elements l, l + 64, ...; N of them at most), and for the keys a thread
+// per element folds the bounds of the keys as they were given and sums what
+// the page holds of them, in 64 bits and in row order, for the mean.
+template <typename T, typename C, int N>
+__device__ __forceinline__ void append8_head(const Append8Args& a, int plane, int head) {
+  constexpr int kCols = (N * kWave + kA8Threads - 1) / kA8Threads;  // elements per folding thread
+  __shared__ uint8_t held[kA8Held][N * kWave];
+  __shared__ float scales[kA8Held];
+  const int D = a.form.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t slice = (int64_t)head * D;                       // of a row: elements and codes
+  const int64_t at_scale = a.form.scales_at + 4 * (int64_t)head;
+  const int64_t plane_at = (int64_t)plane * a.page_size * a.form.bytes;
+  const char* src = plane ? a.v : a.k;
+  double sum[kCols];
+  float lo[kCols], hi[kCols];
+  if (plane == 0) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int e = min(tid + c * kA8Threads, D - 1);
+      lo[c] = load_elem(a.minimum, T::dtype, slice + e);
+      hi[c] = load_elem(a.maximum, T::dtype, slice + e);
+      sum[c] = 0.0;
+      // unconditional loads (rows past the earlier ones re-read the last of them), masked sums
+      for (int r0 = 0; r0 < a.within; r0 += kA8Batch) {
+        float code[kA8Batch], scale[kA8Batch];
+#pragma unroll
+        for (int j = 0; j < kA8Batch; ++j) {
+          const char* row = a.pool_block + (int64_t)min(r0 + j, a.within - 1) * a.form.bytes;
+          code[j] = decode8<C>(static_cast<uint8_t>(row[slice + e]));
+          scale[j] = *reinterpret_cast<const float*>(row + at_scale);
+        }
+#pragma unroll
+        for (int j = 0; j < kA8Batch; ++j)
+          if (r0 + j < a.within) sum[c] += (double)code[j] * (double)scale[j];
+      }
+    }
+  }
+  for (int t0 = 0; t0 < a.count; t0 += kA8Held) {
+    const int n = min(kA8Held, a.count - t0);
+    for (int t = wave; t < n; t += kA8Waves) {
+      float x[N];
+      uint32_t largest = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = lane + i * kWave;
+        x[i] = e < D ? load_elem(src, T::dtype, (int64_t)(t0 + t) * a.token_stride + slice + e) : 0.f;
+        largest = max(largest, __float_as_uint(x[i]) & 0x7fffffffu);
+      }
+      const float scale = scale8<C>(wave_max(largest)), inv = __fdiv_rn(1.f, scale);
+      const int64_t row = plane_at + (int64_t)(a.within + t0 + t) * a.form.bytes;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = lane + i * kWave;
+        if (e >= D) break;
+        const float four[4] = {x[i], 0.f, 0.f, 0.f};
+        const uint8_t code = (uint8_t)codes8<C>(four, scale, inv);
+        a.pool_block[row + slice + e] = (char)code;
+        if (a.host_block) a.host_block[row + slice + e] = (char)code;
+        held[t][e] = code;
+      }
+      if (lane == 0) {
+        *reinterpret_cast<float*>(a.pool_block + row + at_scale) = scale;
+        if (a.host_block) *reinterpret_cast<float*>(a.host_block + row + at_scale) = scale;
+        scales[t] = scale;
+      }
+    }
+    if (plane) continue;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int e = min(tid + c * kA8Threads, D - 1);
+      for (int t = 0; t < n; ++t) {
+        const float key = load_elem(a.k, T::dtype, (int64_t)(t0 + t) * a.token_stride + slice + e);
+        lo[c] = least(lo[c], key);
+        hi[c] = most(hi[c], key);
+        sum[c] += (double)decode8<C>(held[t][e]) * (double)scales[t];
+      }
+    }
+    __syncthreads();  // the next rows overwrite the held ones
+  }
+  if (plane) return;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    const int e = tid + c * kA8Threads;
+    if (e >= D) break;
+    store_elem(a.minimum, T::dtype, slice + e, lo[c]);
+    store_elem(a.maximum, T::dtype, slice + e, hi[c]);
+    a.summary[slice + e] = (float)(sum[c] / (double)(a.within + a.count));
+  }
+}
+
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kA8Threads) void append8_page_kernel(Append8Args a) {
+  const int plane = (int)blockIdx.x >= a.form.kv_heads;
+  append8_head<T, C, N>(a, plane, (int)blockIdx.x - plane * a.form.kv_heads);
+}
+
+struct Append8ItemsArgs {
+  Append8Args a;  // k, v, token_stride, form and page_size; pool_block and host_block are the whole pool and host
+  int64_t pool_block_bytes;
+  const nhs_layer_item* items;
+  const int64_t* lengths;
+};
+
+// Item blockIdx.y appends its one token: its page and row follow from its
+// length and its page tables. An item whose page is not bound is left alone.
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kA8Threads) void append8_items_kernel(Append8ItemsArgs g) {
+  const int b = blockIdx.y;
+  const nhs_layer_item& item = g.items[b];
+  Append8Args a = g.a;
+  const int64_t length = g.lengths[b], page = length / a.page_size;
+  if (length < 0 || page >= item.n_pages) return;
+  const int block = item.resident[page], host_page = item.source[page];
+  if (block < 0) return;
+  const int64_t row_elems = (int64_t)a.form.kv_heads * a.form.head_dim;
+  a.k += (int64_t)b * a.token_stride * T::bytes;
+  a.v += (int64_t)b * a.token_stride * T::bytes;
+  a.pool_block += block * g.pool_block_bytes;
+  a.host_block = a.host_block && host_page >= 0 ? a.host_block + host_page * 2 * (a.page_size * a.form.bytes) : nullptr;
+  a.within = (int)(length - page * a.page_size);
+  a.count = 1;
+  a.summary = item.summaries + page * row_elems;
+  a.minimum = static_cast<char*>(item.minimum) + page * row_elems * T::bytes;
+  a.maximum = static_cast<char*>(item.maximum) + page * row_elems * T::bytes;
+  const int plane = (int)blockIdx.x >= a.form.kv_heads;
+  append8_head<T, C, N>(a, plane, (int)blockIdx.x - plane * a.form.kv_heads);
+}
+
+// ---- read back ----------------------------------------------------------------------
+
+struct Read8Args {
+  const char* pool;
+  int64_t pool_rows, block_stride;
+  Row8 form;
+  int page_size;
+  FastDiv page_div, dim_div;
+  const int64_t* rows;
+  int64_t rows_stride;
+  int64_t n;
+  char* out[2];
+  int64_t out_stride[2];  // elements between rows
+};
+
+__device__ __forceinline__ const char* row8_at(const char* pool, int64_t row, int64_t pool_rows, int64_t block_stride,
+                                               int64_t row_bytes, int page_size, FastDiv page_div) {
+  if (row < 0 || row >= pool_rows) return nullptr;
+  const uint32_t page = page_div.div((uint32_t)row);
+  return pool + page * block_stride + (int64_t)((uint32_t)row - page * page_size) * row_bytes;
+}
+
+// A wave per row and plane.
+template <typename T, typename C>
+__global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= 2 * a.n) return;
+  const int plane = (int)(unit & 1);
+  const int64_t i = unit >> 1;
+  const char* row = row8_at(a.pool, a.rows[i * a.rows_stride], a.pool_rows, a.block_stride, a.form.bytes, a.page_size,
+                            a.page_div);
+  if (row) row += (int64_t)plane * a.page_size * a.form.bytes;
+  char* out = a.out[plane] + i * a.out_stride[plane] * T::bytes;
+  const int width = a.form.kv_heads * a.form.head_dim;
+  for (int e = lane; e < width; e += kWave) {
+    float value = 0.f;
+    if (row) {
+      const int head = (int)a.dim_div.div((uint32_t)e);
+      value = value8(decode8<C>((uint8_t)row[e]), *reinterpret_cast<const float*>(row + a.form.scales_at + 4 * head));
+    }
+    store_elem(out, T::dtype, e, value);
+  }
+}
+
+// Calls f with the tags of a storage type and a code.
+template <typename F>
+static void with_types(int dtype, int code, F f) {
+  const auto second = [&](auto t) {
+    if (code == NHS_CODE_I8)
+      f(t, I8());
+    else
+      f(t, E4M3());
+  };
+  if (dtype == NHS_BF16)
+    second(BF16());
+  else if (dtype == NHS_F16)
+    second(F16());
+  else
+    second(F32());
+}
+
+// Common checks of a pool of rows in 8 bits; sets a zero block stride to that of contiguous blocks.
+static int check_pool8(const char* who, const void* pool, int code, int kv_heads, int head_dim, int page_size,
+                       int64_t* block_stride) {
+  if (!pool) return fail(NHS_ERR_INVALID, "%s: null pointer", who);
+  if (!valid_code(code)) return fail(NHS_ERR_INVALID, "%s: bad code", who);
+  if (kv_heads < 1 || head_dim < 1 || page_size < 1) return fail(NHS_ERR_INVALID, "%s: invalid shape", who);
+  if (head_dim > NHS_MAX_HEAD_DIM8 || (int64_t)kv_heads * head_dim > (1 << 24))
+    return fail(NHS_ERR_UNSUPPORTED, "%s: head_dim must be <= %d and rows of at most 2^24 elements", who,
+                NHS_MAX_HEAD_DIM8);
+  const int64_t block = 2 * (int64_t)page_size * row8(kv_heads, head_dim).bytes;
+  if (*block_stride == 0) *block_stride = block;
+  if (*block_stride < block || *block_stride % 16 || (uintptr_t)pool % 16)
+    return fail(NHS_ERR_INVALID, "%s: the pool and its block stride must be multiples of 16 bytes, the stride at least "
+                "a block", who);
+  return NHS_OK;
+}
+
+template <typename T, typename C, typename F>
+static void with_width(int head_dim, F f) {
+  if (head_dim <= 2 * kWave)
+    f(std::integral_constant<int, 2>());
+  else if (head_dim <= 4 * kWave)
+    f(std::integral_constant<int, 4>());
+  else
+    f(std::integral_constant<int, kA8MaxDim / kWave>());
+}
+
+}  // namespace nhs
+
+extern "C" int64_t nhs_row8_bytes(int32_t kv_heads, int32_t head_dim) {
+  return kv_heads < 1 || head_dim < 1 ? 0 : nhs::row8(kv_heads, head_dim).bytes;
+}
+
+extern "C" int nhs_append_page8(const void* k, const void* v, int64_t token_stride, int32_t kv_dtype, int32_t code,
+                                int32_t kv_heads, int32_t head_dim, int32_t page_size, void* pool,
+                                int64_t pool_block_stride, int64_t block, int32_t within, int32_t count,
+                                void* host_alias, int64_t host_page, float* summary, void* minimum, void* maximum,
+                                void* stream) {
+  using namespace nhs;
+  const LaunchEvents ev = take_launch_events();
+  if (!k || !v || !summary || !minimum || !maximum) return fail(NHS_ERR_INVALID, "nhs_append_page8: null pointer");
+  if (!valid_dtype(kv_dtype)) return fail(NHS_ERR_INVALID, "nhs_append_page8: bad dtype");
+  if (const int st = check_pool8("nhs_append_page8", pool, code, kv_heads, head_dim, page_size, &pool_block_stride))
+    return st;
+  if (block < 0 || within < 0 || count < 1 || count > page_size || within > page_size - count ||
+      token_stride < (int64_t)kv_heads * head_dim || (host_alias && host_page < 0) || (uintptr_t)host_alias % 16)
+    return fail(NHS_ERR_INVALID, "nhs_append_page8: invalid page, rows, strides or host alignment");
+  Append8Args a;
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.token_stride = token_stride;
+  a.form = row8(kv_heads, head_dim);
+  a.page_size = page_size;
+  a.pool_block = static_cast<char*>(pool) + block * pool_block_stride;
+  a.host_block = host_alias ? static_cast<char*>(host_alias) + host_page * 2 * (page_size * a.form.bytes) : nullptr;
+  a.within = within;
+  a.count = count;
+  a.summary = summary;
+  a.minimum = minimum;
+  a.maximum = maximum;
+  with_types(kv_dtype, code, [&](auto t, auto c) {
+    using T = decltype(t);
+    using C = decltype(c);
+    with_width<T, C>(head_dim, [&](auto n) {
+      launch(append8_page_kernel<T, C, decltype(n)::value>, dim3((unsigned)(2 * kv_heads)), dim3(kA8Threads), 0,
+             (hipStream_t)stream, ev.start, ev.stop, a);
+    });
+  });
+  return launch_status("nhs_append_page8");
+}
+
+extern "C" int nhs_append_items8(int32_t batch, const void* k, const void* v, int64_t token_stride, int32_t kv_dtype,
+                                 int32_t code, int32_t kv_heads, int32_t head_dim, int32_t page_size, void* pool,
+                                 int64_t pool_block_stride, void* host_alias, const nhs_layer_item* items,
+                                 const int64_t* lengths, void* stream) {
+  using namespace nhs;
+  const LaunchEvents ev = take_launch_events();
+  if (!k || !v || !items || !lengths) return fail(NHS_ERR_INVALID, "nhs_append_items8: null pointer");
+  if (!valid_dtype(kv_dtype)) return fail(NHS_ERR_INVALID, "nhs_append_items8: bad dtype");
+  if (const int st = check_pool8("nhs_append_items8", pool, code, kv_heads, head_dim, page_size, &pool_block_stride))
+    return st;
+  if (batch < 0 || batch > 65535 || token_stride < (int64_t)kv_heads * head_dim || (uintptr_t)host_alias % 16)
+    return fail(NHS_ERR_INVALID, "nhs_append_items8: invalid batch, strides or host alignment");
+  if (batch == 0) return NHS_OK;
+  Append8ItemsArgs g;
+  g.a = Append8Args();
+  g.a.k = static_cast<const char*>(k);
+  g.a.v = static_cast<const char*>(v);
+  g.a.token_stride = token_stride;
+  g.a.form = row8(kv_heads, head_dim);
+  g.a.page_size = page_size;
+  g.a.pool_block = static_cast<char*>(pool);
+  g.a.host_block = static_cast<char*>(host_alias);
+  g.pool_block_bytes = pool_block_stride;
+  g.items = items;
+  g.lengths = lengths;
+  with_types(kv_dtype, code, [&](auto t, auto c) {
+    using T = decltype(t);
+    using C = decltype(c);
+    with_width<T, C>(head_dim, [&](auto n) {
+      launch(append8_items_kernel<T, C, decltype(n)::value>, dim3((unsigned)(2 * kv_heads), (unsigned)batch),
+             dim3(kA8Threads), 0, (hipStream_t)stream, ev.start, ev.stop, g);
+    });
+  });
+  return launch_status("nhs_append_items8");
+}
+
+extern "C" int nhs_read_rows8(const void* pool, int64_t pool_rows, int64_t pool_block_stride, int32_t code,
+                              int32_t kv_heads, int32_t head_dim, int32_t page_size, const int64_t* rows,
+                              int64_t rows_stride, int64_t n, int32_t out_dtype, void* k_out, int64_t k_stride,
+                              void* v_out, int64_t v_stride, void* stream) {
+  using namespace nhs;
+  const LaunchEvents ev = take_launch_events();
+  if (!rows || !k_out || !v_out) return fail(NHS_ERR_INVALID, "nhs_read_rows8: null pointer");
+  if (!valid_dtype(out_dtype)) return fail(NHS_ERR_INVALID, "nhs_read_rows8: bad dtype");
+  if (const int st = check_pool8("nhs_read_rows8", pool, code, kv_heads, head_dim, page_size, &pool_block_stride))
+    return st;
+  const int64_t width = (int64_t)kv_heads * head_dim;
+  if (n < 0 || pool_rows < 0 || pool_rows >= (1ll << 31) || k_stride < width || v_stride < width)
+    return fail(NHS_ERR_INVALID, "nhs_read_rows8: invalid rows or strides");
+  if (n == 0) return NHS_OK;
+  const int64_t groups = (2 * n + 3) / 4;
+  if (groups > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_read_rows8: too many rows");
+  Read8Args a;
+  a.pool = static_cast<const char*>(pool);
+  a.pool_rows = pool_rows;
+  a.block_stride = pool_block_stride;
+  a.form = row8(kv_heads, head_dim);
+  a.page_size = page_size;
+  a.page_div = FastDiv((uint32_t)page_size);
+  a.dim_div = FastDiv((uint32_t)head_dim);
+  a.rows = rows;
+  a.rows_stride = rows_stride;
+  a.n = n;
+  a.out[0] = static_cast<char*>(k_out);
+  a.out[1] = static_cast<char*>(v_out);
+  a.out_stride[0] = k_stride;
+  a.out_stride[1] = v_stride;
+  with_types(out_dtype, code, [&](auto t, auto c) {
+    launch(read8_kernel<decltype(t), decltype(c)>, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, ev.start,
+           ev.stop, a);
+  });
+  return launch_status("nhs_read_rows8");
+}

@@ -18,6 +18,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -647,23 +648,123 @@ PyObject* select_resolve_batched(PyObject*, PyObject* const* a, Py_ssize_t nargs
   });
 }
 
+// ---- rows in 8 bits ----------------------------------------------------------------------------
+
+// A row_kernels.Rows8 that the library takes.
+struct Form {
+  int code;
+  int32_t kv_heads, head_dim;
+  int64_t row_bytes;
+};
+Form form_of(PyObject* o) {
+  need(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 3 && THPDtype_Check(PyTuple_GET_ITEM(o, 0)));
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(PyTuple_GET_ITEM(o, 0))->scalar_type;
+  need(type == at::kChar || type == at::kFloat8_e4m3fn);
+  Form f;
+  f.code = type == at::kChar ? NHS_CODE_I8 : NHS_CODE_E4M3;
+  f.kv_heads = integer32(PyTuple_GET_ITEM(o, 1));
+  f.head_dim = integer32(PyTuple_GET_ITEM(o, 2));
+  need(f.kv_heads >= 1 && f.head_dim >= 1 && f.head_dim <= NHS_MAX_HEAD_DIM8);
+  f.row_bytes = nhs_row8_bytes(f.kv_heads, f.head_dim);
+  return f;
+}
+
+// Bytes between the blocks of a pool [blocks, 2, P, row_bytes].
+int64_t pool8_block_stride(const Tensor& pool, const Form& f) {
+  const int64_t P = pool.size(2), R = pool.size(3);
+  need(pool.scalar_type() == at::kByte && pool.size(1) == 2 && R == f.row_bytes && pool.stride(1) == P * R &&
+       pool.stride(2) == R && pool.stride(3) == 1 && pool.stride(0) >= 2 * P * R &&
+       pool.size(0) * P < (int64_t(1) << 31));
+  return pool.stride(0);
+}
+
+PyObject* attend_8bit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 5, [&]() -> PyObject* {
+    const Tensor &q = tensor(a[0]), &pool = tensor(a[1]), &rows = tensor(a[3]);
+    const Form f = form_of(a[2]);
+    on_gpu(q, 3);
+    on_gpu(pool, 4, q);
+    need(rows.dim() == 2 || rows.dim() == 3);
+    on_gpu(rows, rows.dim(), q);
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), n = rows.size(-1);
+    const int code = dtype_code(q);
+    need(rows.scalar_type() == at::kLong && D == f.head_dim && Hq % f.kv_heads == 0 && q.stride(2) == 1 &&
+         rows.size(0) == B && (rows.dim() == 2 || rows.size(1) == Hq) && n <= (1 << 30));
+    const int64_t stride = pool8_block_stride(pool, f);
+    Tensor out;
+    if (a[4] != Py_None) {
+      out = tensor(a[4]);
+      check_out(out, q);
+    }
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(q);
+      if (!out.defined()) out = make(q.sizes(), q, q.scalar_type());
+      const int64_t bytes =
+          nhs_attend_rows8_workspace_bytes((int32_t)B, (int32_t)n, (int32_t)Hq, f.kv_heads, f.head_dim);
+      const Tensor ws = scratch(bytes, q);
+      st = nhs_attend_rows8(q.data_ptr(), code, q.stride(0), q.stride(1), pool.data_ptr(), pool.size(0) * pool.size(2),
+                            stride, f.code, static_cast<const int64_t*>(rows.data_ptr()), rows.stride(0),
+                            rows.dim() == 3 ? rows.stride(1) : 0, rows.stride(-1), (int32_t)B, (int32_t)n, (int32_t)Hq,
+                            f.kv_heads, f.head_dim, (int32_t)pool.size(2), out.data_ptr(), out.stride(0),
+                            out.stride(1), scratch_ptr(ws), bytes, stream_of(q));
+    }
+    return st ? failed("nhs_attend_rows8", st) : THPVariable_Wrap(out);
+  });
+}
+
+// read_rows_8bit into new tensors
+PyObject* read_rows_8bit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 4, [&]() -> PyObject* {
+    const Tensor &pool = tensor(a[0]), &rows = tensor(a[2]);
+    const Form f = form_of(a[1]);
+    need(THPDtype_Check(a[3]));
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(a[3])->scalar_type;
+    need(type == at::kFloat || type == at::kHalf || type == at::kBFloat16);
+    on_gpu(pool, 4);
+    on_gpu(rows, 1, pool);
+    need(rows.scalar_type() == at::kLong);
+    const int64_t stride = pool8_block_stride(pool, f), n = rows.size(0), width = (int64_t)f.kv_heads * f.head_dim;
+    Tensor k, v;
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(pool);
+      k = make({n, f.kv_heads, f.head_dim}, pool, type);
+      v = make({n, f.kv_heads, f.head_dim}, pool, type);
+      st = nhs_read_rows8(pool.data_ptr(), pool.size(0) * pool.size(2), stride, f.code, f.kv_heads, f.head_dim,
+                          (int32_t)pool.size(2), static_cast<const int64_t*>(rows.data_ptr()), rows.stride(0), n,
+                          dtype_code(k), k.data_ptr(), width, v.data_ptr(), width, stream_of(pool));
+    }
+    return st ? failed("nhs_read_rows8", st) : tuple_of({k, v});
+  });
+}
+
 // ---- append ------------------------------------------------------------------------------------
 
-// nhs_append_page with the arguments row_kernels.PageAppender prepared (checked there), as whole numbers of any integer
-// type; returns the status.
-PyObject* append_page(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-  if (nargs != 17) {
+// Whole numbers of any integer type; negative ones go to the library, which refuses them.
+template <int N>
+bool whole_numbers(PyObject* const* a, Py_ssize_t nargs, int64_t (&v)[N]) {
+  if (nargs != N) {
     PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
-    return nullptr;
+    return false;
   }
-  int64_t v[17];
-  for (int i = 0; i < 17; ++i) {  // negative numbers go to the library, which refuses them
+  for (int i = 0; i < N; ++i) {
     PyObject* whole = PyNumber_Index(a[i]);
-    if (!whole) return nullptr;
+    if (!whole) return false;
     v[i] = (int64_t)PyLong_AsUnsignedLongLongMask(whole);
     Py_DECREF(whole);
-    if (PyErr_Occurred()) return nullptr;
+    if (PyErr_Occurred()) return false;
   }
+  return true;
+}
+
+// nhs_append_page and nhs_append_page8 with the arguments that row_kernels.PageAppender prepared (checked there);
+// they return the status.
+PyObject* append_page(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  int64_t v[17];
+  if (!whole_numbers(a, nargs, v)) return nullptr;
   const auto at = [&](int i) { return reinterpret_cast<void*>((uintptr_t)v[i]); };
   int st;
   {
@@ -671,6 +772,20 @@ PyObject* append_page(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     st = nhs_append_page(at(0), at(1), v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], at(6), v[7], v[8],
                          (int32_t)v[9], (int32_t)v[10], at(11), v[12], static_cast<float*>(at(13)), at(14), at(15),
                          at(16));
+  }
+  return PyLong_FromLong(st);
+}
+
+PyObject* append_page8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  int64_t v[19];
+  if (!whole_numbers(a, nargs, v)) return nullptr;
+  const auto at = [&](int i) { return reinterpret_cast<void*>((uintptr_t)v[i]); };
+  int st;
+  {
+    NoGil free;
+    st = nhs_append_page8(at(0), at(1), v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], (int32_t)v[6],
+                          (int32_t)v[7], at(8), v[9], v[10], (int32_t)v[11], (int32_t)v[12], at(13), v[14],
+                          static_cast<float*>(at(15)), at(16), at(17), at(18));
   }
   return PyLong_FromLong(st);
 }
@@ -733,6 +848,7 @@ PyMethodDef methods[] = {NHS_METHOD(linear_small_m), NHS_METHOD(linear_silu_mul)
                          NHS_METHOD(quest_batched),  NHS_METHOD(select_resolve_batched),
                          NHS_METHOD(append_page),    NHS_METHOD(held_state),        NHS_METHOD(tree_plan),
                          NHS_METHOD(tree_attention), NHS_METHOD(qk_norm_rope),      NHS_METHOD(token_logprobs),
+                         NHS_METHOD(attend_8bit),    NHS_METHOD(read_rows_8bit),    NHS_METHOD(append_page8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

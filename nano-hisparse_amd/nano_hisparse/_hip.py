@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_DIR, "libnhs_hip.so")
 HEADER_PATH = os.path.normpath(os.path.join(_DIR, "..", "..", "include", "nhs.h"))
 
 NHS_F32, NHS_F16, NHS_BF16 = 0, 1, 2
+NHS_CODE_I8, NHS_CODE_E4M3 = 0, 1
 ABI_VERSION = 2
 
 _i32, _i64, _p = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
@@ -103,6 +104,20 @@ SIGNATURES = {
     "nhs_token_logprobs_workspace_bytes": ([_i32, _i32, _i32, _i32], ctypes.c_int64),
     "nhs_token_logprobs": (
         [_p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _i32, _p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
+    "nhs_row8_bytes": ([_i32, _i32], ctypes.c_int64),
+    "nhs_append_page8": (
+        [_p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _i32, _i32, _p, _i64, _p, _p, _p, _p],
+        ctypes.c_int,
+    ),
+    "nhs_append_items8": ([_i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p], ctypes.c_int),
+    "nhs_read_rows8": (
+        [_p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i64, _i32, _p, _i64, _p, _i64, _p], ctypes.c_int),
+    "nhs_attend_rows8_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], ctypes.c_int64),
+    "nhs_attend_rows8": (
+        [_p, _i32, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p,
+         _i64, _i64, _p, _i64, _p],
+        ctypes.c_int,
+    ),
     "nhs_expand_columns": ([_p, _i64, _p, _i64, _i64, _p, _p], ctypes.c_int),
 }
 

@@ -193,7 +193,13 @@ def padded_pool(blocks, page_size, kv_heads, head_dim, dtype, device):
 def pool_block_stride(pool):
     """Bytes between consecutive blocks of a pool [blocks, 2, P, Hkv, D]: each
     block must be contiguous; a gap may follow it (stride(0) above
-    2 * P * Hkv * D elements), as in the cache's padded pool."""
+    2 * P * Hkv * D elements), as in the cache's padded pool. A pool of rows
+    in 8 bits is [blocks, 2, P, row_bytes] uint8."""
+    if pool.ndim == 4 and pool.dtype == torch.uint8:
+        _, _, P, R = pool.shape
+        if tuple(pool.stride()[1:]) != (P * R, R, 1) or pool.stride(0) < 2 * P * R:
+            raise ValueError("the pool's blocks must be contiguous [2, P, row_bytes] (a gap after each is allowed)")
+        return pool.stride(0)
     if pool.ndim != 5:
         raise ValueError("the pool must be [blocks, 2, page_size, kv_heads, head_dim]")
     _, _, P, Hkv, D = pool.shape
@@ -233,6 +239,234 @@ def set_gather_workgroups(workgroups):
 def gather_rows(host, pool, plan, config):
     """Reference signature (row_kernels.py:58-70): gather one RowPlan's misses."""
     gather_plan(host, pool, plan.miss_host_rows, plan.miss_device_rows, config.page_size)
+
+
+# ---- rows in 8 bits ----------------------------------------------------------------
+
+_CODES = {torch.int8: _hip.NHS_CODE_I8, torch.float8_e4m3fn: _hip.NHS_CODE_E4M3}
+MAX_HEAD_DIM8 = 1024
+
+
+class Rows8(NamedTuple):
+    """The form of a row held in 8 bits. In each of its two planes: kv_heads x
+    head_dim codes of the type `code` (torch.int8 or torch.float8_e4m3fn), then
+    (at the next multiple of 4 bytes) an fp32 scale for every KV head, padded
+    to a multiple of 16 bytes. Of the head_dim elements x of one token and
+    head, with Q the type's largest value (127 or 448):
+
+        scale = max(max|x| / Q, 2^-80)
+        code  = the type's value nearest to x / scale, ties to even
+        value = code * scale
+
+    A slice with an element that is not finite has scale NaN. Pools are uint8
+    [blocks, 2, page_size, row_bytes] (pool_8bit), host stores the same."""
+
+    code: torch.dtype
+    kv_heads: int
+    head_dim: int
+
+    @property
+    def scales_at(self) -> int:
+        """The offset of the scales in a plane's row."""
+        return -(-self.kv_heads * self.head_dim // 4) * 4
+
+    @property
+    def row_bytes(self) -> int:
+        return -(-(self.scales_at + 4 * self.kv_heads) // 16) * 16
+
+    def check(self, who):
+        if self.code not in _CODES:
+            raise ValueError(f"{who}: rows in 8 bits are int8 or float8_e4m3fn")
+        if self.kv_heads < 1 or not 1 <= self.head_dim <= MAX_HEAD_DIM8:
+            raise ValueError(f"{who}: at least one KV head, of 1 to {MAX_HEAD_DIM8} dims")
+
+    def codes(self, rows):
+        """The codes [..., kv_heads, head_dim] of rows [..., row_bytes], a view."""
+        n = self.kv_heads * self.head_dim
+        return rows[..., :n].view(self.code).unflatten(-1, (self.kv_heads, self.head_dim))
+
+    def scales(self, rows):
+        """The scales [..., kv_heads] of rows [..., row_bytes], a view."""
+        return rows[..., self.scales_at : self.scales_at + 4 * self.kv_heads].view(torch.float32)
+
+
+def pool_8bit(blocks, page_size, form, device):
+    """A pool of rows in 8 bits, uint8 [blocks, 2, page_size, row_bytes]. It
+    needs no padding (padded_pool): a row's scales shift the next row's heads."""
+    form.check("pool_8bit")
+    return torch.empty(blocks, 2, page_size, form.row_bytes, dtype=torch.uint8, device=device)
+
+
+def _check_pool8(who, pool, form):
+    """Checks a pool of rows in 8 bits; returns its block stride in bytes."""
+    form.check(who)
+    if pool.ndim != 4 or pool.dtype != torch.uint8 or pool.shape[1] != 2 or pool.shape[3] != form.row_bytes:
+        raise ValueError(f"{who}: the pool must be uint8 [blocks, 2, page_size, {form.row_bytes}]")
+    return pool_block_stride(pool)
+
+
+def append_page_8bit(k, v, pool, form, block, within, host, host_page, summary, minimum, maximum):
+    """append_page into a pool of rows in 8 bits: K/V rows [count, Hkv, D]
+    (bf16, fp16 or fp32) quantised into pool block `block` and, when `host` (a
+    MappedHost) is given, host block `host_page`; minimum/maximum [Hkv, D] (K's
+    dtype) fold in the keys as given, and summary [Hkv, D] (fp32) becomes the
+    mean of code * scale over the page's keys."""
+    token_stride = _check_append8("append_page_8bit", k, v, pool, form, host, (summary,), (minimum, maximum))
+    for t in (summary, minimum, maximum):
+        if t.shape != k.shape[1:]:
+            raise ValueError("append_page_8bit: summary and bounds are [kv_heads, head_dim]")
+    if not (0 <= block < pool.shape[0] and 0 <= within and 1 <= len(k) <= pool.shape[2] - within):
+        raise ValueError("append_page_8bit: block or rows outside the pool")
+    if host is not None and not 0 <= host_page < len(host.tensor):
+        raise ValueError("append_page_8bit: host page outside the store")
+    with _on(k.device):
+        status = _hip.load().nhs_append_page8(
+            _ptr(k), _ptr(v), token_stride, dtype_code(k.dtype), _CODES[form.code], form.kv_heads, form.head_dim,
+            pool.shape[2], _ptr(pool), pool_block_stride(pool), int(block), int(within), len(k),
+            ctypes.c_void_p(host.data_ptr() if host is not None else 0), int(host_page if host is not None else 0),
+            _ptr(summary), _ptr(minimum), _ptr(maximum), _stream(k.device),
+        )
+    _hip.check(status, "nhs_append_page8")
+
+
+def _check_append8(who, k, v, pool, form, host, summaries, bounds):
+    """The checks of appends into rows in 8 bits that do not depend on a page;
+    returns the elements between tokens."""
+    _require_gpu(who, k, v, pool, *summaries, *bounds)
+    _check_pool8(who, pool, form)
+    dtype_code(k.dtype)
+    if k.shape != v.shape or k.ndim != 3 or tuple(k.shape[1:]) != (form.kv_heads, form.head_dim):
+        raise ValueError(f"{who}: K/V must be [tokens, {form.kv_heads}, {form.head_dim}]")
+    if v.dtype != k.dtype or any(t.dtype != k.dtype for t in bounds):
+        raise ValueError(f"{who}: K, V and bounds must have one dtype")
+    if any(t.dtype != torch.float32 for t in summaries):
+        raise ValueError(f"{who}: summaries are float32")
+    if any(not t.is_contiguous() or t.shape[-2:] != k.shape[1:] for t in (*summaries, *bounds)):
+        raise ValueError(f"{who}: summaries and bounds are contiguous [..., kv_heads, head_dim]")
+    stride = k.stride(0) if len(k) > 1 else form.kv_heads * form.head_dim
+    if len(k) and not (k[0].is_contiguous() and v[0].is_contiguous()) or (len(k) > 1 and v.stride(0) != stride) \
+            or stride < form.kv_heads * form.head_dim:
+        raise ValueError(f"{who}: K/V rows must be contiguous with equal token strides")
+    if host is not None and (host.dtype != torch.uint8 or tuple(host.tensor.shape[1:]) != tuple(pool.shape[1:])
+                             or not host.tensor.is_contiguous()):
+        raise ValueError(f"{who}: the host store must be contiguous blocks of the pool's")
+    return stride
+
+
+def append_items_8bit(k, v, pool, form, host, items, lengths):
+    """append_items into a pool of rows in 8 bits: one token per item, k/v
+    [B, Hkv, D], appended at lengths[b] of each item's layer. An item whose
+    page is not bound is left alone."""
+    token_stride = _check_append8("append_items_8bit", k, v, pool, form, host, (), ())
+    device, B = k.device, len(k)
+    if items.shape[0] != B or items.dtype != torch.int64 or lengths.shape != (B,) or lengths.dtype != torch.int64 \
+            or items.device != device or lengths.device != device:
+        raise ValueError("append_items_8bit: one item and one int64 length per row")
+    if items.shape[1:] != (len(_hip.LAYER_ITEM_FIELDS),) or not items.is_contiguous() or not lengths.is_contiguous():
+        raise ValueError("append_items_8bit: items are contiguous [B, 9] (layer_items), lengths contiguous")
+    if B == 0:
+        return
+    with _on(device):
+        status = _hip.load().nhs_append_items8(
+            B, _ptr(k), _ptr(v), token_stride, dtype_code(k.dtype), _CODES[form.code], form.kv_heads, form.head_dim,
+            pool.shape[2], _ptr(pool), pool_block_stride(pool),
+            ctypes.c_void_p(host.data_ptr() if host is not None else 0), _ptr(items), _ptr(lengths), _stream(device),
+        )
+    _hip.check(status, "nhs_append_items8")
+
+
+def read_rows_8bit(pool, form, rows, dtype, out=None):
+    """The K and V rows [n, Hkv, D], in `dtype` (bf16, fp16 or fp32), that a
+    pool of rows in 8 bits holds at the physical rows rows [n] (int64, any
+    order, the same one as often as wanted); zeros for rows outside the pool,
+    such as -1. `out`: a pair to write to, each with contiguous [Hkv, D] rows;
+    they overlap neither each other nor an input."""
+    if pool.is_cuda and out is None:
+        done = (_launch or _load_launch()).read_rows_8bit(pool, form, rows, dtype)
+        if done is not None:
+            return done
+    device = _require_gpu("read_rows_8bit", pool, rows)
+    stride = _check_pool8("read_rows_8bit", pool, form)
+    code = dtype_code(dtype)
+    if rows.ndim != 1 or rows.dtype != torch.int64:
+        raise ValueError("read_rows_8bit: rows [n] int64")
+    n, shape = len(rows), (len(rows), form.kv_heads, form.head_dim)
+    _check_counts("read_rows_8bit", n)
+    if pool.shape[0] * pool.shape[2] >= 2**31:
+        raise ValueError("read_rows_8bit: pool rows must be < 2^31")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    else:
+        out = tuple(out)
+        if len(out) != 2:
+            raise ValueError("read_rows_8bit: out is a pair (k, v)")
+        for t in out:
+            _check_out("read_rows_8bit", t, shape, dtype, device)
+            if n and (t.stride(1) != form.head_dim and form.kv_heads > 1):
+                raise ValueError("read_rows_8bit: out's rows must be contiguous")
+        if n and out[0].data_ptr() == out[1].data_ptr():
+            raise ValueError("read_rows_8bit: out's elements must be distinct")
+    if n == 0:
+        return out
+    if pool.shape[0] == 0:
+        return out[0].zero_(), out[1].zero_()
+    width = form.kv_heads * form.head_dim
+    with _on(device):
+        status = _hip.load().nhs_read_rows8(
+            _ptr(pool), pool.shape[0] * pool.shape[2], stride, _CODES[form.code], form.kv_heads, form.head_dim,
+            pool.shape[2], _ptr(rows), rows.stride(0), n, code, _ptr(out[0]), out[0].stride(0) if n > 1 else width,
+            _ptr(out[1]), out[1].stride(0) if n > 1 else width, _stream(device),
+        )
+    _hip.check(status, "nhs_read_rows8")
+    return out
+
+
+def attend_8bit(query, pool, form, rows, out=None):
+    """attend_batched over a pool of rows in 8 bits: query [B, Hq, D] (bf16,
+    fp16 or fp32) over the physical rows rows [B, N] (shared by the heads of a
+    request) or [B, Hq, N] (a list per head), int64, those outside the pool
+    (such as -1) masked. Returns [B, Hq, D] in the query's dtype, zeros for a
+    head without a row. `out` may be given and overlaps no input."""
+    if query.is_cuda:
+        done = (_launch or _load_launch()).attend_8bit(query, pool, form, rows, out)
+        if done is not None:
+            return done
+    device = _require_gpu("attend_8bit", query, pool, rows)
+    stride = _check_pool8("attend_8bit", pool, form)
+    if query.ndim != 3 or rows.ndim not in (2, 3) or rows.dtype != torch.int64:
+        raise ValueError("attend_8bit: query [B, Hq, D], int64 rows [B, N] or [B, Hq, N]")
+    B, Hq, D = query.shape
+    if D != form.head_dim or Hq < 1 or Hq % form.kv_heads:
+        raise ValueError("attend_8bit: query/pool head shape mismatch")
+    code = dtype_code(query.dtype)
+    if query.stride(2) != 1 and D > 1:
+        raise ValueError("attend_8bit: query rows must be contiguous")
+    if rows.shape[0] != B or (rows.ndim == 3 and rows.shape[1] != Hq):
+        raise ValueError("attend_8bit: rows do not match the query batch/heads")
+    if pool.shape[0] * pool.shape[2] >= 2**31 or rows.shape[-1] > 2**30:
+        raise ValueError("attend_8bit: pool rows must be < 2^31, a list at most 2^30")
+    _check_counts("attend_8bit", B, Hq)
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=query.dtype, device=device)
+    else:
+        _check_out("attend_8bit", out, query.shape, query.dtype, device)
+    if out.numel() == 0:
+        return out
+    n_rows = rows.shape[-1] if pool.shape[0] else 0
+    if n_rows == 0:
+        return out.zero_()
+    lib = _hip.load()
+    with _on(device):
+        need = lib.nhs_attend_rows8_workspace_bytes(B, n_rows, Hq, form.kv_heads, D)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        status = lib.nhs_attend_rows8(
+            _ptr(query), code, query.stride(0), query.stride(1), _ptr(pool), pool.shape[0] * pool.shape[2], stride,
+            _CODES[form.code], _ptr(rows), rows.stride(0), rows.stride(1) if rows.ndim == 3 else 0, rows.stride(-1), B,
+            n_rows, Hq, form.kv_heads, D, pool.shape[2], _ptr(out), out.stride(0), out.stride(1), _ptr(workspace), need,
+            _stream(device),
+        )
+    _hip.check(status, "nhs_attend_rows8")
+    return out
 
 
 # ---- append ----------------------------------------------------------------------
@@ -277,15 +511,39 @@ class PageAppender:
     checked and turned into launch arguments once, so that each page costs
     one library call."""
 
-    def __init__(self, k, v, pool, host, summaries, minimum, maximum):
-        device = _require_gpu("append_page", k, v, pool, summaries, minimum, maximum)
+    def __init__(self, k, v, pool, host, summaries, minimum, maximum, form=None):
+        """form (Rows8): the pool and the host store hold rows in 8 bits (append_page_8bit)."""
+        launch = _launch or _load_launch()
+        if form is not None:
+            self.token_stride = _check_append8("append_page", k, v, pool, form, host, (summaries,), (minimum, maximum))
+            self.append_page = launch.append_page8
+            shape = (_CODES[form.code], form.kv_heads, form.head_dim)
+            self.limits = (pool.shape[0], len(host.tensor) if host is not None else 1,
+                           min(t.shape[:-2].numel() for t in (summaries, minimum, maximum)))
+        else:
+            self._check(k, v, pool, host, summaries, minimum, maximum)
+            self.token_stride = k.stride(0)
+            self.append_page = launch.append_page
+            shape = (k.shape[1] * k.shape[2],)
+            self.limits = None
+        self.k, self.v = k, v  # held for the write
+        self.esize = k.element_size()
+        self.k_ptr, self.v_ptr = k.data_ptr(), v.data_ptr()
+        self.row_elems, self.shape = k.shape[1] * k.shape[2], (dtype_code(k.dtype), *shape, pool.shape[2])
+        self.pool_ptr, self.pool_stride = pool.data_ptr(), pool_block_stride(pool)
+        self.host_ptr = host.data_ptr() if host is not None else 0
+        self.sum_ptr, self.min_ptr, self.max_ptr = summaries.data_ptr(), minimum.data_ptr(), maximum.data_ptr()
+        self.stream = _raw_stream(_device_index(k.device))
+
+    @staticmethod
+    def _check(k, v, pool, host, summaries, minimum, maximum):
+        _require_gpu("append_page", k, v, pool, summaries, minimum, maximum)
         if k.shape != v.shape or k.ndim != 3 or tuple(k.shape[1:]) != tuple(pool.shape[3:]):
             raise ValueError("append_page: K/V must be [tokens, kv_heads, head_dim] of the pool")
         if k.dtype != pool.dtype or v.dtype != pool.dtype or minimum.dtype != pool.dtype or maximum.dtype != pool.dtype:
             raise ValueError("append_page: K/V and bounds must have the pool dtype")
         if summaries.dtype != torch.float32:
             raise ValueError("append_page: the summary is float32")
-        row_elems = k.shape[1] * k.shape[2]
         for t in (summaries, minimum, maximum):
             if not t.is_contiguous() or t.shape[-2:] != k.shape[1:]:
                 raise ValueError("append_page: summaries and bounds are contiguous [..., kv_heads, head_dim]")
@@ -294,15 +552,6 @@ class PageAppender:
             raise ValueError("append_page: K/V rows must be contiguous with equal token strides")
         if host is not None and host.dtype != pool.dtype:
             raise ValueError("append_page: host and pool dtypes differ")
-        self.append_page = (_launch or _load_launch()).append_page
-        self.k, self.v = k, v  # held for the write
-        self.esize = k.element_size()
-        self.k_ptr, self.v_ptr, self.token_stride = k.data_ptr(), v.data_ptr(), k.stride(0)
-        self.dtype, self.row_elems, self.page_size = dtype_code(pool.dtype), row_elems, pool.shape[2]
-        self.pool_ptr, self.pool_stride = pool.data_ptr(), pool_block_stride(pool)
-        self.host_ptr = host.data_ptr() if host is not None else 0
-        self.sum_ptr, self.min_ptr, self.max_ptr = summaries.data_ptr(), minimum.data_ptr(), maximum.data_ptr()
-        self.stream = _raw_stream(_device_index(device))
 
     def __call__(self, first, count, block, within, host_page, bounds_index):
         """Rows first..first+count-1 of the write into rows within.. of pool
@@ -310,12 +559,15 @@ class PageAppender:
         page's index in the flattened [layers, pages] bounds."""
         if not (0 <= first and count >= 1 and first + count <= self.k.shape[0]):
             raise ValueError("append_page: rows outside the write")
+        if self.limits is not None and not (0 <= block < self.limits[0] and 0 <= bounds_index < self.limits[2]
+                                            and (not self.host_ptr or 0 <= host_page < self.limits[1])):
+            raise ValueError("append_page: page outside the pool, the host store or the bounds")
         off = bounds_index * self.row_elems
         row = first * self.token_stride * self.esize
         status = self.append_page(
-            self.k_ptr + row, self.v_ptr + row, self.token_stride, self.dtype, self.row_elems, self.page_size,
-            self.pool_ptr, self.pool_stride, block, within, count, self.host_ptr, host_page if self.host_ptr else 0,
-            self.sum_ptr + off * 4, self.min_ptr + off * self.esize, self.max_ptr + off * self.esize, self.stream,
+            self.k_ptr + row, self.v_ptr + row, self.token_stride, *self.shape, self.pool_ptr, self.pool_stride, block,
+            within, count, self.host_ptr, host_page if self.host_ptr else 0, self.sum_ptr + off * 4,
+            self.min_ptr + off * self.esize, self.max_ptr + off * self.esize, self.stream,
         )
         _hip.check(status, "nhs_append_page")
 
