@@ -26,6 +26,9 @@ struct Attend8Args {
   int64_t r_bs, r_hs, r_cs;
   int batch, n_rows, q_heads, kv_heads, group, head_dim, page_size;
   int rows_per_split, n_splits;
+  // the kernel on the matrix cores: items of a (request, split) = kv_heads x chunks of heads_per_item query heads
+  int heads_per_item, chunks, subs, groups;
+  bool near, q_aligned;  // near: the items of a (request, split) on one XCD
   FastDiv page_div;
   float scale_log2;  // D^-1/2 * log2(e)
   void* out;
@@ -133,6 +136,342 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
   }
 }
 
+// ---- heads of 32, 64, 128 and 256, on the matrix cores ------------------------------------
+
+// A workgroup of 8 waves takes up to 16 query heads of one (request, KV head)
+// and one split of the rows; wave w takes tiles w, w + 8, ... of 32 rows.
+// Codes are exact in bf16, so the products run on v_mfma_f32_16x16x32_bf16:
+// S^T = K Q^T and O^T = V^T P^T. Lane l supplies A[l % 16][8 (l / 16) + j] and
+// B[8 (l / 16) + j][l % 16], j = 0..7, and holds D[4 (l / 16) + i][l % 16],
+// i = 0..3: so lane l has the scores of head l % 16 against rows 4 (l / 16) + i
+// of the tile's halves, which are the rows it has to supply to P^T (the order
+// of rows within a product is free), its softmax is a lane's own work, and V
+// comes transposed from LDS (ds_read_b64_tr_b8: of each 16 lanes, lanes 2r and
+// 2r + 1 name 16 bytes of row r, and lane i receives column i of the 8 rows).
+//
+// A bf16 query is one operand, an fp16 query the sum of two bf16 numbers and
+// an fp32 query of three, exactly; a weight (times the scale of the row's
+// values) goes as two bf16 numbers, 2^-17 of it lost, or for fp32 queries as
+// three.
+constexpr int kF8Threads = 512, kF8Waves = kF8Threads / kWave, kF8Tile = 32, kF8Heads = 16;
+
+typedef __bf16 f8_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 f8_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f8_f32x2 __attribute__((ext_vector_type(2)));
+typedef float f8_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t f8_u32x4 __attribute__((ext_vector_type(4)));
+typedef int f8_i32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __attribute__((aligned(256))) char attend8_zeros[256];  // read in place of a masked row
+
+__device__ __forceinline__ f8_f32x4 f8_mfma(f8_u32x4 a, f8_u32x4 b, f8_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(f8_bf16x8, a), __builtin_bit_cast(f8_bf16x8, b), c,
+                                                 0, 0, 0);
+}
+
+// two codes (the lower or the upper half of a word) as a pair of bf16 numbers, exactly
+template <typename C, bool UPPER>
+__device__ __forceinline__ uint32_t f8_pair(uint32_t word) {
+  if constexpr (C::code == NHS_CODE_E4M3) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)word, 1.f, UPPER));
+  } else {
+    const float a = (float)(int8_t)(word >> (UPPER ? 16 : 0)), b = (float)(int8_t)(word >> (UPPER ? 24 : 8));
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  }
+}
+
+// eight codes as an operand
+template <typename C>
+__device__ __forceinline__ f8_u32x4 f8_operand(uint32_t lo, uint32_t hi) {
+  return (f8_u32x4){f8_pair<C, false>(lo), f8_pair<C, true>(lo), f8_pair<C, false>(hi), f8_pair<C, true>(hi)};
+}
+
+__device__ __forceinline__ uint32_t f8_round(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f8_f32x2){lo, hi}, f8_bf16x2));
+}
+
+// eight fp32 numbers as P bf16 operands whose sum they are
+template <int P>
+__device__ __forceinline__ void f8_split(float (&x)[8], f8_u32x4 (&out)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = f8_round(x[2 * j], x[2 * j + 1]);
+      out[p][j] = pair;
+      if (p + 1 < P) {
+        x[2 * j] -= __uint_as_float(pair << 16);
+        x[2 * j + 1] -= __uint_as_float(pair & 0xffff0000u);
+      }
+    }
+}
+
+// LDS slot of 16-byte chunk c of K row r (N chunks a row): eight consecutive rows at one chunk fall on distinct banks
+template <int N>
+__device__ __forceinline__ int f8_k_slot(int r, int c) {
+  return N >= 8 ? c ^ (r & 7) : N == 4 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1);
+}
+// and of V row r: the eight rows of a transposing read, 4g .. 4g + 3 of both halves of a tile
+template <int N>
+__device__ __forceinline__ int f8_v_slot(int r, int c) {
+  return N >= 8   ? c ^ ((r & 3) | (r >> 2 & 4))
+         : N == 4 ? c ^ ((r >> 1 & 1) | (r >> 3 & 2))
+                  : c ^ (r >> 4 & 1);
+}
+
+// The tiles in LDS are written and read by the lanes of one wave, whose LDS instructions the hardware runs in order:
+// only the compiler has to keep them so.
+__device__ __forceinline__ void f8_order() { asm volatile("" ::: "memory"); }
+
+template <typename C, int QP, int D, int DEPTH>
+__global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a) {
+  constexpr int PP = QP == 3 ? 3 : 2;     // operands of the weights
+  constexpr int N = D / 16;               // 16-byte chunks of a head's row
+  constexpr int RI = kWave / N;           // rows of a load instruction
+  constexpr int KI = kF8Tile / RI;        // load instructions of a tile, for K and for V each
+  constexpr int KS = D / 32;              // products of a score
+  constexpr int kRows = DEPTH * kF8Tile;  // of a wave's round
+  struct Wave {
+    f8_u32x4 k[kF8Tile * N], v[kF8Tile * N];
+    const char* at[kRows][2];  // the rows' K and V
+    float ks[kRows], vs[kRows];
+  };
+  constexpr int kMerged = kF8Waves * kF8Heads * (D + 4) * 4;
+  constexpr int kBytes = kF8Waves * (int)sizeof(Wave) > kMerged ? kF8Waves * (int)sizeof(Wave) : kMerged;
+  __shared__ __attribute__((aligned(16))) char lds[kBytes];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  int sub, group;
+  if (a.near) {
+    const int rest = blockIdx.x >> 3;
+    sub = rest % a.subs;
+    group = rest / a.subs * 8 + (blockIdx.x & 7);
+    if (group >= a.groups) return;
+  } else {
+    sub = blockIdx.x % a.subs;
+    group = blockIdx.x / a.subs;
+  }
+  const int b = group / a.n_splits, split = group - b * a.n_splits;
+  const int kv = sub / a.chunks, h0 = kv * a.group + (sub - kv * a.chunks) * a.heads_per_item;
+  const int heads = min(a.heads_per_item, (kv + 1) * a.group - h0);
+  Wave& w = reinterpret_cast<Wave*>(lds)[wave];
+
+  const int64_t* list = a.rows + (int64_t)b * a.r_bs + (int64_t)h0 * a.r_hs;
+  const int begin = split * a.rows_per_split, end = min(a.n_rows, begin + a.rows_per_split);
+  // row of the wave's round that entry e of its addresses is for
+  const auto row_of = [&](int round, int e) {
+    return begin + ((round * DEPTH + e / kF8Tile) * kF8Waves + wave) * kF8Tile + e % kF8Tile;
+  };
+  constexpr int kMine = (kRows + kWave - 1) / kWave;  // addresses of a lane
+  int64_t index[kMine];
+  const auto fetch = [&](int round) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int r = row_of(round, (lane + i * kWave) % kRows);
+      index[i] = r < end ? list[(int64_t)r * a.r_cs] : -1;
+    }
+  };
+  fetch(0);
+
+  // the query as operand B: head n, dims in the order in which K's chunks give them
+  f8_u32x4 q[QP][KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d0 = N >= 4 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * g;
+    float x[8];
+    const int64_t at = (int64_t)b * a.q_bs + (int64_t)(h0 + min(n, heads - 1)) * a.q_hs + d0;
+    if (a.q_aligned) {
+      if constexpr (QP == 1)
+        load_vec<BF16, 8>(a.q, at, x);
+      else if constexpr (QP == 2)
+        load_vec<F16, 8>(a.q, at, x);
+      else
+        load_vec<F32, 8>(a.q, at, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = load_elem(a.q, QP == 1 ? NHS_BF16 : QP == 2 ? NHS_F16 : NHS_F32, at + j);
+    }
+    f8_u32x4 parts[QP];
+    f8_split<QP>(x, parts);
+#pragma unroll
+    for (int p = 0; p < QP; ++p) q[p][s] = parts[p];
+  }
+
+  f8_f32x4 acc[N];
+#pragma unroll
+  for (int t = 0; t < N; ++t) acc[t] = (f8_f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  const int rounds = (end - begin + kF8Waves * kRows - 1) / (kF8Waves * kRows);
+  for (int round = 0; round < rounds; ++round) {
+    // addresses and scales of the round's rows
+    uint64_t seen[kMine];
+    float ks[kMine], vs[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const bool in = index[i] >= 0 && index[i] < a.pool_rows;
+      const uint32_t at = in ? (uint32_t)index[i] : 0u, page = a.page_div.div(at);
+      const char* row = a.pool + page * a.block_stride + (int64_t)(at - page * a.page_size) * a.row_bytes;
+      const char* kp = in ? row + kv * D : attend8_zeros;
+      const char* vp = in ? row + a.plane_bytes + kv * D : attend8_zeros;
+      const int64_t to_scale = in ? a.scales_at + 4 * (int64_t)kv - kv * D : 0;
+      seen[i] = __ballot(in);
+      if (kMine * kWave == kRows || lane < kRows) {
+        w.at[lane + i * kWave][0] = kp;
+        w.at[lane + i * kWave][1] = vp;
+      }
+      ks[i] = *(const NHS_GLOBAL float*)(kp + to_scale);
+      vs[i] = *(const NHS_GLOBAL float*)(vp + to_scale);
+    }
+    f8_order();
+    // all loads of the round, then its tiles one by one
+    f8_u32x4 k[DEPTH][KI], v[DEPTH][KI];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const char* at[KI][2];
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        at[i][0] = w.at[d * kF8Tile + i * RI + lane / N][0] + lane % N * 16;
+        at[i][1] = w.at[d * kF8Tile + i * RI + lane / N][1] + lane % N * 16;
+      }
+#pragma unroll
+      for (int i = 0; i < KI; ++i) k[d][i] = *(const NHS_GLOBAL f8_u32x4*)at[i][0];
+#pragma unroll
+      for (int i = 0; i < KI; ++i) v[d][i] = *(const NHS_GLOBAL f8_u32x4*)at[i][1];
+    }
+    if (round + 1 < rounds) fetch(round + 1);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (kMine * kWave == kRows || lane < kRows) {
+        w.ks[lane + i * kWave] = ks[i] * a.scale_log2;
+        w.vs[lane + i * kWave] = vs[i];
+      }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      f8_order();
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int r = i * RI + lane / N;
+        w.k[r * N + f8_k_slot<N>(r, lane % N)] = k[d][i];
+        w.v[r * N + f8_v_slot<N>(r, lane % N)] = v[d][i];
+      }
+      f8_order();
+      f8_f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = (f8_f32x4){0.f, 0.f, 0.f, 0.f};
+        const int r = 16 * u + n;
+        if constexpr (N >= 4) {
+#pragma unroll
+          for (int c = 0; c < N / 4; ++c) {
+            const f8_u32x4 x = w.k[r * N + f8_k_slot<N>(r, 4 * c + g)];
+            const f8_u32x4 lo = f8_operand<C>(x[0], x[1]), hi = f8_operand<C>(x[2], x[3]);
+#pragma unroll
+            for (int p = 0; p < QP; ++p) {
+              s[u] = f8_mfma(lo, q[p][2 * c], s[u]);
+              s[u] = f8_mfma(hi, q[p][2 * c + 1], s[u]);
+            }
+          }
+        } else {
+          const char* at = reinterpret_cast<const char*>(&w.k[r * N + f8_k_slot<N>(r, g >> 1)]) + 8 * (g & 1);
+          const uint2 x = *reinterpret_cast<const uint2*>(at);
+#pragma unroll
+          for (int p = 0; p < QP; ++p) s[u] = f8_mfma(f8_operand<C>(x.x, x.y), q[p][0], s[u]);
+        }
+      }
+      // weights of rows 4g + i and 16 + 4g + i
+      const uint32_t word = (uint32_t)(seen[d * kF8Tile / kWave] >> (d * kF8Tile % kWave));
+      float p[8], top = m;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f8_f32x4 scale = *reinterpret_cast<const f8_f32x4*>(&w.ks[d * kF8Tile + 16 * u + 4 * g]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[4 * u + i] = word >> (16 * u + 4 * g + i) & 1 ? s[u][i] * scale[i] : -INFINITY;
+          top = fmaxf(top, p[4 * u + i]);
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f8_f32x4 scale = *reinterpret_cast<const f8_f32x4*>(&w.vs[d * kF8Tile + 16 * u + 4 * g]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(p[4 * u + i] - ref);
+          l += e;
+          p[4 * u + i] = e * scale[i];
+        }
+      }
+      f8_u32x4 weights[PP];
+      f8_split<PP>(p, weights);
+      if (__ballot(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) acc[t] *= alpha;
+      }
+      const int vr = (n >> 1 & 3) + 4 * g + (n >> 3) * 16;  // the row that this lane names for a transposing read
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        const char* at = reinterpret_cast<const char*>(&w.v[vr * N + f8_v_slot<N>(vr, t)]) + 8 * (n & 1);
+        const f8_i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) f8_i32x2*)const_cast<char*>(at));
+        const f8_u32x4 values = f8_operand<C>((uint32_t)x.x, (uint32_t)x.y);
+#pragma unroll
+        for (int pp = 0; pp < PP; ++pp) acc[t] = f8_mfma(values, weights[pp], acc[t]);
+      }
+    }
+    f8_order();
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // the waves' sums are joined through LDS: [wave][head][D, max, sum]
+  __syncthreads();
+  constexpr int kPitch = D + 4;
+  float* merged = reinterpret_cast<float*>(lds);
+  if (n < heads) {
+    float* mine = merged + (wave * heads + n) * kPitch;
+#pragma unroll
+    for (int t = 0; t < N; ++t) *reinterpret_cast<f8_f32x4*>(mine + 16 * t + 4 * g) = acc[t];
+    if (g == 0) {
+      mine[D] = m;
+      mine[D + 1] = l;
+    }
+  }
+  __syncthreads();
+  const int64_t all = (int64_t)a.batch * a.q_heads;
+  for (int i = threadIdx.x; i < heads * D; i += kF8Threads) {
+    const int h = i / D, d = i - h * D;
+    const float* from = merged + h * kPitch;
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kF8Waves; ++x) top = fmaxf(top, from[x * heads * kPitch + D]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float total = 0.f, o = 0.f;
+#pragma unroll
+    for (int x = 0; x < kF8Waves; ++x) {
+      const float* one = from + x * heads * kPitch;
+      const float f = __builtin_amdgcn_exp2f(one[D] - ref);
+      total = __builtin_fmaf(one[D + 1], f, total);
+      o = __builtin_fmaf(one[d], f, o);
+    }
+    if (a.n_splits > 1) {
+      const int64_t at = split * all + (int64_t)b * a.q_heads + h0 + h;
+      a.partial[at * D + d] = o;
+      if (d == 0) {
+        a.stats[2 * at] = top;
+        a.stats[2 * at + 1] = total;
+      }
+    } else {
+      store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)(h0 + h) * a.o_hs + d, total != 0.f ? o / total : 0.f);
+    }
+  }
+}
+
 // ---- joining the splits ------------------------------------------------------------------
 
 // A wave per (request, query head).
@@ -161,10 +500,58 @@ __global__ __launch_bounds__(kWave) void attend8_join_kernel(Attend8Args a) {
 
 constexpr int kA8MaxSplits = 64;
 
-// About two workgroups per CU, splits of at least 64 rows.
-static int splits8(int64_t items, int n_rows) {
-  const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + 63) / 64);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(most, 512 / items));
+struct Plan8 {
+  bool flash;
+  int heads_per_item, chunks, subs, splits, rows_per_split, depth;
+};
+
+// own_lists: every query head has a row list of its own.
+static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_dim, bool own_lists) {
+  Plan8 p;
+  p.flash = head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256;
+  p.heads_per_item = p.flash && !own_lists ? kF8Heads : 1;
+  const int group = q_heads / kv_heads;
+  p.chunks = (group + p.heads_per_item - 1) / p.heads_per_item;
+  p.subs = kv_heads * p.chunks;
+  const int64_t items = (int64_t)batch * p.subs;
+  if (!p.flash) {
+    // about two workgroups per CU, splits of at least 64 rows
+    const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + 63) / 64);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, 512 / items));
+    p.rows_per_split = (n_rows + p.splits - 1) / p.splits;
+    p.depth = 1;
+    return p;
+  }
+  // about one workgroup per CU, splits of whole rounds of its eight waves
+  constexpr int kStep = kF8Waves * kF8Tile;
+  const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + kStep - 1) / kStep);
+  int splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (256 + items / 2) / items));
+  int per = (n_rows + splits - 1) / splits;
+  per = (per + kStep - 1) / kStep * kStep;
+  p.splits = (n_rows + per - 1) / per;
+  p.rows_per_split = per;
+  p.depth = per <= kStep || head_dim == 256 ? 1 : per <= 2 * kStep ? 2 : 4;
+  return p;
+}
+
+static int64_t workspace8(const Plan8& p, int64_t heads, int head_dim) {
+  return p.splits == 1 ? 0 : p.splits * heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+template <typename C, int QP>
+static void (*flash8(int head_dim, int depth))(Attend8Args) {
+  switch (head_dim * 8 + depth) {
+    case 32 * 8 + 1: return attend8_flash_kernel<C, QP, 32, 1>;
+    case 32 * 8 + 2: return attend8_flash_kernel<C, QP, 32, 2>;
+    case 32 * 8 + 4: return attend8_flash_kernel<C, QP, 32, 4>;
+    case 64 * 8 + 1: return attend8_flash_kernel<C, QP, 64, 1>;
+    case 64 * 8 + 2: return attend8_flash_kernel<C, QP, 64, 2>;
+    case 64 * 8 + 4: return attend8_flash_kernel<C, QP, 64, 4>;
+    case 128 * 8 + 1: return attend8_flash_kernel<C, QP, 128, 1>;
+    case 128 * 8 + 2: return attend8_flash_kernel<C, QP, 128, 2>;
+    case 128 * 8 + 4: return attend8_flash_kernel<C, QP, 128, QP == 3 ? 2 : 4>;  // (fp32 queries: registers)
+    default: return attend8_flash_kernel<C, QP, 256, 1>;
+  }
 }
 
 }  // namespace nhs
@@ -174,8 +561,9 @@ extern "C" int64_t nhs_attend_rows8_workspace_bytes(int32_t batch, int32_t n_row
   using namespace nhs;
   if (batch < 1 || n_rows < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1) return 0;
   const int64_t heads = (int64_t)batch * q_heads;
-  const int splits = splits8(heads, n_rows);
-  return splits == 1 ? 0 : splits * heads * (head_dim + 2) * (int64_t)sizeof(float);
+  if (q_heads % kv_heads || n_rows > (1 << 30)) return 0;
+  return std::max(workspace8(plan8(batch, n_rows, q_heads, kv_heads, head_dim, false), heads, head_dim),
+                  workspace8(plan8(batch, n_rows, q_heads, kv_heads, head_dim, true), heads, head_dim));
 }
 
 extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_batch_stride, int64_t q_head_stride,
@@ -202,7 +590,8 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
     return fail(NHS_ERR_INVALID, "nhs_attend_rows8: the pool and its block stride must be multiples of 16 bytes, the "
                 "stride at least a block");
   const int64_t heads = (int64_t)batch * q_heads;
-  const int64_t need = nhs_attend_rows8_workspace_bytes(batch, n_rows, q_heads, kv_heads, head_dim);
+  const Plan8 plan = plan8(batch, n_rows, q_heads, kv_heads, head_dim, rows_head_stride != 0);
+  const int64_t need = workspace8(plan, heads, head_dim);
   if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
     return fail(NHS_ERR_WORKSPACE, "nhs_attend_rows8: needs a 16-byte aligned workspace of %lld bytes",
                 (long long)need);
@@ -233,29 +622,51 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
   a.out = out;
   a.o_bs = out_batch_stride;
   a.o_hs = out_head_stride;
-  a.n_splits = splits8(heads, n_rows);
-  a.rows_per_split = (n_rows + a.n_splits - 1) / a.n_splits;
+  a.n_splits = plan.splits;
+  a.rows_per_split = plan.rows_per_split;
   a.partial = static_cast<float*>(workspace);
   a.stats = a.partial ? a.partial + a.n_splits * heads * head_dim : nullptr;
-  if (heads * a.n_splits > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_attend_rows8: grid too large");
   const bool join = a.n_splits > 1;
-  const auto run = [&](auto c, auto n) {
-    launch(attend8_general_kernel<decltype(c), decltype(n)::value>, dim3((unsigned)(heads * a.n_splits)),
-           dim3(kG8Threads), 0, (hipStream_t)stream, ev.start, join ? nullptr : ev.stop, a);
-  };
-  const auto wide = [&](auto c) {
-    if (head_dim <= 2 * kWave)
-      run(c, std::integral_constant<int, 2>());
-    else if (head_dim <= 4 * kWave)
-      run(c, std::integral_constant<int, 4>());
+  hipStream_t s = (hipStream_t)stream;
+  hipEvent_t stop = join ? nullptr : ev.stop;
+  if (plan.flash) {
+    a.heads_per_item = plan.heads_per_item;
+    a.chunks = plan.chunks;
+    a.subs = plan.subs;
+    if ((int64_t)batch * plan.splits * plan.subs > (1 << 30))
+      return fail(NHS_ERR_UNSUPPORTED, "nhs_attend_rows8: grid too large");
+    a.groups = batch * plan.splits;
+    a.near = a.groups >= 8;
+    const int vec = q_dtype == NHS_F32 ? 4 : 8;  // elements of 16 bytes
+    a.q_aligned = (uintptr_t)query % 16 == 0 && q_batch_stride % vec == 0 && q_head_stride % vec == 0;
+    const int64_t grid = (int64_t)plan.subs * (a.near ? (a.groups + 7) / 8 * 8 : a.groups);
+    const auto pick = [&](auto c) {
+      using C = decltype(c);
+      return q_dtype == NHS_BF16  ? flash8<C, 1>(head_dim, plan.depth)
+             : q_dtype == NHS_F16 ? flash8<C, 2>(head_dim, plan.depth)
+                                  : flash8<C, 3>(head_dim, plan.depth);
+    };
+    launch(code == NHS_CODE_I8 ? pick(I8()) : pick(E4M3()), dim3((unsigned)grid), dim3(kF8Threads), 0, s, ev.start, stop,
+           a);
+  } else {
+    if (heads * a.n_splits > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_attend_rows8: grid too large");
+    const auto run = [&](auto c, auto n) {
+      launch(attend8_general_kernel<decltype(c), decltype(n)::value>, dim3((unsigned)(heads * a.n_splits)),
+             dim3(kG8Threads), 0, s, ev.start, stop, a);
+    };
+    const auto wide = [&](auto c) {
+      if (head_dim <= 2 * kWave)
+        run(c, std::integral_constant<int, 2>());
+      else if (head_dim <= 4 * kWave)
+        run(c, std::integral_constant<int, 4>());
+      else
+        run(c, std::integral_constant<int, NHS_MAX_HEAD_DIM8 / kWave>());
+    };
+    if (code == NHS_CODE_I8)
+      wide(I8());
     else
-      run(c, std::integral_constant<int, NHS_MAX_HEAD_DIM8 / kWave>());
-  };
-  if (code == NHS_CODE_I8)
-    wide(I8());
-  else
-    wide(E4M3());
-  if (join)
-    launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kWave), 0, (hipStream_t)stream, nullptr, ev.stop, a);
+      wide(E4M3());
+  }
+  if (join) launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kWave), 0, s, nullptr, ev.stop, a);
   return launch_status("nhs_attend_rows8");
 }
