@@ -119,7 +119,7 @@ constexpr int kRowsHeld = 2 * kRowsPerPass;                 // rows folded betwe
 constexpr int kFoldBatch = 16;                              // rows read from LDS together
 constexpr int kCopyChunks = 4;                              // chunks per thread of a copying workgroup
 
-typedef uint32_t append_u4 __attribute__((ext_vector_type(4)));
+typedef u32x4 append_u4;
 
 template <typename T, typename Elem>
 __device__ __forceinline__ float widen(Elem bits) {
@@ -137,15 +137,6 @@ __device__ __forceinline__ const NHS_GLOBAL append_u4* new_chunk(const AppendArg
                                                                  uint32_t chunk, int esize) {
   const NHS_GLOBAL char* src = to_global(static_cast<const char*>(plane ? a.v : a.k));
   return (const NHS_GLOBAL append_u4*)(src + (int64_t)row * a.token_stride * esize + (int64_t)chunk * 16);
-}
-
-// A store that leaves the caches at once (system scope). Plain stores to
-// pinned host memory stay in L2 until the kernel ends, and the PCIe writes
-// then follow everything else: a page took 10.9 us, against 6.6 with the
-// fold beside the writes. The builtin spelling (a volatile store) would wait
-// after every store. s_nop: the data registers must outlive the issue.
-__device__ __forceinline__ void store_through(NHS_GLOBAL char* p, append_u4 v) {
-  asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
 }
 
 // Copies the new rows to the pool and the host block, kCopyChunks * 256

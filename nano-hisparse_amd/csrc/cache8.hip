@@ -4,6 +4,7 @@
 // model's type (nhs_read_rows8).
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "rows8.h"
@@ -145,29 +146,222 @@ struct Append8ItemsArgs {
   const int64_t* lengths;
 };
 
-// Item blockIdx.y appends its one token: its page and row follow from its
-// length and its page tables. An item whose page is not bound is left alone.
+// The page and row that an item's one token goes to follow from its length and
+// its page tables; false for one whose page is not bound, which is left alone.
+template <typename T>
+__device__ __forceinline__ bool item8(const Append8ItemsArgs& g, int b, Append8Args* a) {
+  const nhs_layer_item& item = g.items[b];
+  *a = g.a;
+  const int64_t length = g.lengths[b], page = length / a->page_size;
+  if (length < 0 || page >= item.n_pages) return false;
+  const int block = item.resident[page], host_page = item.source[page];
+  if (block < 0) return false;
+  const int64_t row_elems = (int64_t)a->form.kv_heads * a->form.head_dim;
+  a->k += (int64_t)b * a->token_stride * T::bytes;
+  a->v += (int64_t)b * a->token_stride * T::bytes;
+  a->pool_block += block * g.pool_block_bytes;
+  a->host_block =
+      a->host_block && host_page >= 0 ? a->host_block + host_page * 2 * (a->page_size * a->form.bytes) : nullptr;
+  a->within = (int)(length - page * a->page_size);
+  a->count = 1;
+  a->summary = item.summaries + page * row_elems;
+  a->minimum = static_cast<char*>(item.minimum) + page * row_elems * T::bytes;
+  a->maximum = static_cast<char*>(item.maximum) + page * row_elems * T::bytes;
+  return true;
+}
+
 template <typename T, typename C, int N>
 __global__ __launch_bounds__(kA8Threads) void append8_items_kernel(Append8ItemsArgs g) {
-  const int b = blockIdx.y;
-  const nhs_layer_item& item = g.items[b];
-  Append8Args a = g.a;
-  const int64_t length = g.lengths[b], page = length / a.page_size;
-  if (length < 0 || page >= item.n_pages) return;
-  const int block = item.resident[page], host_page = item.source[page];
-  if (block < 0) return;
-  const int64_t row_elems = (int64_t)a.form.kv_heads * a.form.head_dim;
-  a.k += (int64_t)b * a.token_stride * T::bytes;
-  a.v += (int64_t)b * a.token_stride * T::bytes;
-  a.pool_block += block * g.pool_block_bytes;
-  a.host_block = a.host_block && host_page >= 0 ? a.host_block + host_page * 2 * (a.page_size * a.form.bytes) : nullptr;
-  a.within = (int)(length - page * a.page_size);
-  a.count = 1;
-  a.summary = item.summaries + page * row_elems;
-  a.minimum = static_cast<char*>(item.minimum) + page * row_elems * T::bytes;
-  a.maximum = static_cast<char*>(item.maximum) + page * row_elems * T::bytes;
+  Append8Args a;
+  if (!item8<T>(g, blockIdx.y, &a)) return;
   const int plane = (int)blockIdx.x >= a.form.kv_heads;
   append8_head<T, C, N>(a, plane, (int)blockIdx.x - plane * a.form.kv_heads);
+}
+
+// ---- heads of 32, 64, 128 and 256 dims: rows of whole chunks ------------------------------
+
+// Some workgroups copy: a wave takes 64 chunks of 16 elements of a row's plane
+// (so whole heads), quantises them and writes 1 KB of codes to the pool and
+// past the caches to the host block, whose rows are consecutive. Others fold
+// the keys of one head each: they quantise them too (the copies' codes are not
+// written yet), hold 64 rows of codes and keys in LDS and walk them, a thread
+// per element and share of the rows.
+constexpr int kFold8Rows = 64;
+
+template <typename T, int N>
+struct Fold8 {
+  uint32_t codes[kFold8Rows * N * 4];
+  std::conditional_t<T::bytes == 4, float, uint16_t> keys[kFold8Rows * N * 16];
+  float scales[kFold8Rows];
+  double sums[kA8Threads];
+  float low[kA8Threads], high[kA8Threads];
+};
+
+// 16 elements of one lane as they lie, and as fp32
+template <typename T>
+struct Chunk8 {
+  u32x4 raw[T::bytes];
+  float x[16];
+  __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+    for (int i = 0; i < T::bytes; ++i) raw[i] = reinterpret_cast<const NHS_GLOBAL u32x4*>(to_global(p))[i];
+  }
+  __device__ __forceinline__ void widen() {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (T::dtype == NHS_F32) {
+        x[e] = __uint_as_float(raw[e / 4][e % 4]);
+      } else {
+        const uint32_t half = raw[e / 8][e / 2 % 4] >> (e % 2 * 16) & 0xffffu;
+        x[e] = T::dtype == NHS_BF16 ? bf16_bits_to_f32(half) : f16_bits_to_f32(half);
+      }
+    }
+  }
+};
+
+// The codes and the scale of a slice that N neighbouring lanes hold.
+template <typename T, typename C, int N>
+__device__ __forceinline__ u32x4 quantise8(Chunk8<T>& c, float* scale) {
+  c.widen();
+  uint32_t largest = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) largest = max(largest, __float_as_uint(c.x[e]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < N; d <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d));
+  *scale = scale8<C>(largest);
+  const float inv = __fdiv_rn(1.f, *scale);
+  u32x4 codes;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float four[4] = {c.x[4 * i], c.x[4 * i + 1], c.x[4 * i + 2], c.x[4 * i + 3]};
+    codes[i] = codes8<C>(four, *scale, inv);
+  }
+  return codes;
+}
+
+template <typename T, typename C, int N>
+__device__ __forceinline__ void copy8(const Append8Args& a, int unit, int groups) {
+  const int lane = threadIdx.x & 63, chunks = a.form.kv_heads * N;
+  const int row = unit / groups, group = unit - row * groups;
+  if (row >= 2 * a.count) return;
+  const int plane = row >= a.count, t = row - plane * a.count;
+  const int chunk = group * kWave + lane;
+  const bool live = chunk < chunks;
+  Chunk8<T> c;
+  c.load((plane ? a.v : a.k) + ((int64_t)t * a.token_stride + min(chunk, chunks - 1) * 16) * T::bytes);
+  float scale;
+  const u32x4 codes = quantise8<T, C, N>(c, &scale);
+  const int64_t at = ((int64_t)plane * a.page_size + a.within + t) * a.form.bytes;
+  const float head_scale = __shfl(scale, lane * N % kWave);
+  const bool scales = lane < kWave / N && group * (kWave / N) + lane < a.form.kv_heads;
+  const int64_t to_scale = at + a.form.scales_at + 4 * (group * (kWave / N) + lane);
+  if (live) {
+    *(NHS_GLOBAL u32x4*)to_global(a.pool_block + at + chunk * 16) = codes;
+    if (a.host_block) store_through(to_global(a.host_block + at + chunk * 16), codes);
+  }
+  if (scales) {
+    *(NHS_GLOBAL float*)to_global(a.pool_block + to_scale) = head_scale;
+    if (a.host_block) *(NHS_GLOBAL float*)to_global(a.host_block + to_scale) = head_scale;
+  }
+}
+
+template <typename T, typename C, int N>
+__device__ __forceinline__ void fold8(const Append8Args& a, int head) {
+  constexpr int D = N * 16, kParts = kA8Threads / D, kRowsPerPass = kA8Threads / N;
+  constexpr int kPasses = (kFold8Rows + kRowsPerPass - 1) / kRowsPerPass;
+  __shared__ __attribute__((aligned(16))) Fold8<T, N> s;
+  const int tid = threadIdx.x, chunk = tid % N, slot = tid / N;
+  const int col = tid % D, part = tid / D;
+  const int64_t slice = (int64_t)head * D, at_scale = a.form.scales_at + 4 * (int64_t)head;
+  const int total = a.within + a.count;
+  double sum = 0.0;
+  float low = INFINITY, high = -INFINITY, low0 = 0.f, high0 = 0.f;
+  if (part == 0) {
+    low0 = load_elem(a.minimum, T::dtype, slice + col);
+    high0 = load_elem(a.maximum, T::dtype, slice + col);
+  }
+  for (int r0 = 0; r0 < total; r0 += kFold8Rows) {
+    const int rows = min(kFold8Rows, total - r0);
+    // every load of the rows before the first wait: earlier ones from the pool, new ones as they were given (both in
+    // bounds for every thread)
+    u32x4 held[kPasses];
+    float scale[kPasses];
+    Chunk8<T> fresh[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = min(r0 + slot + i * kRowsPerPass, total - 1);
+      if (r < a.within) {
+        const char* row = a.pool_block + (int64_t)r * a.form.bytes;
+        held[i] = *(const NHS_GLOBAL u32x4*)to_global(row + slice + chunk * 16);
+        scale[i] = *(const NHS_GLOBAL float*)to_global(row + at_scale);
+      }
+      fresh[i].load(a.k + ((int64_t)max(r - a.within, 0) * a.token_stride + slice + chunk * 16) * T::bytes);
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int j = slot + i * kRowsPerPass, r = r0 + j;
+      float own;
+      const u32x4 codes = quantise8<T, C, N>(fresh[i], &own);
+      if (j >= rows) continue;
+      const bool earlier = r < a.within;
+      *reinterpret_cast<u32x4*>(&s.codes[(j * N + chunk) * 4]) = earlier ? held[i] : codes;
+      if (!earlier)
+#pragma unroll
+        for (int x = 0; x < T::bytes; ++x)
+          reinterpret_cast<u32x4*>(&s.keys[(j * N + chunk) * 16])[x] = fresh[i].raw[x];
+      if (chunk == 0) s.scales[j] = earlier ? scale[i] : own;
+    }
+    __syncthreads();
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(s.codes) + col;
+#pragma unroll 8
+    for (int j = part; j < rows; j += kParts) sum += (double)decode8<C>(codes[j * D]) * (double)s.scales[j];
+#pragma unroll 8
+    for (int j = max(a.within - r0, 0) + part; j < rows; j += kParts) {
+      const float key = load_elem(s.keys, T::dtype, j * D + col);
+      low = least(low, key);
+      high = most(high, key);
+    }
+    __syncthreads();
+  }
+  s.sums[tid] = sum;
+  s.low[tid] = low;
+  s.high[tid] = high;
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int p = 1; p < kParts; ++p) {
+    sum += s.sums[p * D + col];
+    low = least(low, s.low[p * D + col]);
+    high = most(high, s.high[p * D + col]);
+  }
+  store_elem(a.minimum, T::dtype, slice + col, least(low0, low));
+  store_elem(a.maximum, T::dtype, slice + col, most(high0, high));
+  a.summary[slice + col] = (float)(sum / (double)total);
+}
+
+template <typename T, typename C, int N>
+__device__ __forceinline__ void append8_rows(const Append8Args& a) {
+  const int group = blockIdx.x;
+  if (group < a.form.kv_heads) return fold8<T, C, N>(a, group);
+  const int groups = (a.form.kv_heads * N + kWave - 1) / kWave;
+  copy8<T, C, N>(a, (group - a.form.kv_heads) * kA8Waves + ((int)threadIdx.x >> 6), groups);
+}
+
+// Workgroups of a launch for `count` rows.
+static unsigned rows8_grid(const Row8& form, int count) {
+  const int64_t groups = ((int64_t)form.kv_heads * (form.head_dim / 16) + kWave - 1) / kWave;
+  return (unsigned)(form.kv_heads + (2 * count * groups + kA8Waves - 1) / kA8Waves);
+}
+
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kA8Threads) void append8_rows_kernel(Append8Args a) {
+  append8_rows<T, C, N>(a);
+}
+
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kA8Threads) void append8_item_rows_kernel(Append8ItemsArgs g) {
+  Append8Args a;
+  if (item8<T>(g, blockIdx.y, &a)) append8_rows<T, C, N>(a);
 }
 
 // ---- read back ----------------------------------------------------------------------
@@ -215,6 +409,63 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
   }
 }
 
+// Heads of a multiple of 8 dims: a thread turns V codes into 16 bytes, kRead8
+// of them in flight (heads and units of a row by exact division).
+constexpr int kRead8 = 4;
+
+template <typename T, typename C>
+__global__ __launch_bounds__(256) void read8_chunks_kernel(Read8Args a, FastDiv per_row, FastDiv per_head,
+                                                           int rows_per_group) {
+  constexpr int V = 16 / T::bytes;
+  const int64_t first = (int64_t)blockIdx.x * rows_per_group;
+  const uint32_t units = (uint32_t)min((int64_t)rows_per_group, a.n - first) * per_row.d, half = per_row.d / 2;
+  for (uint32_t x0 = threadIdx.x; x0 < units; x0 += 256 * kRead8) {
+    uint32_t code[kRead8][V / 4];
+    float scale[kRead8];
+    bool there[kRead8];
+    char* out[kRead8];
+#pragma unroll
+    for (int u = 0; u < kRead8; ++u) {
+      const uint32_t x = min(x0 + u * 256, units - 1), i = per_row.div(x), in_row = x - i * per_row.d;
+      const uint32_t plane = in_row >= half, unit = in_row - plane * half;
+      const int64_t at = first + i;
+      const char* row = row8_at(a.pool, a.rows[at * a.rows_stride], a.pool_rows, a.block_stride, a.form.bytes,
+                                a.page_size, a.page_div);
+      out[u] = (plane ? a.out[1] : a.out[0]) + (at * (plane ? a.out_stride[1] : a.out_stride[0]) + unit * V) * T::bytes;
+      // unconditional loads (row 0 in place of one outside the pool), so that no branch separates them
+      const char* from = (row ? row : a.pool) + (int64_t)plane * a.page_size * a.form.bytes;
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w) code[u][w] = reinterpret_cast<const NHS_GLOBAL uint32_t*>(to_global(from) + unit * V)[w];
+      scale[u] = *(const NHS_GLOBAL float*)(to_global(from) + a.form.scales_at + 4 * per_head.div(unit));
+      there[u] = row != nullptr;
+    }
+#pragma unroll
+    for (int u = 0; u < kRead8; ++u) {
+      if (x0 + u * 256 >= units) break;
+      float v[V];
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w) {
+        float four[4];
+        decode8<C>(code[u][w], four);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * w + e] = there[u] ? value8(four[e], scale[u]) : 0.f;
+      }
+      u32x4 words;
+      if constexpr (T::dtype == NHS_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) words[e] = __float_as_uint(v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          words[e] = T::dtype == NHS_BF16
+                         ? f32_to_bf16_bits(v[2 * e]) | (uint32_t)f32_to_bf16_bits(v[2 * e + 1]) << 16
+                         : f32_to_f16_bits(v[2 * e]) | (uint32_t)f32_to_f16_bits(v[2 * e + 1]) << 16;
+      }
+      *(NHS_GLOBAL u32x4*)to_global(out[u]) = words;
+    }
+  }
+}
+
 // Calls f with the tags of a storage type and a code.
 template <typename F>
 static void with_types(int dtype, int code, F f) {
@@ -247,6 +498,26 @@ static int check_pool8(const char* who, const void* pool, int code, int kv_heads
     return fail(NHS_ERR_INVALID, "%s: the pool and its block stride must be multiples of 16 bytes, the stride at least "
                 "a block", who);
   return NHS_OK;
+}
+
+// Whether rows are whole chunks of 16 elements wherever append8_rows touches them.
+static bool whole_chunks8(const Append8Args& a, int dtype) {
+  const int d = a.form.head_dim;
+  return (d == 32 || d == 64 || d == 128 || d == 256) && a.token_stride * elem_size(dtype) % 16 == 0 &&
+         ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0;
+}
+
+// Calls f with the chunks of 16 elements of a head.
+template <typename F>
+static void with_chunks(int head_dim, F f) {
+  if (head_dim == 32)
+    f(std::integral_constant<int, 2>());
+  else if (head_dim == 64)
+    f(std::integral_constant<int, 4>());
+  else if (head_dim == 128)
+    f(std::integral_constant<int, 8>());
+  else
+    f(std::integral_constant<int, 16>());
 }
 
 template <typename T, typename C, typename F>
@@ -292,6 +563,16 @@ extern "C" int nhs_append_page8(const void* k, const void* v, int64_t token_stri
   a.summary = summary;
   a.minimum = minimum;
   a.maximum = maximum;
+  if (whole_chunks8(a, kv_dtype)) {
+    const dim3 grid(rows8_grid(a.form, count));
+    with_types(kv_dtype, code, [&](auto t, auto c) {
+      with_chunks(head_dim, [&](auto n) {
+        launch(append8_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kA8Threads), 0,
+               (hipStream_t)stream, ev.start, ev.stop, a);
+      });
+    });
+    return launch_status("nhs_append_page8");
+  }
   with_types(kv_dtype, code, [&](auto t, auto c) {
     using T = decltype(t);
     using C = decltype(c);
@@ -328,6 +609,16 @@ extern "C" int nhs_append_items8(int32_t batch, const void* k, const void* v, in
   g.pool_block_bytes = pool_block_stride;
   g.items = items;
   g.lengths = lengths;
+  if (whole_chunks8(g.a, kv_dtype)) {
+    const dim3 grid(rows8_grid(g.a.form, 1), (unsigned)batch);
+    with_types(kv_dtype, code, [&](auto t, auto c) {
+      with_chunks(head_dim, [&](auto n) {
+        launch(append8_item_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kA8Threads), 0,
+               (hipStream_t)stream, ev.start, ev.stop, g);
+      });
+    });
+    return launch_status("nhs_append_items8");
+  }
   with_types(kv_dtype, code, [&](auto t, auto c) {
     using T = decltype(t);
     using C = decltype(c);
@@ -370,6 +661,19 @@ extern "C" int nhs_read_rows8(const void* pool, int64_t pool_rows, int64_t pool_
   a.out[1] = static_cast<char*>(v_out);
   a.out_stride[0] = k_stride;
   a.out_stride[1] = v_stride;
+  const int esize = elem_size(out_dtype), vec = 16 / esize;
+  if (pool_rows > 0 && head_dim % 8 == 0 && ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 && k_stride * esize % 16 == 0 &&
+      v_stride * esize % 16 == 0) {
+    const uint32_t per_row = (uint32_t)(2 * width / vec);
+    const int rows_per_group = (int)std::max<int64_t>(1, 256 * kRead8 / per_row);
+    const int64_t grid = (n + rows_per_group - 1) / rows_per_group;
+    if (grid > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_read_rows8: too many rows");
+    with_types(out_dtype, code, [&](auto t, auto c) {
+      launch(read8_chunks_kernel<decltype(t), decltype(c)>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,
+             ev.start, ev.stop, a, FastDiv(per_row), FastDiv((uint32_t)(head_dim / vec)), rows_per_group);
+    });
+    return launch_status("nhs_read_rows8");
+  }
   with_types(out_dtype, code, [&](auto t, auto c) {
     launch(read8_kernel<decltype(t), decltype(c)>, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, ev.start,
            ev.stop, a);

@@ -93,6 +93,17 @@ __device__ __forceinline__ uint16_t f32_to_f16_bits(float f) {
   return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A store that leaves the caches at once (system scope). Plain stores to
+// pinned host memory stay in L2 until the kernel ends, and the PCIe writes
+// then follow everything else: appending a page took 10.9 us, against 6.6 with
+// the fold beside the writes. The builtin spelling (a volatile store) would wait
+// after every store. s_nop: the data registers must outlive the issue.
+__device__ __forceinline__ void store_through(NHS_GLOBAL char* p, u32x4 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
+}
+
 // Scalar load/store of one element with a runtime dtype (used for queries
 // and outputs, which are touched once per workgroup).
 __device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
