@@ -472,33 +472,83 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   }
 }
 
+constexpr int kA8MaxSplits = 64;  // (one lane of the joining waves each)
+
 // ---- joining the splits ------------------------------------------------------------------
 
-// A wave per (request, query head).
-__global__ __launch_bounds__(kWave) void attend8_join_kernel(Attend8Args a) {
-  const int heads = a.batch * a.q_heads, item = blockIdx.x, lane = threadIdx.x, D = a.head_dim;
-  float top = -INFINITY;
-  for (int s = 0; s < a.n_splits; ++s) top = fmaxf(top, a.stats[2 * ((int64_t)s * heads + item)]);
-  const float ref = top == -INFINITY ? 0.f : top;
+// A workgroup per (request, query head): a thread takes four dims (D / 4
+// rounded up to a power of two threads) of every shares-th split, and the
+// shares are added through LDS. One wave that walked 32 splits took 29.8 us
+// for 32 heads of 128.
+constexpr int kJ8Threads = 256;
+
+__global__ __launch_bounds__(kJ8Threads) void attend8_join_kernel(Attend8Args a, int quads) {
+  __shared__ float sums[kJ8Threads][4];
+  __shared__ float weights[kA8MaxSplits];
+  const int64_t heads = (int64_t)a.batch * a.q_heads;
+  const int item = blockIdx.x, tid = threadIdx.x, D = a.head_dim;
   const int b = item / a.q_heads, h = item - b * a.q_heads;
-  float total = 0.f;
-  for (int s = 0; s < a.n_splits; ++s) {
-    const float* st = a.stats + 2 * ((int64_t)s * heads + item);
-    total = __builtin_fmaf(st[1], __builtin_amdgcn_exp2f(st[0] - ref), total);
-  }
-  for (int d = lane; d < D; d += kWave) {
-    float o = 0.f;
-    for (int s = 0; s < a.n_splits; ++s) {
-      const int64_t at = (int64_t)s * heads + item;
-      o = __builtin_fmaf(a.partial[at * D + d], __builtin_amdgcn_exp2f(a.stats[2 * at] - ref), o);
+  const int quad = tid & (quads - 1), share = tid / quads, shares = kJ8Threads / quads;
+  // the first partial sums of a thread are asked for beside the statistics
+  const bool wide = D % 4 == 0;
+  const auto load = [&](int s, int d, float (&v)[4]) {
+    const float* p = a.partial + (s * heads + item) * D + d;
+    if (wide) {
+      const f8_f32x4 x = *reinterpret_cast<const f8_f32x4*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = p[min(e, D - 1 - d)];
     }
-    store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d, total != 0.f ? o / total : 0.f);
+  };
+  constexpr int kAhead = 4;
+  float ahead[kAhead][4];
+  const int d0 = min(4 * quad, (D - 1) / 4 * 4);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(min(share + i * shares, a.n_splits - 1), d0, ahead[i]);
+  const int lane = tid & 63;  // every wave reduces the statistics of up to 64 splits
+  const float* st = a.stats + 2 * ((int64_t)min(lane, a.n_splits - 1) * heads + item);
+  const float m = lane < a.n_splits ? st[0] : -INFINITY, l = lane < a.n_splits ? st[1] : 0.f;
+  float top = m;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m - ref);
+  const float total = wave_sum(l * f);
+  if (tid < a.n_splits) weights[tid] = f;
+  __syncthreads();
+  for (int d = 4 * quad; d < (D + 4 * quads - 1) / (4 * quads) * (4 * quads); d += 4 * quads) {
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d < D)
+      for (int s = share, i = 0; s < a.n_splits; s += shares, ++i) {
+        float v[4];
+        if (d == 4 * quad && i < kAhead) {
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x)
+            if (i == x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = ahead[x][e];
+        } else {
+          load(s, d, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], weights[s], o[e]);
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[tid][e] = o[e];
+    __syncthreads();
+    if (share == 0 && d < D) {
+      for (int x = 1; x < shares; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += sums[x * quads + quad][e];
+      for (int e = 0; e < 4 && d + e < D; ++e)
+        store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d + e, total != 0.f ? o[e] / total : 0.f);
+    }
+    __syncthreads();
   }
 }
 
 // ---- host --------------------------------------------------------------------------------
-
-constexpr int kA8MaxSplits = 64;
 
 struct Plan8 {
   bool flash;
@@ -667,6 +717,10 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
     else
       wide(E4M3());
   }
-  if (join) launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kWave), 0, s, nullptr, ev.stop, a);
+  if (join) {
+    int quads = 1;
+    while (quads * 4 < head_dim && quads < kJ8Threads) quads *= 2;
+    launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kJ8Threads), 0, s, nullptr, ev.stop, a, quads);
+  }
   return launch_status("nhs_attend_rows8");
 }
