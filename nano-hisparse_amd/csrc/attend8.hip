@@ -325,21 +325,18 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
       vs[i] = *(const NHS_GLOBAL float*)(vp + to_scale);
     }
     f8_order();
-    // all loads of the round, then its tiles one by one
+    // all loads of the round, the keys first: scores and weights are there when the last values come
     f8_u32x4 k[DEPTH][KI], v[DEPTH][KI];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const char* at[KI][2];
+    for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        at[i][0] = w.at[d * kF8Tile + i * RI + lane / N][0] + lane % N * 16;
-        at[i][1] = w.at[d * kF8Tile + i * RI + lane / N][1] + lane % N * 16;
-      }
+      for (int i = 0; i < KI; ++i)
+        k[d][i] = *(const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][0] + lane % N * 16);
 #pragma unroll
-      for (int i = 0; i < KI; ++i) k[d][i] = *(const NHS_GLOBAL f8_u32x4*)at[i][0];
+    for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
-      for (int i = 0; i < KI; ++i) v[d][i] = *(const NHS_GLOBAL f8_u32x4*)at[i][1];
-    }
+      for (int i = 0; i < KI; ++i)
+        v[d][i] = *(const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][1] + lane % N * 16);
     if (round + 1 < rounds) fetch(round + 1);
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
@@ -347,6 +344,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
         w.ks[lane + i * kWave] = ks[i] * a.scale_log2;
         w.vs[lane + i * kWave] = vs[i];
       }
+    // scores of rows 4g + i and 16 + 4g + i of every tile
+    float p[DEPTH][8], top = m;
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       f8_order();
@@ -354,13 +353,12 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
       for (int i = 0; i < KI; ++i) {
         const int r = i * RI + lane / N;
         w.k[r * N + f8_k_slot<N>(r, lane % N)] = k[d][i];
-        w.v[r * N + f8_v_slot<N>(r, lane % N)] = v[d][i];
       }
       f8_order();
-      f8_f32x4 s[2];
+      const uint32_t word = (uint32_t)(seen[d * kF8Tile / kWave] >> (d * kF8Tile % kWave));
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        s[u] = (f8_f32x4){0.f, 0.f, 0.f, 0.f};
+        f8_f32x4 s = (f8_f32x4){0.f, 0.f, 0.f, 0.f};
         const int r = 16 * u + n;
         if constexpr (N >= 4) {
 #pragma unroll
@@ -368,52 +366,60 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
             const f8_u32x4 x = w.k[r * N + f8_k_slot<N>(r, 4 * c + g)];
             const f8_u32x4 lo = f8_operand<C>(x[0], x[1]), hi = f8_operand<C>(x[2], x[3]);
 #pragma unroll
-            for (int p = 0; p < QP; ++p) {
-              s[u] = f8_mfma(lo, q[p][2 * c], s[u]);
-              s[u] = f8_mfma(hi, q[p][2 * c + 1], s[u]);
+            for (int part = 0; part < QP; ++part) {
+              s = f8_mfma(lo, q[part][2 * c], s);
+              s = f8_mfma(hi, q[part][2 * c + 1], s);
             }
           }
         } else {
           const char* at = reinterpret_cast<const char*>(&w.k[r * N + f8_k_slot<N>(r, g >> 1)]) + 8 * (g & 1);
           const uint2 x = *reinterpret_cast<const uint2*>(at);
 #pragma unroll
-          for (int p = 0; p < QP; ++p) s[u] = f8_mfma(f8_operand<C>(x.x, x.y), q[p][0], s[u]);
+          for (int part = 0; part < QP; ++part) s = f8_mfma(f8_operand<C>(x.x, x.y), q[part][0], s);
         }
-      }
-      // weights of rows 4g + i and 16 + 4g + i
-      const uint32_t word = (uint32_t)(seen[d * kF8Tile / kWave] >> (d * kF8Tile % kWave));
-      float p[8], top = m;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
         const f8_f32x4 scale = *reinterpret_cast<const f8_f32x4*>(&w.ks[d * kF8Tile + 16 * u + 4 * g]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[4 * u + i] = word >> (16 * u + 4 * g + i) & 1 ? s[u][i] * scale[i] : -INFINITY;
-          top = fmaxf(top, p[4 * u + i]);
+          const float score = word >> (16 * u + 4 * g + i) & 1 ? s[i] * scale[i] : -INFINITY;
+          p[d][4 * u + i] = score;
+          top = fmaxf(top, score);
         }
       }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
-      m = top;
-      l *= alpha;
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = top;
+    l *= alpha;
+    if (round > 0 && __ballot(alpha != 1.f) != 0) {
+#pragma unroll
+      for (int t = 0; t < N; ++t) acc[t] *= alpha;
+    }
+    f8_u32x4 weights[DEPTH][PP];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const f8_f32x4 scale = *reinterpret_cast<const f8_f32x4*>(&w.vs[d * kF8Tile + 16 * u + 4 * g]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(p[4 * u + i] - ref);
+          const float e = __builtin_amdgcn_exp2f(p[d][4 * u + i] - ref);
           l += e;
-          p[4 * u + i] = e * scale[i];
+          p[d][4 * u + i] = e * scale[i];
         }
       }
-      f8_u32x4 weights[PP];
-      f8_split<PP>(p, weights);
-      if (__ballot(alpha != 1.f) != 0) {
+      f8_split<PP>(p[d], weights[d]);
+    }
+    const int vr = (n >> 1 & 3) + 4 * g + (n >> 3) * 16;  // the row that this lane names for a transposing read
 #pragma unroll
-        for (int t = 0; t < N; ++t) acc[t] *= alpha;
+    for (int d = 0; d < DEPTH; ++d) {
+      f8_order();
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int r = i * RI + lane / N;
+        w.v[r * N + f8_v_slot<N>(r, lane % N)] = v[d][i];
       }
-      const int vr = (n >> 1 & 3) + 4 * g + (n >> 3) * 16;  // the row that this lane names for a transposing read
+      f8_order();
 #pragma unroll
       for (int t = 0; t < N; ++t) {
         const char* at = reinterpret_cast<const char*>(&w.v[vr * N + f8_v_slot<N>(vr, t)]) + 8 * (n & 1);
@@ -421,7 +427,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
             (__attribute__((address_space(3))) f8_i32x2*)const_cast<char*>(at));
         const f8_u32x4 values = f8_operand<C>((uint32_t)x.x, (uint32_t)x.y);
 #pragma unroll
-        for (int pp = 0; pp < PP; ++pp) acc[t] = f8_mfma(values, weights[pp], acc[t]);
+        for (int part = 0; part < PP; ++part) acc[t] = f8_mfma(values, weights[d][part], acc[t]);
       }
     }
     f8_order();
@@ -546,6 +552,39 @@ __global__ __launch_bounds__(kJ8Threads) void attend8_join_kernel(Attend8Args a,
     }
     __syncthreads();
   }
+}
+
+// Few splits of heads of a multiple of four dims: a thread per four dims, every load in flight at once.
+template <int SPLITS>
+__global__ __launch_bounds__(kJ8Threads) void attend8_join_few_kernel(Attend8Args a, FastDiv quads) {
+  const uint32_t heads = (uint32_t)(a.batch * a.q_heads), x = blockIdx.x * kJ8Threads + threadIdx.x;
+  const uint32_t item = quads.div(x);
+  if (item >= heads) return;
+  const uint32_t d = 4 * (x - item * quads.d);
+  float m[SPLITS], l[SPLITS], top = -INFINITY, total = 0.f;
+  f8_f32x4 v[SPLITS], o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < SPLITS; ++s) {  // (past the last one the last again, with no weight)
+    const int64_t at = (int64_t)min(s, a.n_splits - 1) * heads + item;
+    const f8_f32x2 st = *(const NHS_GLOBAL f8_f32x2*)to_global(a.stats + 2 * at);
+    m[s] = s < a.n_splits ? st[0] : -INFINITY;
+    l[s] = st[1];
+    v[s] = *(const NHS_GLOBAL f8_f32x4*)to_global(a.partial + at * a.head_dim + d);
+  }
+#pragma unroll
+  for (int s = 0; s < SPLITS; ++s) top = fmaxf(top, m[s]);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int s = 0; s < SPLITS; ++s) {
+    const float f = s < a.n_splits ? __builtin_amdgcn_exp2f(m[s] - ref) : 0.f;
+    total = __builtin_fmaf(l[s], f, total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = s < a.n_splits ? __builtin_fmaf(v[s][e], f, o[e]) : o[e];
+  }
+  const uint32_t b = item / a.q_heads, h = item - b * a.q_heads;
+  const int64_t at = (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_elem(a.out, a.q_dtype, at + e, total != 0.f ? o[e] / total : 0.f);
 }
 
 // ---- host --------------------------------------------------------------------------------
@@ -717,7 +756,14 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
     else
       wide(E4M3());
   }
-  if (join) {
+  if (join && plan.splits <= 8 && head_dim % 4 == 0 && heads * (head_dim / 4) < (1ll << 31)) {
+    const FastDiv quads((uint32_t)(head_dim / 4));
+    const dim3 grid((unsigned)((heads * (head_dim / 4) + kJ8Threads - 1) / kJ8Threads));
+    launch(plan.splits <= 2   ? attend8_join_few_kernel<2>
+           : plan.splits <= 4 ? attend8_join_few_kernel<4>
+                              : attend8_join_few_kernel<8>,
+           grid, dim3(kJ8Threads), 0, s, nullptr, ev.stop, a, quads);
+  } else if (join) {
     int quads = 1;
     while (quads * 4 < head_dim && quads < kJ8Threads) quads *= 2;
     launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kJ8Threads), 0, s, nullptr, ev.stop, a, quads);
