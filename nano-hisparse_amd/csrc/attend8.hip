@@ -482,109 +482,72 @@ constexpr int kA8MaxSplits = 64;  // (one lane of the joining waves each)
 
 // ---- joining the splits ------------------------------------------------------------------
 
-// A workgroup per (request, query head): a thread takes four dims (D / 4
-// rounded up to a power of two threads) of every shares-th split, and the
-// shares are added through LDS. One wave that walked 32 splits took 29.8 us
-// for 32 heads of 128.
-constexpr int kJ8Threads = 256;
+// Heads of a multiple of four dims: a thread takes four dims of every parts-th
+// split, up to 8 of them and all their loads in flight at once; the parts of a
+// sum are lanes of one wave. (One wave per head that walked its 32 splits took
+// 29.8 us for 32 heads of 128.)
+constexpr int kJ8Threads = 256, kJ8Each = 8;
 
-__global__ __launch_bounds__(kJ8Threads) void attend8_join_kernel(Attend8Args a, int quads) {
-  __shared__ float sums[kJ8Threads][4];
-  __shared__ float weights[kA8MaxSplits];
+template <int EACH>
+__global__ __launch_bounds__(kJ8Threads) void attend8_join_kernel(Attend8Args a, FastDiv quads, int parts) {
+  const uint32_t heads = (uint32_t)(a.batch * a.q_heads), lane = threadIdx.x & 63, span = kWave / parts;
+  const uint32_t part = lane / span, wave = blockIdx.x * (kJ8Threads / kWave) + (threadIdx.x >> 6);
+  const uint32_t x = min(wave * span + lane % span, heads * quads.d - 1), item = quads.div(x);
+  const uint32_t d = 4 * (x - item * quads.d);
+  float m[EACH], l[EACH], top = -INFINITY, total = 0.f;
+  f8_f32x4 v[EACH], o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {  // (past the last split that one again, without a weight)
+    const int s = (int)part + i * parts;
+    const int64_t at = (int64_t)min(s, a.n_splits - 1) * heads + item;
+    const f8_f32x2 st = *(const NHS_GLOBAL f8_f32x2*)to_global(a.stats + 2 * at);
+    m[i] = s < a.n_splits ? st[0] : -INFINITY;
+    l[i] = st[1];
+    v[i] = *(const NHS_GLOBAL f8_f32x4*)to_global(a.partial + at * a.head_dim + d);
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) top = fmaxf(top, m[i]);
+  for (uint32_t step = span; step < kWave; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const bool there = (int)part + i * parts < a.n_splits;
+    const float f = there ? __builtin_amdgcn_exp2f(m[i] - ref) : 0.f;
+    total = there ? __builtin_fmaf(l[i], f, total) : total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = there ? __builtin_fmaf(v[i][e], f, o[e]) : o[e];
+  }
+  for (uint32_t step = span; step < kWave; step *= 2) {
+    total += __shfl_xor(total, step);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], step);
+  }
+  if (part || wave * span + lane >= heads * quads.d) return;
+  const uint32_t b = item / a.q_heads, h = item - b * a.q_heads;
+  const int64_t at = (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_elem(a.out, a.q_dtype, at + e, total != 0.f ? o[e] / total : 0.f);
+}
+
+// Other heads: a wave per (request, query head).
+__global__ __launch_bounds__(kWave) void attend8_join_any_kernel(Attend8Args a) {
   const int64_t heads = (int64_t)a.batch * a.q_heads;
-  const int item = blockIdx.x, tid = threadIdx.x, D = a.head_dim;
-  const int b = item / a.q_heads, h = item - b * a.q_heads;
-  const int quad = tid & (quads - 1), share = tid / quads, shares = kJ8Threads / quads;
-  // the first partial sums of a thread are asked for beside the statistics
-  const bool wide = D % 4 == 0;
-  const auto load = [&](int s, int d, float (&v)[4]) {
-    const float* p = a.partial + (s * heads + item) * D + d;
-    if (wide) {
-      const f8_f32x4 x = *reinterpret_cast<const f8_f32x4*>(p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = x[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = p[min(e, D - 1 - d)];
-    }
-  };
-  constexpr int kAhead = 4;
-  float ahead[kAhead][4];
-  const int d0 = min(4 * quad, (D - 1) / 4 * 4);
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(min(share + i * shares, a.n_splits - 1), d0, ahead[i]);
-  const int lane = tid & 63;  // every wave reduces the statistics of up to 64 splits
+  const int item = blockIdx.x, lane = threadIdx.x, D = a.head_dim;
   const float* st = a.stats + 2 * ((int64_t)min(lane, a.n_splits - 1) * heads + item);
   const float m = lane < a.n_splits ? st[0] : -INFINITY, l = lane < a.n_splits ? st[1] : 0.f;
   float top = m;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m - ref);
+  const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
   const float total = wave_sum(l * f);
-  if (tid < a.n_splits) weights[tid] = f;
-  __syncthreads();
-  for (int d = 4 * quad; d < (D + 4 * quads - 1) / (4 * quads) * (4 * quads); d += 4 * quads) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
-    if (d < D)
-      for (int s = share, i = 0; s < a.n_splits; s += shares, ++i) {
-        float v[4];
-        if (d == 4 * quad && i < kAhead) {
-#pragma unroll
-          for (int x = 0; x < kAhead; ++x)
-            if (i == x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = ahead[x][e];
-        } else {
-          load(s, d, v);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], weights[s], o[e]);
-      }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sums[tid][e] = o[e];
-    __syncthreads();
-    if (share == 0 && d < D) {
-      for (int x = 1; x < shares; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += sums[x * quads + quad][e];
-      for (int e = 0; e < 4 && d + e < D; ++e)
-        store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d + e, total != 0.f ? o[e] / total : 0.f);
-    }
-    __syncthreads();
+  const int b = item / a.q_heads, h = item - b * a.q_heads;
+  for (int d0 = 0; d0 < D; d0 += kWave) {
+    const int d = min(d0 + lane, D - 1);
+    float o = 0.f;
+    for (int s = 0; s < a.n_splits; ++s) o = __builtin_fmaf(a.partial[(s * heads + item) * D + d], __shfl(f, s), o);
+    if (d0 + lane < D)
+      store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d, total != 0.f ? o / total : 0.f);
   }
-}
-
-// Few splits of heads of a multiple of four dims: a thread per four dims, every load in flight at once.
-template <int SPLITS>
-__global__ __launch_bounds__(kJ8Threads) void attend8_join_few_kernel(Attend8Args a, FastDiv quads) {
-  const uint32_t heads = (uint32_t)(a.batch * a.q_heads), x = blockIdx.x * kJ8Threads + threadIdx.x;
-  const uint32_t item = quads.div(x);
-  if (item >= heads) return;
-  const uint32_t d = 4 * (x - item * quads.d);
-  float m[SPLITS], l[SPLITS], top = -INFINITY, total = 0.f;
-  f8_f32x4 v[SPLITS], o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int s = 0; s < SPLITS; ++s) {  // (past the last one the last again, with no weight)
-    const int64_t at = (int64_t)min(s, a.n_splits - 1) * heads + item;
-    const f8_f32x2 st = *(const NHS_GLOBAL f8_f32x2*)to_global(a.stats + 2 * at);
-    m[s] = s < a.n_splits ? st[0] : -INFINITY;
-    l[s] = st[1];
-    v[s] = *(const NHS_GLOBAL f8_f32x4*)to_global(a.partial + at * a.head_dim + d);
-  }
-#pragma unroll
-  for (int s = 0; s < SPLITS; ++s) top = fmaxf(top, m[s]);
-  const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-  for (int s = 0; s < SPLITS; ++s) {
-    const float f = s < a.n_splits ? __builtin_amdgcn_exp2f(m[s] - ref) : 0.f;
-    total = __builtin_fmaf(l[s], f, total);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = s < a.n_splits ? __builtin_fmaf(v[s][e], f, o[e]) : o[e];
-  }
-  const uint32_t b = item / a.q_heads, h = item - b * a.q_heads;
-  const int64_t at = (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) store_elem(a.out, a.q_dtype, at + e, total != 0.f ? o[e] / total : 0.f);
 }
 
 // ---- host --------------------------------------------------------------------------------
@@ -756,17 +719,17 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
     else
       wide(E4M3());
   }
-  if (join && plan.splits <= 8 && head_dim % 4 == 0 && heads * (head_dim / 4) < (1ll << 31)) {
-    const FastDiv quads((uint32_t)(head_dim / 4));
-    const dim3 grid((unsigned)((heads * (head_dim / 4) + kJ8Threads - 1) / kJ8Threads));
-    launch(plan.splits <= 2   ? attend8_join_few_kernel<2>
-           : plan.splits <= 4 ? attend8_join_few_kernel<4>
-                              : attend8_join_few_kernel<8>,
-           grid, dim3(kJ8Threads), 0, s, nullptr, ev.stop, a, quads);
+  if (join && head_dim % 4 == 0 && heads * head_dim < (1ll << 31)) {
+    int parts = 1;
+    while (parts * kJ8Each < plan.splits) parts *= 2;
+    const int64_t per_group = kJ8Threads / parts, threads = heads * (head_dim / 4);
+    launch(plan.splits <= 2   ? attend8_join_kernel<2>
+           : plan.splits <= 4 ? attend8_join_kernel<4>
+                              : attend8_join_kernel<kJ8Each>,
+           dim3((unsigned)((threads + per_group - 1) / per_group)), dim3(kJ8Threads), 0, s, nullptr, ev.stop, a,
+           FastDiv((uint32_t)(head_dim / 4)), parts);
   } else if (join) {
-    int quads = 1;
-    while (quads * 4 < head_dim && quads < kJ8Threads) quads *= 2;
-    launch(attend8_join_kernel, dim3((unsigned)heads), dim3(kJ8Threads), 0, s, nullptr, ev.stop, a, quads);
+    launch(attend8_join_any_kernel, dim3((unsigned)heads), dim3(kWave), 0, s, nullptr, ev.stop, a);
   }
   return launch_status("nhs_attend_rows8");
 }
