@@ -187,14 +187,15 @@ __global__ __launch_bounds__(kA8Threads) void append8_items_kernel(Append8ItemsA
 // written yet), hold 64 rows of codes and keys in LDS and walk them, a thread
 // per element and share of the rows.
 constexpr int kFold8Rows = 64;
+constexpr int kR8Threads = 512, kR8Waves = kR8Threads / kWave;
 
 template <typename T, int N>
 struct Fold8 {
   uint32_t codes[kFold8Rows * N * 4];
   std::conditional_t<T::bytes == 4, float, uint16_t> keys[kFold8Rows * N * 16];
   float scales[kFold8Rows];
-  double sums[kA8Threads];
-  float low[kA8Threads], high[kA8Threads];
+  double sums[kR8Threads];
+  float low[kR8Threads], high[kR8Threads];
 };
 
 // 16 elements of one lane as they lie, and as fp32
@@ -267,7 +268,7 @@ __device__ __forceinline__ void copy8(const Append8Args& a, int unit, int groups
 
 template <typename T, typename C, int N>
 __device__ __forceinline__ void fold8(const Append8Args& a, int head) {
-  constexpr int D = N * 16, kParts = kA8Threads / D, kRowsPerPass = kA8Threads / N;
+  constexpr int D = N * 16, kParts = kR8Threads / D, kRowsPerPass = kR8Threads / N;
   constexpr int kPasses = (kFold8Rows + kRowsPerPass - 1) / kRowsPerPass;
   __shared__ __attribute__((aligned(16))) Fold8<T, N> s;
   const int tid = threadIdx.x, chunk = tid % N, slot = tid / N;
@@ -344,22 +345,22 @@ __device__ __forceinline__ void append8_rows(const Append8Args& a) {
   const int group = blockIdx.x;
   if (group < a.form.kv_heads) return fold8<T, C, N>(a, group);
   const int groups = (a.form.kv_heads * N + kWave - 1) / kWave;
-  copy8<T, C, N>(a, (group - a.form.kv_heads) * kA8Waves + ((int)threadIdx.x >> 6), groups);
+  copy8<T, C, N>(a, (group - a.form.kv_heads) * kR8Waves + ((int)threadIdx.x >> 6), groups);
 }
 
 // Workgroups of a launch for `count` rows.
 static unsigned rows8_grid(const Row8& form, int count) {
   const int64_t groups = ((int64_t)form.kv_heads * (form.head_dim / 16) + kWave - 1) / kWave;
-  return (unsigned)(form.kv_heads + (2 * count * groups + kA8Waves - 1) / kA8Waves);
+  return (unsigned)(form.kv_heads + (2 * count * groups + kR8Waves - 1) / kR8Waves);
 }
 
 template <typename T, typename C, int N>
-__global__ __launch_bounds__(kA8Threads) void append8_rows_kernel(Append8Args a) {
+__global__ __launch_bounds__(kR8Threads) void append8_rows_kernel(Append8Args a) {
   append8_rows<T, C, N>(a);
 }
 
 template <typename T, typename C, int N>
-__global__ __launch_bounds__(kA8Threads) void append8_item_rows_kernel(Append8ItemsArgs g) {
+__global__ __launch_bounds__(kR8Threads) void append8_item_rows_kernel(Append8ItemsArgs g) {
   Append8Args a;
   if (item8<T>(g, blockIdx.y, &a)) append8_rows<T, C, N>(a);
 }
@@ -567,7 +568,7 @@ extern "C" int nhs_append_page8(const void* k, const void* v, int64_t token_stri
     const dim3 grid(rows8_grid(a.form, count));
     with_types(kv_dtype, code, [&](auto t, auto c) {
       with_chunks(head_dim, [&](auto n) {
-        launch(append8_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kA8Threads), 0,
+        launch(append8_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kR8Threads), 0,
                (hipStream_t)stream, ev.start, ev.stop, a);
       });
     });
@@ -613,7 +614,7 @@ extern "C" int nhs_append_items8(int32_t batch, const void* k, const void* v, in
     const dim3 grid(rows8_grid(g.a.form, 1), (unsigned)batch);
     with_types(kv_dtype, code, [&](auto t, auto c) {
       with_chunks(head_dim, [&](auto n) {
-        launch(append8_item_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kA8Threads), 0,
+        launch(append8_item_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kR8Threads), 0,
                (hipStream_t)stream, ev.start, ev.stop, g);
       });
     });

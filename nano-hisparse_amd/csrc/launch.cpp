@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cstring>
 #include <new>
 #include <stdexcept>
 #include <utility>
@@ -741,30 +742,163 @@ PyObject* read_rows_8bit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
-// ---- append ------------------------------------------------------------------------------------
-
-// Whole numbers of any integer type; negative ones go to the library, which refuses them.
-template <int N>
-bool whole_numbers(PyObject* const* a, Py_ssize_t nargs, int64_t (&v)[N]) {
-  if (nargs != N) {
-    PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
-    return false;
+// A pinned host store [pages, 2, P, row_bytes] like the pool's blocks, given as a row_kernels.MappedHost or None.
+struct Host8 {
+  void* alias = nullptr;
+  int64_t pages = 0;
+};
+Host8 host8_of(PyObject* o, const Tensor& pool) {
+  Host8 h;
+  if (o == Py_None) return h;
+  PyObject *held = PyObject_GetAttrString(o, "tensor"), *pointer = PyObject_GetAttrString(o, "pointer");
+  bool ok = held && pointer && THPVariable_Check(held) && PyLong_CheckExact(pointer);
+  if (ok) {
+    const Tensor& t = THPVariable_Unpack(held);
+    ok = t.scalar_type() == at::kByte && t.dim() == 4 && t.is_contiguous() && t.sizes().slice(1) == pool.sizes().slice(1);
+    h.alias = PyLong_AsVoidPtr(pointer);
+    h.pages = t.size(0);
   }
-  for (int i = 0; i < N; ++i) {
-    PyObject* whole = PyNumber_Index(a[i]);
-    if (!whole) return false;
-    v[i] = (int64_t)PyLong_AsUnsignedLongLongMask(whole);
-    Py_DECREF(whole);
-    if (PyErr_Occurred()) return false;
+  Py_XDECREF(held);
+  Py_XDECREF(pointer);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    ok = false;
   }
-  return true;
+  need(ok && h.alias);
+  return h;
 }
 
-// nhs_append_page and nhs_append_page8 with the arguments that row_kernels.PageAppender prepared (checked there);
-// they return the status.
+// Checks k and v [tokens, Hkv, D] for appends; returns the elements between tokens.
+int64_t check_append8(const Tensor& k, const Tensor& v, const Tensor& pool, const Form& f) {
+  on_gpu(k, 3, pool);
+  on_gpu(v, 3, pool);
+  const int64_t width = (int64_t)f.kv_heads * f.head_dim, stride = k.size(0) > 1 ? k.stride(0) : width;
+  need(k.size(1) == f.kv_heads && k.size(2) == f.head_dim && same_sizes(v, k.sizes()) &&
+       v.scalar_type() == k.scalar_type() && contiguous_from(k, 1) && contiguous_from(v, 1) && stride >= width &&
+       (k.size(0) == 1 || v.stride(0) == stride));
+  return stride;
+}
+
+PyObject* append_items_8bit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 7, [&]() -> PyObject* {
+    const Tensor &k = tensor(a[0]), &v = tensor(a[1]), &pool = tensor(a[2]), &items = tensor(a[5]),
+                 &lengths = tensor(a[6]);
+    const Form f = form_of(a[3]);
+    on_gpu(pool, 4);
+    const int64_t token = check_append8(k, v, pool, f), stride = pool8_block_stride(pool, f), B = k.size(0);
+    on_gpu(items, 2, pool);
+    on_gpu(lengths, 1, pool);
+    need(items.scalar_type() == at::kLong && items.size(0) == B && items.size(1) == 9 && items.is_contiguous() &&
+         lengths.scalar_type() == at::kLong && lengths.size(0) == B && lengths.is_contiguous());
+    const Host8 host = host8_of(a[4], pool);
+    const int code = dtype_code(k);
+    int st;
+    {
+      NoGil free;
+      const OnDevice on(pool);
+      st = nhs_append_items8((int32_t)B, k.data_ptr(), v.data_ptr(), token, code, f.code, f.kv_heads, f.head_dim,
+                             (int32_t)pool.size(2), pool.data_ptr(), stride, host.alias,
+                             static_cast<const nhs_layer_item*>(items.data_ptr()),
+                             static_cast<const int64_t*>(lengths.data_ptr()), stream_of(pool));
+    }
+    if (st) return failed("nhs_append_items8", st);
+    Py_RETURN_TRUE;
+  });
+}
+
+// What row_kernels.PageAppender keeps of a write into rows in 8 bits, as bytes; page8 makes one page's call of it.
+struct Write8 {
+  const char *k, *v;
+  char *pool, *host, *summary, *minimum, *maximum;
+  void* stream;
+  int64_t token, stride, tokens, blocks, host_pages, bounds, esize;
+  int32_t dtype, code, kv_heads, head_dim, page_size, device;
+};
+
+PyObject* write8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 8, [&]() -> PyObject* {
+    const Tensor &k = tensor(a[0]), &v = tensor(a[1]), &pool = tensor(a[2]);
+    const Form f = form_of(a[3]);
+    on_gpu(pool, 4);
+    Write8 w;
+    w.token = check_append8(k, v, pool, f);
+    w.stride = pool8_block_stride(pool, f);
+    const Host8 host = host8_of(a[4], pool);
+    w.bounds = INT64_MAX;
+    void* pointers[3];
+    for (int i = 0; i < 3; ++i) {
+      const Tensor& t = tensor(a[5 + i]);
+      need(t.is_cuda() && t.device() == pool.device() && t.numel() > 0 && t.dim() >= 2 && t.is_contiguous() &&
+           t.size(-2) == f.kv_heads && t.size(-1) == f.head_dim &&
+           t.scalar_type() == (i == 0 ? at::kFloat : k.scalar_type()));
+      pointers[i] = t.data_ptr();
+      w.bounds = std::min(w.bounds, t.numel() / ((int64_t)f.kv_heads * f.head_dim));
+    }
+    w.k = static_cast<const char*>(k.data_ptr());
+    w.v = static_cast<const char*>(v.data_ptr());
+    w.pool = static_cast<char*>(pool.data_ptr());
+    w.host = static_cast<char*>(host.alias);
+    w.summary = static_cast<char*>(pointers[0]);
+    w.minimum = static_cast<char*>(pointers[1]);
+    w.maximum = static_cast<char*>(pointers[2]);
+    w.stream = stream_of(pool);
+    w.tokens = k.size(0);
+    w.blocks = pool.size(0);
+    w.host_pages = host.pages;
+    w.esize = k.element_size();
+    w.dtype = dtype_code(k);
+    w.code = f.code;
+    w.kv_heads = f.kv_heads;
+    w.head_dim = f.head_dim;
+    w.page_size = (int32_t)pool.size(2);
+    w.device = pool.device().index();
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&w), sizeof w);
+  });
+}
+
+// page8(write, first, count, block, within, host_page, bounds_index) -> the library's status, or None where an index
+// is outside the write's tensors.
+PyObject* page8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return native(nargs, 7, [&]() -> PyObject* {
+    need(PyBytes_CheckExact(a[0]) && PyBytes_GET_SIZE(a[0]) == sizeof(Write8));
+    Write8 w;
+    memcpy(&w, PyBytes_AS_STRING(a[0]), sizeof w);
+    const int64_t first = integer(a[1]), count = integer(a[2]), block = integer(a[3]), within = integer(a[4]),
+                  host_page = integer(a[5]), at = integer(a[6]);
+    need(first >= 0 && count >= 1 && count <= w.tokens && first <= w.tokens - count && block >= 0 && block < w.blocks &&
+         within >= 0 && within <= w.page_size && count <= w.page_size && at >= 0 && at < w.bounds &&
+         (!w.host || (host_page >= 0 && host_page < w.host_pages)));
+    const int64_t width = (int64_t)w.kv_heads * w.head_dim, row = first * w.token * w.esize;
+    int st;
+    {
+      NoGil free;
+      const c10::OptionalDeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)w.device));
+      st = nhs_append_page8(w.k + row, w.v + row, w.token, w.dtype, w.code, w.kv_heads, w.head_dim, w.page_size, w.pool,
+                            w.stride, block, (int32_t)within, (int32_t)count, w.host, w.host ? host_page : 0,
+                            reinterpret_cast<float*>(w.summary) + at * width, w.minimum + at * width * w.esize,
+                            w.maximum + at * width * w.esize, w.stream);
+    }
+    return PyLong_FromLong(st);
+  });
+}
+
+// ---- append ------------------------------------------------------------------------------------
+
+// nhs_append_page with the arguments row_kernels.PageAppender prepared (checked there), as whole numbers of any integer
+// type; returns the status.
 PyObject* append_page(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != 17) {
+    PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
+    return nullptr;
+  }
   int64_t v[17];
-  if (!whole_numbers(a, nargs, v)) return nullptr;
+  for (int i = 0; i < 17; ++i) {  // negative numbers go to the library, which refuses them
+    PyObject* whole = PyNumber_Index(a[i]);
+    if (!whole) return nullptr;
+    v[i] = (int64_t)PyLong_AsUnsignedLongLongMask(whole);
+    Py_DECREF(whole);
+    if (PyErr_Occurred()) return nullptr;
+  }
   const auto at = [&](int i) { return reinterpret_cast<void*>((uintptr_t)v[i]); };
   int st;
   {
@@ -772,20 +906,6 @@ PyObject* append_page(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     st = nhs_append_page(at(0), at(1), v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], at(6), v[7], v[8],
                          (int32_t)v[9], (int32_t)v[10], at(11), v[12], static_cast<float*>(at(13)), at(14), at(15),
                          at(16));
-  }
-  return PyLong_FromLong(st);
-}
-
-PyObject* append_page8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-  int64_t v[19];
-  if (!whole_numbers(a, nargs, v)) return nullptr;
-  const auto at = [&](int i) { return reinterpret_cast<void*>((uintptr_t)v[i]); };
-  int st;
-  {
-    NoGil free;
-    st = nhs_append_page8(at(0), at(1), v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], (int32_t)v[6],
-                          (int32_t)v[7], at(8), v[9], v[10], (int32_t)v[11], (int32_t)v[12], at(13), v[14],
-                          static_cast<float*>(at(15)), at(16), at(17), at(18));
   }
   return PyLong_FromLong(st);
 }
@@ -848,7 +968,8 @@ PyMethodDef methods[] = {NHS_METHOD(linear_small_m), NHS_METHOD(linear_silu_mul)
                          NHS_METHOD(quest_batched),  NHS_METHOD(select_resolve_batched),
                          NHS_METHOD(append_page),    NHS_METHOD(held_state),        NHS_METHOD(tree_plan),
                          NHS_METHOD(tree_attention), NHS_METHOD(qk_norm_rope),      NHS_METHOD(token_logprobs),
-                         NHS_METHOD(attend_8bit),    NHS_METHOD(read_rows_8bit),    NHS_METHOD(append_page8),
+                         NHS_METHOD(attend_8bit),    NHS_METHOD(read_rows_8bit),    NHS_METHOD(append_items_8bit),
+                         NHS_METHOD(write8),         NHS_METHOD(page8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

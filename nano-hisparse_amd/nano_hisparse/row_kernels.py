@@ -357,6 +357,8 @@ def append_items_8bit(k, v, pool, form, host, items, lengths):
     """append_items into a pool of rows in 8 bits: one token per item, k/v
     [B, Hkv, D], appended at lengths[b] of each item's layer. An item whose
     page is not bound is left alone."""
+    if k.is_cuda and (_launch or _load_launch()).append_items_8bit(k, v, pool, form, host, items, lengths):
+        return
     token_stride = _check_append8("append_items_8bit", k, v, pool, form, host, (), ())
     device, B = k.device, len(k)
     if items.shape[0] != B or items.dtype != torch.int64 or lengths.shape != (B,) or lengths.dtype != torch.int64 \
@@ -514,22 +516,21 @@ class PageAppender:
     def __init__(self, k, v, pool, host, summaries, minimum, maximum, form=None):
         """form (Rows8): the pool and the host store hold rows in 8 bits (append_page_8bit)."""
         launch = _launch or _load_launch()
-        if form is not None:
-            self.token_stride = _check_append8("append_page", k, v, pool, form, host, (summaries,), (minimum, maximum))
-            self.append_page = launch.append_page8
-            shape = (_CODES[form.code], form.kv_heads, form.head_dim)
-            self.limits = (pool.shape[0], len(host.tensor) if host is not None else 1,
-                           min(t.shape[:-2].numel() for t in (summaries, minimum, maximum)))
-        else:
-            self._check(k, v, pool, host, summaries, minimum, maximum)
-            self.token_stride = k.stride(0)
-            self.append_page = launch.append_page
-            shape = (k.shape[1] * k.shape[2],)
-            self.limits = None
         self.k, self.v = k, v  # held for the write
+        self.form = form
+        if form is not None:
+            self.held = pool, host, summaries, minimum, maximum
+            self.page8 = launch.page8
+            self.write = launch.write8(k, v, pool, form, host, summaries, minimum, maximum)
+            if self.write is None:  # the checks in words, and forms of a call that the native ones leave to Python
+                _check_append8("append_page", k, v, pool, form, host, (summaries,), (minimum, maximum))
+            return
+        self._check(k, v, pool, host, summaries, minimum, maximum)
+        self.append_page = launch.append_page
         self.esize = k.element_size()
-        self.k_ptr, self.v_ptr = k.data_ptr(), v.data_ptr()
-        self.row_elems, self.shape = k.shape[1] * k.shape[2], (dtype_code(k.dtype), *shape, pool.shape[2])
+        self.k_ptr, self.v_ptr, self.token_stride = k.data_ptr(), v.data_ptr(), k.stride(0)
+        self.row_elems = k.shape[1] * k.shape[2]
+        self.dtype, self.page_size = dtype_code(pool.dtype), pool.shape[2]
         self.pool_ptr, self.pool_stride = pool.data_ptr(), pool_block_stride(pool)
         self.host_ptr = host.data_ptr() if host is not None else 0
         self.sum_ptr, self.min_ptr, self.max_ptr = summaries.data_ptr(), minimum.data_ptr(), maximum.data_ptr()
@@ -557,19 +558,32 @@ class PageAppender:
         """Rows first..first+count-1 of the write into rows within.. of pool
         block `block` (and host block `host_page`); bounds_index is the
         page's index in the flattened [layers, pages] bounds."""
+        if self.form is not None:
+            return self._page8(first, count, block, within, host_page, bounds_index)
         if not (0 <= first and count >= 1 and first + count <= self.k.shape[0]):
             raise ValueError("append_page: rows outside the write")
-        if self.limits is not None and not (0 <= block < self.limits[0] and 0 <= bounds_index < self.limits[2]
-                                            and (not self.host_ptr or 0 <= host_page < self.limits[1])):
-            raise ValueError("append_page: page outside the pool, the host store or the bounds")
         off = bounds_index * self.row_elems
         row = first * self.token_stride * self.esize
         status = self.append_page(
-            self.k_ptr + row, self.v_ptr + row, self.token_stride, *self.shape, self.pool_ptr, self.pool_stride, block,
-            within, count, self.host_ptr, host_page if self.host_ptr else 0, self.sum_ptr + off * 4,
-            self.min_ptr + off * self.esize, self.max_ptr + off * self.esize, self.stream,
+            self.k_ptr + row, self.v_ptr + row, self.token_stride, self.dtype, self.row_elems, self.page_size,
+            self.pool_ptr, self.pool_stride, block, within, count, self.host_ptr, host_page if self.host_ptr else 0,
+            self.sum_ptr + off * 4, self.min_ptr + off * self.esize, self.max_ptr + off * self.esize, self.stream,
         )
         _hip.check(status, "nhs_append_page")
+
+    def _page8(self, first, count, block, within, host_page, bounds_index):
+        if self.write is not None:
+            status = self.page8(self.write, first, count, block, within, host_page, bounds_index)
+            if status is not None:
+                return _hip.check(status, "nhs_append_page8")
+        pool, host, *bounds = self.held
+        if not (0 <= first and count >= 1 and first + count <= len(self.k)):
+            raise ValueError("append_page: rows outside the write")
+        summary, low, high = (t.view(-1, *self.k.shape[1:]) for t in bounds)
+        if not 0 <= bounds_index < min(len(t) for t in (summary, low, high)):
+            raise ValueError("append_page: page outside the bounds")
+        append_page_8bit(self.k[first : first + count], self.v[first : first + count], pool, self.form, block, within,
+                         host, host_page, summary[bounds_index], low[bounds_index], high[bounds_index])
 
 
 # ---- attention ------------------------------------------------------------------
