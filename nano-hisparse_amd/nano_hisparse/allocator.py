@@ -1,7 +1,8 @@
 """Device blocks of the KV pool: ownership, reference counts and reuse.
 
 Reference: nano_hisparse/allocator.py:9-83. One pool tensor of
-[gpu_pages, 2, page_size, kv_heads, head_dim] holds resident pages and hot
+[gpu_pages, 2, page_size, kv_heads, head_dim] (rows in 8 bits:
+[gpu_pages, 2, page_size, row_bytes]) holds resident pages and hot
 blocks alike. A block bound to an owner carries one allocation reference;
 readers add temporary references. A block whose allocation reference was
 given up (unpinned) stays readable until it is reclaimed, which runs the
@@ -36,11 +37,14 @@ class DeviceSlot:
 
 class DeviceAllocator:
     def __init__(self, config):
-        from .row_kernels import padded_pool
+        from .row_kernels import padded_pool, pool_8bit
 
-        # on a GPU each block is followed by a few head slots of padding (padded_pool)
-        self.storage = padded_pool(config.gpu_pages, config.page_size, config.kv_heads, config.head_dim,
-                                   config.dtype, config.device)
+        if config.storage_dtype is not None:
+            self.storage = pool_8bit(config.gpu_pages, config.page_size, config.rows8, config.device)
+        else:
+            # on a GPU each block is followed by a few head slots of padding (padded_pool)
+            self.storage = padded_pool(config.gpu_pages, config.page_size, config.kv_heads, config.head_dim,
+                                       config.dtype, config.device)
         self.budget = config.gpu_pages
         self.slots = [DeviceSlot() for _ in range(config.gpu_pages)]
         self.free: set[int] = set(range(config.gpu_pages))

@@ -33,12 +33,16 @@ def row_attention(query, cache, request_id, layer, topk, backend="auto"):
         if rows.ndim == 1:
             rows = rows[None, :].expand(query.shape[0], -1)
         if cache.storage.cuda:
-            from .row_kernels import attend_rows
+            from . import row_kernels as kernels
+        else:
+            from .row_kernels import cpu_provider
 
-            return attend_rows(query, cache.pool, rows, cache.config)
-        from .row_kernels import cpu_provider
-
-        return cpu_provider("row_attention").attend_rows(query, cache.pool, rows, cache.config)
+            kernels = cpu_provider("row_attention")
+        form = cache.storage.rows8
+        if form is not None:
+            shared = rows.stride(0) == 0  # a stride-0 expansion of one list
+            return kernels.attend_8bit(query[None], cache.pool, form, (rows[0] if shared else rows)[None])[0]
+        return kernels.attend_rows(query, cache.pool, rows, cache.config)
 
 
 @torch.inference_mode()
@@ -61,11 +65,27 @@ def tree_row_attention(query, k, v, mask, cache, request_id, layer, topk, backen
     if backend == "triton" and not cache.storage.cuda:
         raise ValueError("Triton requires CUDA")
     with cache.resolve(request_id, layer, topk) as lease:
-        rows = lease.plan.physical_rows[None]
+        rows = lease.plan.physical_rows
         if cache.storage.cuda:
-            from .row_kernels import tree_attention
+            from . import row_kernels as kernels
         else:
             from .row_kernels import cpu_provider
 
-            tree_attention = cpu_provider("tree_row_attention").tree_attention
-        return tree_attention(query[None], cache.pool, rows, k[None], v[None], mask[None], cfg.page_size)[0]
+            kernels = cpu_provider("tree_row_attention")
+        pool, page_size = cache.pool, cfg.page_size
+        if cache.storage.rows8 is not None:
+            pool, rows, page_size, k, v = _read_for_tree(kernels, cache, rows, k, v)
+        return kernels.tree_attention(query[None], pool, rows[None], k[None], v[None], mask[None], page_size)[0]
+
+
+def _read_for_tree(kernels, cache, rows, k, v):
+    """What tree_attention takes of a cache whose rows are in 8 bits: the
+    selected rows read back as a pool of one page, and the drafted keys and
+    values rounded as the cache will round them when they are appended (a
+    token accepted from a draft then sees what it would have seen alone)."""
+    form, dtype = cache.storage.rows8, k.dtype
+    n = rows.numel()
+    pool = torch.empty(1, 2, n, form.kv_heads, form.head_dim, dtype=dtype, device=k.device)
+    kernels.read_rows_8bit(cache.pool, form, rows, dtype, out=(pool[0, 0], pool[0, 1]))
+    own = torch.where(rows >= 0, torch.arange(n, device=rows.device), -1)
+    return pool, own, n, *kernels.round_8bit(k, v, form)

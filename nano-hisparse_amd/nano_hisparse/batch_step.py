@@ -66,19 +66,20 @@ class SparseDecodeBatch:
     host-row gather -> GQA row attention.
 
     pool: the device KV pool [blocks, 2, P, Hkv, D]; host: the pinned host
-    store of the same page shape. Tensors live on one GPU. chunks: request
+    store of the same page shape. form (row_kernels.Rows8): both hold rows in
+    8 bits, [blocks, 2, P, row_bytes] uint8. Tensors live on one GPU. chunks: request
     groups whose gathers and attentions are pipelined. transfer: the stream
     of the gathers (default: the compute stream for one chunk, a new side
     stream for several).
     """
 
     def __init__(self, pool, host, tables: BatchTables, page_size, top_pages, keep_sink=True, chunks=1,
-                 compute=None, transfer=None):
+                 compute=None, transfer=None, form=None):
         if pool.device.type != "cuda":
             raise ValueError("SparseDecodeBatch runs on a GPU")
         if not 1 <= chunks <= tables.batch:
             raise ValueError("chunks must be between 1 and the batch size")
-        self.pool, self.tables, self.page_size = pool, tables, page_size
+        self.pool, self.tables, self.page_size, self.form = pool, tables, page_size, form
         self.top_pages, self.keep_sink = top_pages, keep_sink
         self.alias = rk.MappedHost(host)
         device = pool.device
@@ -103,6 +104,9 @@ class SparseDecodeBatch:
         }
 
     def _attend(self, query, physical, out):
+        if self.form is not None:
+            rk.attend_8bit(query, self.pool, self.form, physical, out=out)
+            return
         lib = rk._hip.load()
         B, Hq, D = query.shape
         need = lib.nhs_attend_workspace_bytes(B, Hq, D, physical.shape[-1])

@@ -145,7 +145,10 @@ class BatchDecode:
             raise ValueError("K/V dtype/device must match the cache")
         if not (k[0].is_contiguous() and v[0].is_contiguous() and k.stride() == v.stride()):
             k, v = k.contiguous(), v.contiguous()  # rows may be views of a fused projection
-        rk.append_items(k, v, cache.pool, store.host_alias, self.items[layer], self.dev_lengths[0])
+        if store.rows8 is not None:
+            rk.append_items_8bit(k, v, cache.pool, store.rows8, store.host_alias, self.items[layer], self.dev_lengths[0])
+        else:
+            rk.append_items(k, v, cache.pool, store.host_alias, self.items[layer], self.dev_lengths[0])
         self._account_append(layer)
 
     def _account_append(self, layer):
@@ -170,6 +173,8 @@ class BatchDecode:
         captured step's workspace is read by every replay, beside whatever
         else runs with the capture stream's."""
         cfg = self.cache.config
+        if cfg.storage_dtype is not None:  # attend_8bit takes one for each call, from the capture's own memory
+            return
         need = rk._hip.load().nhs_attend_workspace_bytes(len(self.ids), q_heads, cfg.head_dim,
                                                          top_pages * cfg.page_size)
         self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.cache.device)
@@ -303,7 +308,10 @@ class BatchDecode:
         layer, query, physical, gathered = handle
         cache, store = self.cache, self.cache.storage
         store.wait(store.active_compute(), gathered)
-        out = rk.attend_batched(query, cache.pool, physical, cache.config.page_size, workspace=self.workspace)
+        if store.rows8 is not None:
+            out = rk.attend_8bit(query, cache.pool, store.rows8, physical)
+        else:
+            out = rk.attend_batched(query, cache.pool, physical, cache.config.page_size, workspace=self.workspace)
         self._attended.add(layer)
         return out
 

@@ -22,6 +22,11 @@ class CacheConfig:
     pool; host_pages blocks of the same shape make the host store.
     index_budget_bytes bounds the per-request index tensors (page bounds,
     summaries and the resolver tables) on the device.
+
+    dtype is that of the K and V given and of the queries. With storage_dtype
+    (torch.int8 or torch.float8_e4m3fn) pool and host store hold the rows in 8
+    bits, with an fp32 scale per token and KV head (row_kernels.Rows8): half
+    the bytes of a 16-bit row to keep, to gather and to attend over.
     """
 
     gpu_pages: int = 16
@@ -32,6 +37,7 @@ class CacheConfig:
     device: str = "cuda"
     dtype: torch.dtype = torch.float32
     index_budget_bytes: int = 64 * 1024 * 1024
+    storage_dtype: torch.dtype | None = None
 
     def __post_init__(self):
         for name in ("gpu_pages", "host_pages", "page_size", "kv_heads", "head_dim"):
@@ -41,8 +47,20 @@ class CacheConfig:
             raise ValueError("KV dtype must be float32, float16 or bfloat16")
         if self.index_budget_bytes < 1:
             raise ValueError("index budget must be positive")
+        if self.storage_dtype is not None:
+            self.rows8.check("storage dtype")
+
+    @property
+    def rows8(self):
+        """The form of a row held in 8 bits (row_kernels.Rows8), None where
+        rows are held in `dtype`."""
+        from .row_kernels import Rows8
+
+        return None if self.storage_dtype is None else Rows8(self.storage_dtype, self.kv_heads, self.head_dim)
 
     @property
     def row_bytes(self) -> int:
         """Bytes of one token row: K and V for every KV head."""
+        if self.storage_dtype is not None:
+            return 2 * self.rows8.row_bytes
         return 2 * self.kv_heads * self.head_dim * torch.empty((), dtype=self.dtype).element_size()

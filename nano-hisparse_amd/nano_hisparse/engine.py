@@ -66,7 +66,7 @@ class Engine:
         cfg, kv = model.config, cache.config
         if (cfg.num_key_value_heads, cfg.head_dim) != (kv.kv_heads, kv.head_dim):
             raise ValueError("model/cache head dimensions differ")
-        if model.device != cache.pool.device or model.dtype != cache.pool.dtype:
+        if model.device != cache.pool.device or model.dtype != kv.dtype:
             raise ValueError("model/cache dtype or device differ")
         if top_k is not None and top_k < 1:
             raise ValueError("top_k must be positive or None")

@@ -48,7 +48,8 @@ def set_cpu_provider(provider):
     maximum, length, page_size, top_pages, keep_sink) -> position tensor and
     mean_pages(query, summaries, length, page_size, top_pages) -> page list;
     for drafted tokens and log probabilities tree_plan, tree_attention and
-    token_logprobs as below.
+    token_logprobs as below, and for caches of rows in 8 bits attend_8bit,
+    read_rows_8bit and round_8bit.
     """
     global _cpu_provider
     _cpu_provider = provider
@@ -421,6 +422,20 @@ def read_rows_8bit(pool, form, rows, dtype, out=None):
         )
     _hip.check(status, "nhs_read_rows8")
     return out
+
+
+def round_8bit(k, v, form):
+    """K and V [n, Hkv, D] as a cache of rows in 8 bits would hold them, in
+    their own type: appended to a page of their own and read back."""
+    n, shape = len(k), k.shape[1:]
+    if n == 0:
+        return k, v
+    device = _require_gpu("round_8bit", k, v)
+    page = pool_8bit(1, n, form, device)
+    unused = torch.empty(2, *shape, dtype=k.dtype, device=device)  # the page's bounds and mean
+    append_page_8bit(k.contiguous(), v.contiguous(), page, form, 0, 0, None, 0,
+                     torch.empty(shape, dtype=torch.float32, device=device), *unused)
+    return read_rows_8bit(page, form, torch.arange(n, device=device), k.dtype)
 
 
 def attend_8bit(query, pool, form, rows, out=None):

@@ -39,6 +39,27 @@ def upload(values, dtype, device):
     return host.pin_memory().to(device, non_blocking=True)
 
 
+def _rows_in_8_bits(form, x):
+    """Rows [tokens, row_bytes] of x [tokens, kv_heads, head_dim] as a CPU
+    cache holds them (a GPU cache makes them inside nhs_append_page8);
+    quotients in 64 bits, so that those next to a border of two codes go to
+    the right one."""
+    x = x.double()
+    odd = ~torch.isfinite(x).all(-1)
+    x = torch.where(odd[..., None], 0.0, x)
+    largest = 127.0 if form.code == torch.int8 else 448.0
+    scale = (x.abs().amax(-1) / largest).float().clamp(min=2.0**-80)
+    codes = x / scale.double()[..., None]
+    if form.code != torch.int8:  # whole steps: 2^-3 of the power of two below, at least 2^-9
+        exponent = (torch.frexp(codes).exponent - 1).clamp(-6, 8)
+        step = torch.tensor([2.0 ** (e - 3) for e in range(-6, 9)], dtype=torch.float64)[exponent + 6]
+        codes = torch.round(codes / step) * step
+    rows = torch.zeros(len(x), form.row_bytes, dtype=torch.uint8)
+    form.codes(rows).copy_(torch.round(codes) if form.code == torch.int8 else codes)
+    form.scales(rows).copy_(torch.where(odd, torch.nan, scale))
+    return rows
+
+
 _pauses = threading.Lock()
 _paused = [0, False]  # captures in progress, whether collection was on before the first
 
@@ -167,8 +188,8 @@ class HostStore:
         self.cuda = self.device.type == "cuda"
         if self.cuda and not torch.cuda.is_available():
             raise RuntimeError("CUDA unavailable; use device='cpu' for the reference path")
-        shape = (config.host_pages, 2, config.page_size, config.kv_heads, config.head_dim)
-        self.host = torch.empty(shape, dtype=config.dtype, pin_memory=self.cuda)
+        self.rows8 = config.rows8  # the form of rows in 8 bits, or None
+        self.host = torch.empty((config.host_pages, *self.pool.shape[1:]), dtype=self.pool.dtype, pin_memory=self.cuda)
         self.host_alias = None
         if self.cuda:
             from .row_kernels import MappedHost
@@ -213,7 +234,7 @@ class HostStore:
 
     def index_reservation_bytes(self, max_tokens, layers):
         cfg = self.config
-        per_page = cfg.kv_heads * cfg.head_dim * (4 + 2 * self.pool.element_size())
+        per_page = cfg.kv_heads * cfg.head_dim * (4 + 2 * torch.finfo(cfg.dtype).bits // 8)
         return ceil(max_tokens / cfg.page_size) * layers * per_page
 
     @property
@@ -394,7 +415,11 @@ class HostStore:
 
             # one kernel per page: pool rows, host mirror rows, bounds and summary
             appender = PageAppender(k.contiguous(), v.contiguous(), self.pool, self.host_alias, request.summaries,
-                                    request.minimum, request.maximum)
+                                    request.minimum, request.maximum, self.rows8)
+        elif self.rows8 is not None:
+            rows_k, rows_v = (_rows_in_8_bits(self.rows8, x) for x in (k, v))
+        else:
+            rows_k, rows_v = k, v
         done, tokens = 0, len(k)
         while done < tokens:
             index, within = divmod(start + done, P)
@@ -421,9 +446,9 @@ class HostStore:
                 page.host_enqueued_version = page.content_version
             else:
                 block = self.pool[page.slot]
-                block[0, within : within + count].copy_(k[done : done + count])
-                block[1, within : within + count].copy_(v[done : done + count])
-                self._update_bounds(request, layer, index, block, within, count)
+                block[0, within : within + count].copy_(rows_k[done : done + count])
+                block[1, within : within + count].copy_(rows_v[done : done + count])
+                self._update_bounds(request, layer, index, block, within, k[done : done + count])
                 page.ready = self.event(self.compute)
                 self._mirror(page, block, within, count)
             self.stats["d2h_bytes"] += self.page_bytes * count // P
@@ -434,13 +459,18 @@ class HostStore:
             if after_write is not None:
                 after_write(page)
 
-    def _update_bounds(self, request, layer, index, block, within, count):
+    def _update_bounds(self, request, layer, index, block, within, keys):
         """Page mean key (fp32) and running min/max of the new keys
         (reference storage.py:302-309); CPU caches only (a GPU cache does
         this inside nhs_append_page)."""
-        valid = within + count
-        request.summaries[layer, index].copy_(block[0, :valid].float().mean(0))
-        new_keys = block[0, within:valid].float()
+        valid = within + len(keys)
+        held = block[0, :valid]
+        if self.rows8 is not None:
+            held = self.rows8.codes(held).double() * self.rows8.scales(held).double()[..., None]
+        else:
+            held = held.float()
+        request.summaries[layer, index].copy_(held.mean(0))
+        new_keys = keys.float()
         lo, hi = request.minimum[layer, index], request.maximum[layer, index]
         lo.copy_(torch.minimum(lo, new_keys.amin(0)))
         hi.copy_(torch.maximum(hi, new_keys.amax(0)))
@@ -531,6 +561,8 @@ class HostStore:
             page = self.pages[(request_id, layer, i)]
             chunks.append(self.host[page.host_slot, :, : page.valid_tokens])
         kv = torch.cat(chunks, dim=1)
+        if self.rows8 is not None:
+            kv = (self.rows8.codes(kv).float() * self.rows8.scales(kv)[..., None]).to(self.config.dtype)
         return kv[0], kv[1]
 
     def snapshot(self):
