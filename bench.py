@@ -104,6 +104,8 @@ def parse_args():
     ap.add_argument("--requests", type=int, default=8, help="model workload: concurrent requests")
     ap.add_argument("--graph", type=int, default=1, choices=(0, 1),
                     help="model workloads: 1 replays each decode step from a captured HIP graph")
+    ap.add_argument("--storage", choices=("int8", "e4m3"), default=None,
+                    help="model workload: hold the cache's rows in 8 bits (default: in bf16)")
     ap.add_argument("--micro-batches", type=int, default=1, choices=(1, 2),
                     help="model workload: 2 pipelines two halves of the batch (gathers beside compute)")
     return ap.parse_args()
@@ -623,7 +625,8 @@ def model_decode(args, B, L, T, K, W):
     resident = int(0.3 * B * L * pages)
     kv = CacheConfig(gpu_pages=B * hot.admission_blocks(P, L) + resident, host_pages=B * L * pages, page_size=P,
                      kv_heads=8, head_dim=128, dtype=torch.bfloat16, device=str(device),
-                     index_budget_bytes=1 << 31)
+                     index_budget_bytes=1 << 31,
+                     storage_dtype={"int8": torch.int8, "e4m3": torch.float8_e4m3fn, None: None}[args.storage])
     t0 = time.perf_counter()
     cache = HybridKVCache(kv, hot)
     print(f"[bench] cache: {kv.gpu_pages} pool blocks ({kv.gpu_pages * kv.row_bytes * P / 2**30:.1f} GiB), "
@@ -694,6 +697,8 @@ def model_decode(args, B, L, T, K, W):
         "wall_s_timed": round(wall, 3),
         "admit_s": round(admit_s, 2),  # untimed: every prompt prefilled, admitted requests decoding meanwhile
     }
+    if args.storage:
+        result["config"]["storage"] = args.storage
     del engine, cache, model
     torch.cuda.empty_cache()
     return result
