@@ -231,6 +231,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   constexpr int KI = kF8Tile / RI;        // load instructions of a tile, for K and for V each
   constexpr int KS = D / 32;              // products of a score
   constexpr int kRows = DEPTH * kF8Tile;  // of a wave's round
+  constexpr bool kLoops = DEPTH == 2 || D == 256;  // else there is one round (plan8)
+  constexpr bool kAhead = D != 256 || QP == 1;     // registers
   struct Wave {
     f8_u32x4 k[kF8Tile * N], v[kF8Tile * N];
     const char* at[kRows][2];  // the rows' K and V
@@ -305,10 +307,10 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   float m = -INFINITY, l = 0.f;
 
   const int rounds = (end - begin + kF8Waves * kRows - 1) / (kF8Waves * kRows);
-  for (int round = 0; round < rounds; ++round) {
-    // addresses and scales of the round's rows
-    uint64_t seen[kMine];
-    float ks[kMine], vs[kMine];
+  uint64_t seen[kMine];
+  float ks[kMine], vs[kMine];
+  // addresses of a round's rows to LDS, their scales asked for
+  const auto stage = [&] {
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const bool in = index[i] >= 0 && index[i] < a.pool_rows;
@@ -326,26 +328,30 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
       vs[i] = *(const NHS_GLOBAL float*)(vp + to_scale);
     }
     f8_order();
-    // All loads of the round, the keys first: scores and weights are there when the last values come. Non-temporal,
-    // since no one reads a row's codes again (their lines are shared with the neighbouring heads of the same moment), and
-    // before the arithmetic of the wave's neighbours. us of 16 x 2048 rows of 32/8 heads, 64 x 1024 of 28/4: 23.8, 22.3
-    // plain, 22.3, 21.2 non-temporal, 21.8, 20.9 with the priority; with non-temporal scales too (whose lines all heads
-    // read) 23.3, 23.2.
-    f8_u32x4 k[DEPTH][KI], v[DEPTH][KI];
+  };
+  // The loads of a round's keys or values. Non-temporal, since no one reads a row's codes again (their lines are shared
+  // with the neighbouring heads of the same moment), and ahead of the arithmetic of the wave's neighbours. us of 16 x
+  // 2048 rows of 32/8 heads, 64 x 1024 of 28/4: 23.8, 22.3 plain, 22.3, 21.2 non-temporal, 21.8, 20.9 with the priority;
+  // with non-temporal scales too (whose lines all heads read) 23.3, 23.2.
+  f8_u32x4 k[DEPTH][KI], v[DEPTH][KI];
+  const auto load = [&](int plane, f8_u32x4(&to)[DEPTH][KI]) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
       for (int i = 0; i < KI; ++i)
-        k[d][i] = __builtin_nontemporal_load(
-            (const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][0] + lane % N * 16));
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-#pragma unroll
-      for (int i = 0; i < KI; ++i)
-        v[d][i] = __builtin_nontemporal_load(
-            (const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][1] + lane % N * 16));
+        to[d][i] = __builtin_nontemporal_load(
+            (const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][plane] + lane % N * 16));
+  };
+  if (rounds > 0) {
+    stage();
+    if (kLoops && rounds > 1) fetch(1);
+    load(0, k);
+  }
+  // Keys first: scores and weights are there when the last values come. Where there are several rounds, the next one's
+  // keys are asked for as soon as this one's have been multiplied (32 requests x 2048 rows of 32/8 heads 33.4 us, 36.2 without).
+  for (int round = 0; round < (kLoops ? rounds : min(rounds, 1)); ++round) {
+    load(1, v);
     __builtin_amdgcn_s_setprio(0);
-    if (round + 1 < rounds) fetch(round + 1);
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
       if (kMine * kWave == kRows || lane < kRows) {
@@ -394,6 +400,14 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
         }
       }
     }
+    const auto next = [&] {
+      if (!kLoops || round + 1 >= rounds) return;
+      f8_order();
+      stage();
+      if (round + 2 < rounds) fetch(round + 2);
+      load(0, k);
+    };
+    if constexpr (kAhead) next();
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
@@ -438,6 +452,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
         for (int part = 0; part < PP; ++part) acc[t] = f8_mfma(values, weights[d][part], acc[t]);
       }
     }
+    if constexpr (!kAhead) next();
     f8_order();
   }
   l += __shfl_xor(l, 16);
@@ -590,7 +605,7 @@ static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_di
   per = (per + kStep - 1) / kStep * kStep;
   p.splits = (n_rows + per - 1) / per;
   p.rows_per_split = per;
-  p.depth = per <= kStep || head_dim == 256 ? 1 : per <= 2 * kStep ? 2 : 4;
+  p.depth = per <= kStep || head_dim == 256 ? 1 : per > 2 * kStep && per <= 4 * kStep ? 4 : 2;
   return p;
 }
 

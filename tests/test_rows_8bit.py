@@ -617,6 +617,21 @@ def test_attend_long_lists_and_sharp_scores(gpu, heads, kv, dim, dtype, code):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("code", [i8, e4m3])
+@pytest.mark.parametrize("dtype", [bf16, f16, f32])
+@pytest.mark.parametrize("heads, kv, dim, B, N", [(16, 8, 64, 33, 1300), (8, 8, 128, 32, 1025), (8, 8, 32, 40, 2049),
+                                                 (4, 4, 256, 66, 600)])
+def test_attend_large_batches(gpu, heads, kv, dim, B, N, dtype, code):
+    """Enough (request, KV head) pairs that no list is split: waves go over
+    several rounds of rows. Every fifth request has a shorter list, one none."""
+    gen = torch.Generator().manual_seed(B)
+    form, pool, rows, q = attend_case(gen, gpu, heads, kv, dim, code, dtype, B, N, 64)
+    for b in range(0, B, 5):
+        rows[b, N * b // B:] = -1
+    check(rk.attend_8bit(q, pool, form, rows), *attend_oracle(form, q, pool, rows))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads, kv, dim", [(8, 2, 128), (4, 2, 64), (6, 2, 80)])
 def test_attend_strides_and_outputs(gpu, heads, kv, dim):
     gen = torch.Generator().manual_seed(4)
