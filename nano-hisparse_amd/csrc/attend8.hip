@@ -153,6 +153,20 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
 // an fp32 query of three, exactly; a weight (times the scale of the row's
 // values) goes as two bf16 numbers, 2^-17 of it lost, or for fp32 queries as
 // three.
+//
+// Measured (MI355X, rows from HBM, graphs; us with the join of the splits): 16
+// requests x 2048 rows of 32/8 heads of 128, bf16 and e4m3, 21.8 (69 MB; the
+// general kernel 887); 64 x 1024 rows of 28/4 heads, int8, 21.2 in one launch;
+// one request x 32768 rows 22.6; 32 x 2048 rows 33.3. The rows stream at 5.6
+// TB/s once they flow (1.03 times their bytes are read), but 3.5 us pass
+// before the first are in; the scales, a line for each row and head, take 2.4,
+// what follows the last row 2, the join 3 to 4.
+//
+// The heads of a (request, split) are workgroups on one XCD (`near`): a head's
+// slice of a row begins at any multiple of 32 bytes, so neighbours share cache
+// lines, and all share those of the scales (spread over the XCDs: 36.5 us where
+// it takes 25.9). With fewer than 8 such groups the heads are spread instead,
+// over more of the XCDs.
 constexpr int kF8Threads = 512, kF8Waves = kF8Threads / kWave, kF8Tile = 32, kF8Heads = 16;
 
 typedef __bf16 f8_bf16x8 __attribute__((ext_vector_type(8)));
@@ -348,7 +362,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
     load(0, k);
   }
   // Keys first: scores and weights are there when the last values come. Where there are several rounds, the next one's
-  // keys are asked for as soon as this one's have been multiplied (32 requests x 2048 rows of 32/8 heads 33.4 us, 36.2 without).
+  // keys are asked for as soon as this one's have been multiplied (32 requests x 2048 rows of 32/8 heads 33.4 us, 36.2
+  // without).
   for (int round = 0; round < (kLoops ? rounds : min(rounds, 1)); ++round) {
     load(1, v);
     __builtin_amdgcn_s_setprio(0);
@@ -590,14 +605,16 @@ static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_di
   p.subs = kv_heads * p.chunks;
   const int64_t items = (int64_t)batch * p.subs;
   if (!p.flash) {
-    // about two workgroups per CU, splits of at least 64 rows
+    // the general kernel: about two workgroups per CU, splits of at least 64 rows
     const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + 63) / 64);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, 512 / items));
     p.rows_per_split = (n_rows + p.splits - 1) / p.splits;
     p.depth = 1;
     return p;
   }
-  // about one workgroup per CU, splits of whole rounds of its eight waves
+  // About one workgroup per CU, in splits of whole tiles for its eight waves. Twice as many, of half the rows: 16 x 2048
+  // rows 25.2 us against 21.8, 8 x 2048 18.9 against 14.9, 64 x 1024 of 28/4 heads 28.2 against 21.1, one request x 2048
+  // the same. A wave asks for all its rows of a round at once: one, two or four tiles, two where there are more rounds.
   constexpr int kStep = kF8Waves * kF8Tile;
   const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + kStep - 1) / kStep);
   int splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (256 + items / 2) / items));
