@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
   }
 }
 
-// ---- heads of 32, 64, 128 and 256, on the matrix cores ------------------------------------
+// ---- heads of a multiple of 16 dims up to 256, on the matrix cores -------------------------
 
 // A workgroup of 8 waves takes up to 16 query heads of one (request, KV head)
 // and one split of the rows; wave w takes tiles w, w + 8, ... of 32 rows.
@@ -167,6 +167,9 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
 // lines, and all share those of the scales (spread over the XCDs: 36.5 us where
 // it takes 25.9). With fewer than 8 such groups the heads are spread instead,
 // over more of the XCDs.
+//
+// Heads that are no power of two run in the next larger D (PAD): chunks past
+// their dims are zeros, which add nothing to a score and to no one's output.
 constexpr int kF8Threads = 512, kF8Waves = kF8Threads / kWave, kF8Tile = 32, kF8Heads = 16;
 
 typedef __bf16 f8_bf16x8 __attribute__((ext_vector_type(8)));
@@ -237,7 +240,7 @@ __device__ __forceinline__ int f8_v_slot(int r, int c) {
 // only the compiler has to keep them so.
 __device__ __forceinline__ void f8_order() { asm volatile("" ::: "memory"); }
 
-template <typename C, int QP, int D, int DEPTH>
+template <typename C, int QP, int D, int DEPTH, bool LOOP, bool PAD>
 __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a) {
   constexpr int PP = QP == 3 ? 3 : 2;     // operands of the weights
   constexpr int N = D / 16;               // 16-byte chunks of a head's row
@@ -245,7 +248,6 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   constexpr int KI = kF8Tile / RI;        // load instructions of a tile, for K and for V each
   constexpr int KS = D / 32;              // products of a score
   constexpr int kRows = DEPTH * kF8Tile;  // of a wave's round
-  constexpr bool kLoops = DEPTH == 2 || D == 256;  // else there is one round (plan8)
   constexpr bool kAhead = D != 256 || QP == 1;     // registers
   struct Wave {
     f8_u32x4 k[kF8Tile * N], v[kF8Tile * N];
@@ -256,6 +258,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   constexpr int kBytes = kF8Waves * (int)sizeof(Wave) > kMerged ? kF8Waves * (int)sizeof(Wave) : kMerged;
   __shared__ __attribute__((aligned(16))) char lds[kBytes];
 
+  const int dims = PAD ? a.head_dim : D;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   __builtin_amdgcn_s_setprio(3);  // (see the loads)
@@ -298,7 +301,10 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
     const int d0 = N >= 4 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * g;
     float x[8];
     const int64_t at = (int64_t)b * a.q_bs + (int64_t)(h0 + min(n, heads - 1)) * a.q_hs + d0;
-    if (a.q_aligned) {
+    if (PAD && d0 >= dims) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    } else if (a.q_aligned) {
       if constexpr (QP == 1)
         load_vec<BF16, 8>(a.q, at, x);
       else if constexpr (QP == 2)
@@ -330,9 +336,9 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
       const bool in = index[i] >= 0 && index[i] < a.pool_rows;
       const uint32_t at = in ? (uint32_t)index[i] : 0u, page = a.page_div.div(at);
       const char* row = a.pool + page * a.block_stride + (int64_t)(at - page * a.page_size) * a.row_bytes;
-      const char* kp = in ? row + kv * D : attend8_zeros;
-      const char* vp = in ? row + a.plane_bytes + kv * D : attend8_zeros;
-      const int64_t to_scale = in ? a.scales_at + 4 * (int64_t)kv - kv * D : 0;
+      const char* kp = in ? row + kv * dims : attend8_zeros;
+      const char* vp = in ? row + a.plane_bytes + kv * dims : attend8_zeros;
+      const int64_t to_scale = in ? a.scales_at + 4 * (int64_t)kv - kv * dims : 0;
       seen[i] = __ballot(in);
       if (kMine * kWave == kRows || lane < kRows) {
         w.at[lane + i * kWave][0] = kp;
@@ -352,19 +358,21 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
-      for (int i = 0; i < KI; ++i)
-        to[d][i] = __builtin_nontemporal_load(
-            (const NHS_GLOBAL f8_u32x4*)(w.at[d * kF8Tile + i * RI + lane / N][plane] + lane % N * 16));
+      for (int i = 0; i < KI; ++i) {
+        const char* at = w.at[d * kF8Tile + i * RI + lane / N][plane] + lane % N * 16;
+        if (PAD && lane % N * 16 >= dims) at = attend8_zeros;
+        to[d][i] = __builtin_nontemporal_load((const NHS_GLOBAL f8_u32x4*)at);
+      }
   };
   if (rounds > 0) {
     stage();
-    if (kLoops && rounds > 1) fetch(1);
+    if (LOOP && rounds > 1) fetch(1);
     load(0, k);
   }
   // Keys first: scores and weights are there when the last values come. Where there are several rounds, the next one's
   // keys are asked for as soon as this one's have been multiplied (32 requests x 2048 rows of 32/8 heads 33.4 us, 36.2
   // without).
-  for (int round = 0; round < (kLoops ? rounds : min(rounds, 1)); ++round) {
+  for (int round = 0; round < (LOOP ? rounds : min(rounds, 1)); ++round) {  // (without LOOP there is one, see plan8)
     load(1, v);
     __builtin_amdgcn_s_setprio(0);
 #pragma unroll
@@ -416,7 +424,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
       }
     }
     const auto next = [&] {
-      if (!kLoops || round + 1 >= rounds) return;
+      if (!LOOP || round + 1 >= rounds) return;
       f8_order();
       stage();
       if (round + 2 < rounds) fetch(round + 2);
@@ -488,8 +496,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   }
   __syncthreads();
   const int64_t all = (int64_t)a.batch * a.q_heads;
-  for (int i = threadIdx.x; i < heads * D; i += kF8Threads) {
-    const int h = i / D, d = i - h * D;
+  for (int i = threadIdx.x; i < heads * dims; i += kF8Threads) {
+    const int h = i / dims, d = i - h * dims;
     const float* from = merged + h * kPitch;
     float top = -INFINITY;
 #pragma unroll
@@ -505,7 +513,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
     }
     if (a.n_splits > 1) {
       const int64_t at = split * all + (int64_t)b * a.q_heads + h0 + h;
-      a.partial[at * D + d] = o;
+      a.partial[at * dims + d] = o;
       if (d == 0) {
         a.stats[2 * at] = top;
         a.stats[2 * at + 1] = total;
@@ -598,7 +606,7 @@ struct Plan8 {
 // own_lists: every query head has a row list of its own.
 static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_dim, bool own_lists) {
   Plan8 p;
-  p.flash = head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256;
+  p.flash = head_dim % 16 == 0 && head_dim <= 256;
   p.heads_per_item = p.flash && !own_lists ? kF8Heads : 1;
   const int group = q_heads / kv_heads;
   p.chunks = (group + p.heads_per_item - 1) / p.heads_per_item;
@@ -614,7 +622,7 @@ static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_di
   }
   // About one workgroup per CU, in splits of whole tiles for its eight waves. Twice as many, of half the rows: 16 x 2048
   // rows 25.2 us against 21.8, 8 x 2048 18.9 against 14.9, 64 x 1024 of 28/4 heads 28.2 against 21.1, one request x 2048
-  // the same. A wave asks for all its rows of a round at once: one, two or four tiles, two where there are more rounds.
+  // the same. A wave asks for all its rows at once (one tile, or four), or for two tiles in a round.
   constexpr int kStep = kF8Waves * kF8Tile;
   const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + kStep - 1) / kStep);
   int splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (256 + items / 2) / items));
@@ -622,7 +630,7 @@ static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_di
   per = (per + kStep - 1) / kStep * kStep;
   p.splits = (n_rows + per - 1) / per;
   p.rows_per_split = per;
-  p.depth = per <= kStep || head_dim == 256 ? 1 : per > 2 * kStep && per <= 4 * kStep ? 4 : 2;
+  p.depth = per <= kStep ? 1 : per > 2 * kStep && per <= 4 * kStep ? 4 : 0;
   return p;
 }
 
@@ -630,20 +638,31 @@ static int64_t workspace8(const Plan8& p, int64_t heads, int head_dim) {
   return p.splits == 1 ? 0 : p.splits * heads * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
+// depth: tiles of a wave's only round, or 0 for the loop over rounds. (A kernel of its own for a single round of two
+// tiles: 8 requests x 2048 rows of 32/8 heads 15.3 us against 15.7 in the loop, int8 15.9 against 15.4, fp32 16.0
+// against 15.3.)
+template <typename C, int QP, int D, bool PAD>
+static void (*flash8_deep(int depth))(Attend8Args) {
+  constexpr int kRound = D == 256 ? 1 : 2;
+  if constexpr (D != 256) {
+    if (depth == 1) return attend8_flash_kernel<C, QP, D, 1, false, PAD>;
+    if constexpr (!PAD && (QP != 3 || D != 128))  // (four tiles of fp32 queries and heads of 128: registers)
+      if (depth == 4) return attend8_flash_kernel<C, QP, D, 4, false, PAD>;
+  }
+  return attend8_flash_kernel<C, QP, D, kRound, true, PAD>;
+}
+
 template <typename C, int QP>
 static void (*flash8(int head_dim, int depth))(Attend8Args) {
-  switch (head_dim * 8 + depth) {
-    case 32 * 8 + 1: return attend8_flash_kernel<C, QP, 32, 1>;
-    case 32 * 8 + 2: return attend8_flash_kernel<C, QP, 32, 2>;
-    case 32 * 8 + 4: return attend8_flash_kernel<C, QP, 32, 4>;
-    case 64 * 8 + 1: return attend8_flash_kernel<C, QP, 64, 1>;
-    case 64 * 8 + 2: return attend8_flash_kernel<C, QP, 64, 2>;
-    case 64 * 8 + 4: return attend8_flash_kernel<C, QP, 64, 4>;
-    case 128 * 8 + 1: return attend8_flash_kernel<C, QP, 128, 1>;
-    case 128 * 8 + 2: return attend8_flash_kernel<C, QP, 128, 2>;
-    case 128 * 8 + 4: return attend8_flash_kernel<C, QP, 128, QP == 3 ? 2 : 4>;  // (fp32 queries: registers)
-    default: return attend8_flash_kernel<C, QP, 256, 1>;
+  switch (head_dim) {
+    case 32: return flash8_deep<C, QP, 32, false>(depth);
+    case 64: return flash8_deep<C, QP, 64, false>(depth);
+    case 128: return flash8_deep<C, QP, 128, false>(depth);
+    case 256: return flash8_deep<C, QP, 256, false>(depth);
   }
+  return head_dim < 64    ? flash8_deep<C, QP, 64, true>(depth)
+         : head_dim < 128 ? flash8_deep<C, QP, 128, true>(depth)
+                          : flash8_deep<C, QP, 256, true>(depth);
 }
 
 }  // namespace nhs

@@ -178,14 +178,15 @@ __global__ __launch_bounds__(kA8Threads) void append8_items_kernel(Append8ItemsA
   append8_head<T, C, N>(a, plane, (int)blockIdx.x - plane * a.form.kv_heads);
 }
 
-// ---- heads of 32, 64, 128 and 256 dims: rows of whole chunks ------------------------------
+// ---- heads of a multiple of 16 dims up to 256: rows of whole chunks ------------------------
 
 // Some workgroups copy: a wave takes 64 chunks of 16 elements of a row's plane
 // (so whole heads), quantises them and writes 1 KB of codes to the pool and
 // past the caches to the host block, whose rows are consecutive. Others fold
 // the keys of one head each: they quantise them too (the copies' codes are not
 // written yet), hold 64 rows of codes and keys in LDS and walk them, a thread
-// per element and share of the rows.
+// per element and share of the rows. A head is N chunks, a power of two, the
+// last of them beyond its dims where its own number is none.
 constexpr int kFold8Rows = 64;
 constexpr int kR8Threads = 512, kR8Waves = kR8Threads / kWave;
 
@@ -220,13 +221,14 @@ struct Chunk8 {
   }
 };
 
-// The codes and the scale of a slice that N neighbouring lanes hold.
+// The codes and the scale of a slice that N neighbouring lanes hold (those that are not `live` hold none of it).
 template <typename T, typename C, int N>
-__device__ __forceinline__ u32x4 quantise8(Chunk8<T>& c, float* scale) {
+__device__ __forceinline__ u32x4 quantise8(Chunk8<T>& c, bool live, float* scale) {
   c.widen();
   uint32_t largest = 0;
 #pragma unroll
   for (int e = 0; e < 16; ++e) largest = max(largest, __float_as_uint(c.x[e]) & 0x7fffffffu);
+  largest = live ? largest : 0;
 #pragma unroll
   for (int d = 1; d < N; d <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d));
   *scale = scale8<C>(largest);
@@ -242,23 +244,24 @@ __device__ __forceinline__ u32x4 quantise8(Chunk8<T>& c, float* scale) {
 
 template <typename T, typename C, int N>
 __device__ __forceinline__ void copy8(const Append8Args& a, int unit, int groups) {
-  const int lane = threadIdx.x & 63, chunks = a.form.kv_heads * N;
-  const int row = unit / groups, group = unit - row * groups;
+  constexpr int kHeads = kWave / N;  // of a wave
+  const int lane = threadIdx.x & 63, row = unit / groups, group = unit - row * groups;
   if (row >= 2 * a.count) return;
   const int plane = row >= a.count, t = row - plane * a.count;
-  const int chunk = group * kWave + lane;
-  const bool live = chunk < chunks;
+  const int head = group * kHeads + lane / N, from = lane % N * 16;  // the lane's elements of its head
+  const bool live = head < a.form.kv_heads && from < a.form.head_dim;
+  const int at_elem = live ? head * a.form.head_dim + from : 0;
   Chunk8<T> c;
-  c.load((plane ? a.v : a.k) + ((int64_t)t * a.token_stride + min(chunk, chunks - 1) * 16) * T::bytes);
+  c.load((plane ? a.v : a.k) + ((int64_t)t * a.token_stride + at_elem) * T::bytes);
   float scale;
-  const u32x4 codes = quantise8<T, C, N>(c, &scale);
+  const u32x4 codes = quantise8<T, C, N>(c, live, &scale);
   const int64_t at = ((int64_t)plane * a.page_size + a.within + t) * a.form.bytes;
   const float head_scale = __shfl(scale, lane * N % kWave);
-  const bool scales = lane < kWave / N && group * (kWave / N) + lane < a.form.kv_heads;
-  const int64_t to_scale = at + a.form.scales_at + 4 * (group * (kWave / N) + lane);
+  const bool scales = lane < kHeads && group * kHeads + lane < a.form.kv_heads;
+  const int64_t to_scale = at + a.form.scales_at + 4 * (group * kHeads + lane);
   if (live) {
-    *(NHS_GLOBAL u32x4*)to_global(a.pool_block + at + chunk * 16) = codes;
-    if (a.host_block) store_through(to_global(a.host_block + at + chunk * 16), codes);
+    *(NHS_GLOBAL u32x4*)to_global(a.pool_block + at + at_elem) = codes;
+    if (a.host_block) store_through(to_global(a.host_block + at + at_elem), codes);
   }
   if (scales) {
     *(NHS_GLOBAL float*)to_global(a.pool_block + to_scale) = head_scale;
@@ -272,8 +275,9 @@ __device__ __forceinline__ void fold8(const Append8Args& a, int head) {
   constexpr int kPasses = (kFold8Rows + kRowsPerPass - 1) / kRowsPerPass;
   __shared__ __attribute__((aligned(16))) Fold8<T, N> s;
   const int tid = threadIdx.x, chunk = tid % N, slot = tid / N;
-  const int col = tid % D, part = tid / D;
-  const int64_t slice = (int64_t)head * D, at_scale = a.form.scales_at + 4 * (int64_t)head;
+  const int dims = a.form.head_dim, from = chunk * 16 < dims ? chunk * 16 : 0;
+  const int col = min(tid % D, dims - 1), part = tid / D;
+  const int64_t slice = (int64_t)head * dims, at_scale = a.form.scales_at + 4 * (int64_t)head;
   const int total = a.within + a.count;
   double sum = 0.0;
   float low = INFINITY, high = -INFINITY, low0 = 0.f, high0 = 0.f;
@@ -293,16 +297,16 @@ __device__ __forceinline__ void fold8(const Append8Args& a, int head) {
       const int r = min(r0 + slot + i * kRowsPerPass, total - 1);
       if (r < a.within) {
         const char* row = a.pool_block + (int64_t)r * a.form.bytes;
-        held[i] = *(const NHS_GLOBAL u32x4*)to_global(row + slice + chunk * 16);
+        held[i] = *(const NHS_GLOBAL u32x4*)to_global(row + slice + from);
         scale[i] = *(const NHS_GLOBAL float*)to_global(row + at_scale);
       }
-      fresh[i].load(a.k + ((int64_t)max(r - a.within, 0) * a.token_stride + slice + chunk * 16) * T::bytes);
+      fresh[i].load(a.k + ((int64_t)max(r - a.within, 0) * a.token_stride + slice + from) * T::bytes);
     }
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int j = slot + i * kRowsPerPass, r = r0 + j;
       float own;
-      const u32x4 codes = quantise8<T, C, N>(fresh[i], &own);
+      const u32x4 codes = quantise8<T, C, N>(fresh[i], chunk * 16 < dims, &own);
       if (j >= rows) continue;
       const bool earlier = r < a.within;
       *reinterpret_cast<u32x4*>(&s.codes[(j * N + chunk) * 4]) = earlier ? held[i] : codes;
@@ -328,7 +332,7 @@ __device__ __forceinline__ void fold8(const Append8Args& a, int head) {
   s.low[tid] = low;
   s.high[tid] = high;
   __syncthreads();
-  if (part) return;
+  if (part || tid % D >= dims) return;
 #pragma unroll
   for (int p = 1; p < kParts; ++p) {
     sum += s.sums[p * D + col];
@@ -348,9 +352,9 @@ __device__ __forceinline__ void append8_rows(const Append8Args& a) {
   copy8<T, C, N>(a, (group - a.form.kv_heads) * kR8Waves + ((int)threadIdx.x >> 6), groups);
 }
 
-// Workgroups of a launch for `count` rows.
-static unsigned rows8_grid(const Row8& form, int count) {
-  const int64_t groups = ((int64_t)form.kv_heads * (form.head_dim / 16) + kWave - 1) / kWave;
+// Workgroups of a launch for `count` rows of heads of N chunks.
+static unsigned rows8_grid(const Row8& form, int count, int N) {
+  const int64_t groups = ((int64_t)form.kv_heads * N + kWave - 1) / kWave;
   return (unsigned)(form.kv_heads + (2 * count * groups + kR8Waves - 1) / kR8Waves);
 }
 
@@ -504,18 +508,18 @@ static int check_pool8(const char* who, const void* pool, int code, int kv_heads
 // Whether rows are whole chunks of 16 elements wherever append8_rows touches them.
 static bool whole_chunks8(const Append8Args& a, int dtype) {
   const int d = a.form.head_dim;
-  return (d == 32 || d == 64 || d == 128 || d == 256) && a.token_stride * elem_size(dtype) % 16 == 0 &&
+  return d % 16 == 0 && d <= 256 && a.token_stride * elem_size(dtype) % 16 == 0 &&
          ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0;
 }
 
-// Calls f with the chunks of 16 elements of a head.
+// Calls f with the chunks of 16 elements of a head, rounded up to a power of two.
 template <typename F>
 static void with_chunks(int head_dim, F f) {
-  if (head_dim == 32)
+  if (head_dim <= 32)
     f(std::integral_constant<int, 2>());
-  else if (head_dim == 64)
+  else if (head_dim <= 64)
     f(std::integral_constant<int, 4>());
-  else if (head_dim == 128)
+  else if (head_dim <= 128)
     f(std::integral_constant<int, 8>());
   else
     f(std::integral_constant<int, 16>());
@@ -565,11 +569,11 @@ extern "C" int nhs_append_page8(const void* k, const void* v, int64_t token_stri
   a.minimum = minimum;
   a.maximum = maximum;
   if (whole_chunks8(a, kv_dtype)) {
-    const dim3 grid(rows8_grid(a.form, count));
     with_types(kv_dtype, code, [&](auto t, auto c) {
       with_chunks(head_dim, [&](auto n) {
-        launch(append8_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kR8Threads), 0,
-               (hipStream_t)stream, ev.start, ev.stop, a);
+        launch(append8_rows_kernel<decltype(t), decltype(c), decltype(n)::value>,
+               dim3(rows8_grid(a.form, count, decltype(n)::value)), dim3(kR8Threads), 0, (hipStream_t)stream, ev.start,
+               ev.stop, a);
       });
     });
     return launch_status("nhs_append_page8");
@@ -611,10 +615,10 @@ extern "C" int nhs_append_items8(int32_t batch, const void* k, const void* v, in
   g.items = items;
   g.lengths = lengths;
   if (whole_chunks8(g.a, kv_dtype)) {
-    const dim3 grid(rows8_grid(g.a.form, 1), (unsigned)batch);
     with_types(kv_dtype, code, [&](auto t, auto c) {
       with_chunks(head_dim, [&](auto n) {
-        launch(append8_item_rows_kernel<decltype(t), decltype(c), decltype(n)::value>, grid, dim3(kR8Threads), 0,
+        launch(append8_item_rows_kernel<decltype(t), decltype(c), decltype(n)::value>,
+               dim3(rows8_grid(g.a.form, 1, decltype(n)::value), (unsigned)batch), dim3(kR8Threads), 0,
                (hipStream_t)stream, ev.start, ev.stop, g);
       });
     });

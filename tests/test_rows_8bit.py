@@ -275,7 +275,7 @@ def test_a_planted_mistake_is_seen():
 # ---- appends (GPU) -----------------------------------------------------------------------------
 
 SHAPES = [(8, 128), (4, 128), (2, 64), (2, 32), (1, 256), (3, 80), (5, 16), (1, 1), (3, 5), (2, 130), (1, 1024), (2, 300),
-          (12, 48)]
+          (12, 48), (2, 96), (9, 112), (3, 192), (1, 240), (70, 16)]
 
 
 @pytest.mark.gpu
@@ -546,7 +546,8 @@ def test_read_rows_outputs_strides_and_refusals(gpu):
 # ---- attention (GPU) -----------------------------------------------------------------------------
 
 HEADS = [(32, 8, 128), (28, 4, 128), (16, 16, 128), (4, 2, 64), (14, 2, 64), (4, 2, 32), (8, 2, 256), (6, 2, 80),
-         (5, 1, 8), (3, 3, 2), (2, 1, 1024), (40, 2, 128), (4, 4, 130), (1, 1, 128), (17, 1, 64), (6, 3, 1)]
+         (5, 1, 8), (3, 3, 2), (2, 1, 1024), (40, 2, 128), (4, 4, 130), (1, 1, 128), (17, 1, 64), (6, 3, 1),
+         (8, 4, 96), (6, 2, 112), (3, 1, 192), (4, 2, 240), (5, 5, 16), (6, 3, 48)]
 
 
 def attend_case(gen, device, heads, kv, dim, code, dtype, B, N, P=16, scale=1.0, gap=0):
@@ -575,7 +576,7 @@ def test_attend(gpu, heads, kv, dim, dtype, code):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("code", [i8, e4m3])
-@pytest.mark.parametrize("heads, kv, dim", [(32, 8, 128), (14, 2, 64), (8, 2, 256), (4, 2, 32), (6, 2, 80)])
+@pytest.mark.parametrize("heads, kv, dim", [(32, 8, 128), (14, 2, 64), (8, 2, 256), (4, 2, 32), (6, 2, 80), (6, 2, 40)])
 @pytest.mark.parametrize("dtype", [bf16, f32])
 def test_attend_masks(gpu, heads, kv, dim, dtype, code):
     """Masked rows anywhere, lists without a row, rows outside the pool, and
@@ -620,7 +621,7 @@ def test_attend_long_lists_and_sharp_scores(gpu, heads, kv, dim, dtype, code):
 @pytest.mark.parametrize("code", [i8, e4m3])
 @pytest.mark.parametrize("dtype", [bf16, f16, f32])
 @pytest.mark.parametrize("heads, kv, dim, B, N", [(16, 8, 64, 33, 1300), (8, 8, 128, 32, 1025), (8, 8, 32, 40, 2049),
-                                                 (4, 4, 256, 66, 600)])
+                                                 (4, 4, 256, 66, 600), (8, 8, 96, 34, 1200), (4, 4, 160, 70, 520)])
 def test_attend_large_batches(gpu, heads, kv, dim, B, N, dtype, code):
     """Enough (request, KV head) pairs that no list is split: waves go over
     several rounds of rows. Every fifth request has a shorter list, one none."""
@@ -632,7 +633,7 @@ def test_attend_large_batches(gpu, heads, kv, dim, B, N, dtype, code):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads, kv, dim", [(8, 2, 128), (4, 2, 64), (6, 2, 80)])
+@pytest.mark.parametrize("heads, kv, dim", [(8, 2, 128), (4, 2, 64), (6, 2, 80), (6, 2, 72)])
 def test_attend_strides_and_outputs(gpu, heads, kv, dim):
     gen = torch.Generator().manual_seed(4)
     form, pool, rows, q = attend_case(gen, gpu, heads, kv, dim, e4m3, bf16, 3, 150, 16, gap=32)
