@@ -8,9 +8,7 @@
 #include <math.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "rows8.h"
 
@@ -156,7 +154,7 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
 //
 // Measured (MI355X, rows from HBM, graphs; us with the join of the splits): 16
 // requests x 2048 rows of 32/8 heads of 128, bf16 and e4m3, 21.8 (69 MB; the
-// general kernel 887); 64 x 1024 rows of 28/4 heads, int8, 21.2 in one launch;
+// general kernel 887); 64 x 1024 rows of 28/4 heads, int8, 21.1 in one launch;
 // one request x 32768 rows 22.6; 32 x 2048 rows 33.3. The rows stream at 5.6
 // TB/s once they flow (1.03 times their bytes are read), but 3.5 us pass
 // before the first are in; the scales, a line for each row and head, take 2.4,
@@ -248,7 +246,7 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   constexpr int KI = kF8Tile / RI;        // load instructions of a tile, for K and for V each
   constexpr int KS = D / 32;              // products of a score
   constexpr int kRows = DEPTH * kF8Tile;  // of a wave's round
-  constexpr bool kAhead = D != 256 || QP == 1;     // registers
+  constexpr bool kAhead = D != 256 || QP == 1;  // (the others have no registers left for it)
   struct Wave {
     f8_u32x4 k[kF8Tile * N], v[kF8Tile * N];
     const char* at[kRows][2];  // the rows' K and V
@@ -351,8 +349,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
   };
   // The loads of a round's keys or values. Non-temporal, since no one reads a row's codes again (their lines are shared
   // with the neighbouring heads of the same moment), and ahead of the arithmetic of the wave's neighbours. us of 16 x
-  // 2048 rows of 32/8 heads, 64 x 1024 of 28/4: 23.8, 22.3 plain, 22.3, 21.2 non-temporal, 21.8, 20.9 with the priority;
-  // with non-temporal scales too (whose lines all heads read) 23.3, 23.2.
+  // 2048 rows of 32/8 heads, 64 x 1024 of 28/4: 23.8, 22.3 plain, 22.3, 21.2 non-temporal, 21.8, 20.9 with the
+  // priority; with non-temporal scales too (whose lines all heads read) 23.3, 23.2.
   f8_u32x4 k[DEPTH][KI], v[DEPTH][KI];
   const auto load = [&](int plane, f8_u32x4(&to)[DEPTH][KI]) {
 #pragma unroll
@@ -519,7 +517,8 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
         a.stats[2 * at + 1] = total;
       }
     } else {
-      store_elem(a.out, a.q_dtype, (int64_t)b * a.o_bs + (int64_t)(h0 + h) * a.o_hs + d, total != 0.f ? o / total : 0.f);
+      const int64_t at = (int64_t)b * a.o_bs + (int64_t)(h0 + h) * a.o_hs + d;
+      store_elem(a.out, a.q_dtype, at, total != 0.f ? o / total : 0.f);
     }
   }
 }
@@ -621,8 +620,9 @@ static Plan8 plan8(int batch, int n_rows, int q_heads, int kv_heads, int head_di
     return p;
   }
   // About one workgroup per CU, in splits of whole tiles for its eight waves. Twice as many, of half the rows: 16 x 2048
-  // rows 25.2 us against 21.8, 8 x 2048 18.9 against 14.9, 64 x 1024 of 28/4 heads 28.2 against 21.1, one request x 2048
-  // the same. A wave asks for all its rows at once (one tile, or four), or for two tiles in a round.
+  // rows 26.6 us against 21.8, 8 x 2048 15.9 against 15.6, 64 x 1024 of 28/4 heads 27.9 against 21.0, one request x
+  // 32768 27.3 against 22.6, x 2048 the same. A wave asks for all its rows at once (one tile, or four), or for two tiles
+  // in a round.
   constexpr int kStep = kF8Waves * kF8Tile;
   const int64_t most = std::min<int64_t>(kA8MaxSplits, (n_rows + kStep - 1) / kStep);
   int splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (256 + items / 2) / items));
@@ -757,8 +757,8 @@ extern "C" int nhs_attend_rows8(const void* query, int32_t q_dtype, int64_t q_ba
              : q_dtype == NHS_F16 ? flash8<C, 2>(head_dim, plan.depth)
                                   : flash8<C, 3>(head_dim, plan.depth);
     };
-    launch(code == NHS_CODE_I8 ? pick(I8()) : pick(E4M3()), dim3((unsigned)grid), dim3(kF8Threads), 0, s, ev.start, stop,
-           a);
+    launch(code == NHS_CODE_I8 ? pick(I8()) : pick(E4M3()), dim3((unsigned)grid), dim3(kF8Threads), 0, s, ev.start,
+           stop, a);
   } else {
     if (heads * a.n_splits > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_attend_rows8: grid too large");
     const auto run = [&](auto c, auto n) {

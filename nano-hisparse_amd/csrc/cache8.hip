@@ -418,7 +418,15 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
 // of them in flight (heads and units of a row by exact division).
 constexpr int kRead8 = 4;
 
-template <typename T, typename C>
+//
+// STREAM: past the caches. Whoever reads the outputs finds them there only if
+// they fit beside its own traffic; then the plain stores are better, else
+// these. us of a read, its rows not in a cache, and a copy of its outputs,
+// plain and streamed: 8 MB 13.9, 15.7; 32 MB 34.5, 37.5; 64 MB 55.9, 63.4; 128
+// MB 113.5, 108.9; 256 MB 201, 196.
+constexpr int64_t kRead8Stream = 96 << 20;  // bytes of both outputs
+
+template <typename T, typename C, bool STREAM>
 __global__ __launch_bounds__(256) void read8_chunks_kernel(Read8Args a, FastDiv per_row, FastDiv per_head,
                                                            int rows_per_group) {
   constexpr int V = 16 / T::bytes;
@@ -440,7 +448,8 @@ __global__ __launch_bounds__(256) void read8_chunks_kernel(Read8Args a, FastDiv 
       // unconditional loads (row 0 in place of one outside the pool), so that no branch separates them
       const char* from = (row ? row : a.pool) + (int64_t)plane * a.page_size * a.form.bytes;
 #pragma unroll
-      for (int w = 0; w < V / 4; ++w) code[u][w] = reinterpret_cast<const NHS_GLOBAL uint32_t*>(to_global(from) + unit * V)[w];
+      for (int w = 0; w < V / 4; ++w)
+        code[u][w] = reinterpret_cast<const NHS_GLOBAL uint32_t*>(to_global(from) + unit * V)[w];
       scale[u] = *(const NHS_GLOBAL float*)(to_global(from) + a.form.scales_at + 4 * per_head.div(unit));
       there[u] = row != nullptr;
     }
@@ -466,7 +475,11 @@ __global__ __launch_bounds__(256) void read8_chunks_kernel(Read8Args a, FastDiv 
                          ? f32_to_bf16_bits(v[2 * e]) | (uint32_t)f32_to_bf16_bits(v[2 * e + 1]) << 16
                          : f32_to_f16_bits(v[2 * e]) | (uint32_t)f32_to_f16_bits(v[2 * e + 1]) << 16;
       }
-      *(NHS_GLOBAL u32x4*)to_global(out[u]) = words;
+      NHS_GLOBAL u32x4* to = (NHS_GLOBAL u32x4*)to_global(out[u]);
+      if constexpr (STREAM)
+        __builtin_nontemporal_store(words, to);
+      else
+        *to = words;
     }
   }
 }
@@ -667,15 +680,18 @@ extern "C" int nhs_read_rows8(const void* pool, int64_t pool_rows, int64_t pool_
   a.out_stride[0] = k_stride;
   a.out_stride[1] = v_stride;
   const int esize = elem_size(out_dtype), vec = 16 / esize;
-  if (pool_rows > 0 && head_dim % 8 == 0 && ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 && k_stride * esize % 16 == 0 &&
-      v_stride * esize % 16 == 0) {
+  if (pool_rows > 0 && head_dim % 8 == 0 && ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 &&
+      k_stride * esize % 16 == 0 && v_stride * esize % 16 == 0) {
     const uint32_t per_row = (uint32_t)(2 * width / vec);
     const int rows_per_group = (int)std::max<int64_t>(1, 256 * kRead8 / per_row);
     const int64_t grid = (n + rows_per_group - 1) / rows_per_group;
     if (grid > 0x7fffffff) return fail(NHS_ERR_UNSUPPORTED, "nhs_read_rows8: too many rows");
     with_types(out_dtype, code, [&](auto t, auto c) {
-      launch(read8_chunks_kernel<decltype(t), decltype(c)>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,
-             ev.start, ev.stop, a, FastDiv(per_row), FastDiv((uint32_t)(head_dim / vec)), rows_per_group);
+      using T = decltype(t);
+      using C = decltype(c);
+      launch(2 * n * width * esize >= kRead8Stream ? read8_chunks_kernel<T, C, true> : read8_chunks_kernel<T, C, false>,
+             dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, ev.start, ev.stop, a, FastDiv(per_row),
+             FastDiv((uint32_t)(head_dim / vec)), rows_per_group);
     });
     return launch_status("nhs_read_rows8");
   }

@@ -754,7 +754,8 @@ Host8 host8_of(PyObject* o, const Tensor& pool) {
   bool ok = held && pointer && THPVariable_Check(held) && PyLong_CheckExact(pointer);
   if (ok) {
     const Tensor& t = THPVariable_Unpack(held);
-    ok = t.scalar_type() == at::kByte && t.dim() == 4 && t.is_contiguous() && t.sizes().slice(1) == pool.sizes().slice(1);
+    ok = t.scalar_type() == at::kByte && t.dim() == 4 && t.is_contiguous() &&
+         t.sizes().slice(1) == pool.sizes().slice(1);
     h.alias = PyLong_AsVoidPtr(pointer);
     h.pages = t.size(0);
   }

@@ -146,7 +146,8 @@ class BatchDecode:
         if not (k[0].is_contiguous() and v[0].is_contiguous() and k.stride() == v.stride()):
             k, v = k.contiguous(), v.contiguous()  # rows may be views of a fused projection
         if store.rows8 is not None:
-            rk.append_items_8bit(k, v, cache.pool, store.rows8, store.host_alias, self.items[layer], self.dev_lengths[0])
+            rk.append_items_8bit(k, v, cache.pool, store.rows8, store.host_alias, self.items[layer],
+                                 self.dev_lengths[0])
         else:
             rk.append_items(k, v, cache.pool, store.host_alias, self.items[layer], self.dev_lengths[0])
         self._account_append(layer)

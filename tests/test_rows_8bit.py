@@ -509,6 +509,21 @@ def test_read_rows(gpu, heads, dim, dtype, code):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("code", [i8, e4m3])
+@pytest.mark.parametrize("dtype, n", [(bf16, 24577), (f16, 26001), (f32, 12700)])
+def test_read_rows_into_large_outputs(gpu, dtype, n, code):
+    """Outputs above 96 MB, which are stored past the caches: the values of reads in parts, and read by the next kernel
+    on the stream."""
+    gen = torch.Generator().manual_seed(9)
+    form, P = rk.Rows8(code, 8, 128), 16
+    pool = make_pool(form, 9, P, gen, gpu)
+    rows = torch.randint(-1, 9 * P + 1, (n,), generator=gen).to(gpu)
+    for got, parts in zip(rk.read_rows_8bit(pool, form, rows, dtype),
+                          zip(*(rk.read_rows_8bit(pool, form, x, dtype) for x in rows.split(5000)))):
+        assert torch.equal(got, torch.cat(parts))
+
+
+@pytest.mark.gpu
 def test_read_rows_outputs_strides_and_refusals(gpu):
     gen = torch.Generator().manual_seed(2)
     form = rk.Rows8(e4m3, 4, 64)
