@@ -64,6 +64,8 @@ def tree_row_attention(query, k, v, mask, cache, request_id, layer, topk, backen
         raise ValueError("a tree's nodes and heads share one selection")
     if backend == "triton" and not cache.storage.cuda:
         raise ValueError("Triton requires CUDA")
+    if cache.storage.rows8 is not None and not query.dtype == k.dtype == v.dtype == cfg.dtype:
+        raise ValueError("query, K and V dtype must match the cache")
     with cache.resolve(request_id, layer, topk) as lease:
         rows = lease.plan.physical_rows
         if cache.storage.cuda:
@@ -72,20 +74,23 @@ def tree_row_attention(query, k, v, mask, cache, request_id, layer, topk, backen
             from .row_kernels import cpu_provider
 
             kernels = cpu_provider("tree_row_attention")
-        pool, page_size = cache.pool, cfg.page_size
+        pool, page_size, dtype = cache.pool, cfg.page_size, query.dtype
         if cache.storage.rows8 is not None:
-            pool, rows, page_size, k, v = _read_for_tree(kernels, cache, rows, k, v)
-        return kernels.tree_attention(query[None], pool, rows[None], k[None], v[None], mask[None], page_size)[0]
+            pool, rows, page_size, query, k, v = _read_for_tree(kernels, cache, rows, query, k, v)
+        out = kernels.tree_attention(query[None], pool, rows[None], k[None], v[None], mask[None], page_size)[0]
+        return out.to(dtype)  # (over rows in 8 bits the output's one rounding)
 
 
-def _read_for_tree(kernels, cache, rows, k, v):
+def _read_for_tree(kernels, cache, rows, query, k, v):
     """What tree_attention takes of a cache whose rows are in 8 bits: the
     selected rows read back as a pool of one page, and the drafted keys and
-    values rounded as the cache will round them when they are appended (a
-    token accepted from a draft then sees what it would have seen alone)."""
-    form, dtype = cache.storage.rows8, k.dtype
-    n = rows.numel()
-    pool = torch.empty(1, 2, n, form.kv_heads, form.head_dim, dtype=dtype, device=k.device)
-    kernels.read_rows_8bit(cache.pool, form, rows, dtype, out=(pool[0, 0], pool[0, 1]))
+    values rounded as the cache will round them when they are appended. All of
+    it in fp32, where code * scale is what attend_8bit multiplies with: a
+    token accepted from a draft then sees what it would have seen alone, in a
+    16-bit model too (whose type would round every value once more, by up to
+    half a step of its own)."""
+    form, n = cache.storage.rows8, rows.numel()
+    pool = torch.empty(1, 2, n, form.kv_heads, form.head_dim, dtype=torch.float32, device=k.device)
+    kernels.read_rows_8bit(cache.pool, form, rows, torch.float32, out=(pool[0, 0], pool[0, 1]))
     own = torch.where(rows >= 0, torch.arange(n, device=rows.device), -1)
-    return pool, own, n, *kernels.round_8bit(k, v, form)
+    return pool, own, n, query.float(), *kernels.round_8bit(k.float(), v.float(), form)
