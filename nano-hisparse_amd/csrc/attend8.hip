@@ -14,6 +14,11 @@
 
 namespace nhs {
 
+// An element of a query, NaN in place of an infinity. With an infinity every
+// score is one too, or NaN, so the softmax is NaN; but where all of them are
+// minus infinity the sums below would read as those of a list without a row.
+__device__ __forceinline__ float query8(float x) { return x + (x - x); }
+
 struct Attend8Args {
   const void* q;
   int q_dtype;
@@ -59,7 +64,7 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int d = lane + i * kWave;
-    q[i] = d < D ? load_elem(a.q, a.q_dtype, (int64_t)b * a.q_bs + (int64_t)h * a.q_hs + d) : 0.f;
+    q[i] = d < D ? query8(load_elem(a.q, a.q_dtype, (int64_t)b * a.q_bs + (int64_t)h * a.q_hs + d)) : 0.f;
     acc[i] = 0.f;
   }
   const int64_t* list = a.rows + (int64_t)b * a.r_bs + (int64_t)h * a.r_hs;
@@ -313,6 +318,9 @@ __global__ __launch_bounds__(kF8Threads) void attend8_flash_kernel(Attend8Args a
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = load_elem(a.q, QP == 1 ? NHS_BF16 : QP == 2 ? NHS_F16 : NHS_F32, at + j);
     }
+    if constexpr (QP == 1)  // (in parts an infinity leaves NaN)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = query8(x[j]);
     f8_u32x4 parts[QP];
     f8_split<QP>(x, parts);
 #pragma unroll
