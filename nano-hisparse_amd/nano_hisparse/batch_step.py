@@ -75,6 +75,13 @@ class SparseDecodeBatch:
 
     def __init__(self, pool, host, tables: BatchTables, page_size, top_pages, keep_sink=True, chunks=1,
                  compute=None, transfer=None, form=None):
+        if form is not None:
+            rk._check_pool8("SparseDecodeBatch", pool, form)
+            if page_size != pool.shape[2] or host.dtype != pool.dtype or not host.is_contiguous() \
+                    or host.shape[1:] != pool.shape[1:]:
+                raise ValueError("SparseDecodeBatch: pool and host hold pages of page_size rows in 8 bits")
+        elif pool.ndim == 4:
+            raise ValueError("SparseDecodeBatch: a pool of rows in 8 bits needs its form")
         if pool.device.type != "cuda":
             raise ValueError("SparseDecodeBatch runs on a GPU")
         if not 1 <= chunks <= tables.batch:
