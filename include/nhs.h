@@ -603,9 +603,11 @@ int nhs_read_rows8(const void* pool, int64_t pool_rows, int64_t pool_block_strid
  * nhs_attend_rows over rows in 8 bits: out[b,h] = softmax_r(q[b,h] . K[r] *
  * head_dim^-0.5) . V[r] over the rows rows[b, h, c] in [0, pool_rows); zeros
  * for a head without any, else NaN for one whose query is not finite. Scores
- * and sums are fp32; query and out have q_dtype. The workspace (16-byte aligned; may be NULL where 0 bytes are
- * needed) holds anything before and after a call; calls that may overlap need
- * different ones.
+ * and sums are fp32, but for bf16 and fp16 queries the weights that multiply
+ * the values may have 16 bits (2^-17 of each lost; the sum that divides takes
+ * them whole); query and out have q_dtype. The workspace (16-byte aligned; may
+ * be NULL where 0 bytes are needed) holds anything before and after a call;
+ * calls that may overlap need different ones.
  */
 int64_t nhs_attend_rows8_workspace_bytes(int32_t batch, int32_t n_rows, int32_t q_heads, int32_t kv_heads,
                                          int32_t head_dim);

@@ -167,9 +167,9 @@ __global__ __launch_bounds__(kG8Threads) void attend8_general_kernel(Attend8Args
 //
 // The heads of a (request, split) are workgroups on one XCD (`near`): a head's
 // slice of a row begins at any multiple of 32 bytes, so neighbours share cache
-// lines, and all share those of the scales (spread over the XCDs: 36.5 us where
-// it takes 25.9). With fewer than 8 such groups the heads are spread instead,
-// over more of the XCDs.
+// lines, and all share those of the scales (spread over the XCDs: 16 x 2048 rows
+// 33.9 us where they take 21.9, 8 x 2048 21.0 where 15.2). With fewer than 8
+// such groups the heads are spread instead, over more of the XCDs.
 //
 // Heads that are no power of two run in the next larger D (PAD): chunks past
 // their dims are zeros, which add nothing to a score and to no one's output.
@@ -210,7 +210,8 @@ __device__ __forceinline__ uint32_t f8_round(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f8_f32x2){lo, hi}, f8_bf16x2));
 }
 
-// eight fp32 numbers as P bf16 operands whose sum they are
+// eight fp32 numbers as P bf16 operands: their sum with one part for bf16 numbers, two for fp16, three for fp32, else
+// near it (two parts of an fp32 weight lose up to 2^-17 of it; the denominator takes the weight as it was)
 template <int P>
 __device__ __forceinline__ void f8_split(float (&x)[8], f8_u32x4 (&out)[P]) {
 #pragma unroll
@@ -648,7 +649,8 @@ static int64_t workspace8(const Plan8& p, int64_t heads, int head_dim) {
 
 // depth: tiles of a wave's only round, or 0 for the loop over rounds. (A kernel of its own for a single round of two
 // tiles: 8 requests x 2048 rows of 32/8 heads 15.3 us against 15.7 in the loop, int8 15.9 against 15.4, fp32 16.0
-// against 15.3.)
+// against 15.3.) Padded heads have no four tiles: 16 requests x 2048 rows of 32/8 heads of 96 21.5 us with them and 20.7
+// in the loop, of 112 in int8 23.7 and 22.8, of 48 16.8 and 16.4.
 template <typename C, int QP, int D, bool PAD>
 static void (*flash8_deep(int depth))(Attend8Args) {
   constexpr int kRound = D == 256 ? 1 : 2;

@@ -418,7 +418,6 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
 // of them in flight (heads and units of a row by exact division).
 constexpr int kRead8 = 4;
 
-//
 // STREAM: past the caches. Whoever reads the outputs finds them there only if
 // they fit beside its own traffic; then the plain stores are better, else
 // these. us of a read, its rows not in a cache, and a copy of its outputs,
